@@ -442,6 +442,51 @@ int xqt_b200_peer_allgather_counted(const void* const* sources, void* const* fla
  * (convrot_w8a8_sm89_kernel.cu:756-837). */
 int xqt_b200_swiglu(const void* gate_up, void* output, int m, int inter, int dtype, xqt_b200_stream_t stream);
 
+/* RMS norm of query and key heads and the position rotation in one pass (no counterpart in the reference):
+ *   y = x * rsqrt(mean(x^2) + eps) * weight   where the weight is given (fp16 / bf16 / fp32 [dim]; null: y = x), then pair j of the
+ *   first `rotary` channels -- (j, j + rotary/2), interleaved: (2j, 2j+1) -- turned by positions[axes[j]][token] * frequencies[j]
+ *   radians; fp32 arithmetic, one rounding, the angle exact modulo a turn at any position.
+ * q [tokens, q_heads, dim], k [tokens, k_heads, dim] (k_heads 0: none) and their outputs with strides; an output may be its input.
+ * strides (host): token and head stride in elements of q, q_out, k, k_out (8 values, multiples of 8), then axis and token
+ * stride of positions.  positions: [axis_count, tokens] of int64 (wide_positions) or int32; frequencies: [rotary/2], device memory,
+ * reduced modulo a turn; axes: [rotary/2] or null (all 0), clamped to [0, axis_count).  dim <= 256 and rotary multiples of 16. */
+int xqt_b200_qk_norm_rope(const void* q, const void* k, void* q_out, void* k_out, const void* q_weight,
+                          const void* k_weight, const void* positions, const double* frequencies, const int* axes,
+                          const long long* strides, int tokens, int q_heads, int k_heads, int dim, int rotary,
+                          int axis_count, int wide_positions, int interleaved, int dtype, int weight_dtype, float eps,
+                          xqt_b200_stream_t stream);
+
+/* A paged cache of keys and values in 4 bits.  A vector of one token and head is held as codes c and a pair (scale s, minimum m) of
+ * the activation type T: m = min x, s = T((max x - min x) / 15) or 1 where that is 0, c = clamp(rint((x - m) / s), 0, 15); it stands
+ * for c * s + m.  A vector with an infinity or NaN gets s = m = NaN.
+ *   codes  uint8 [pages, 2 (key, value), heads, page_size, dim / 2], low nibble = even channel
+ *   params T     [pages, 2, heads, page_size, 2] = (s, m)
+ * dim 64, 128 or 256.  slots [tokens] (int64 with wide_slots, else int32): page * page_size + row of each token; a slot outside
+ * the cache is skipped (append) or read as zeros (gather).  The slots of one append are distinct.
+ * append: k, v [tokens, heads, dim]; strides (host): token and head stride of k, then of v, in elements, multiples of 8.
+ * gather: k_out, v_out [tokens, heads, dim] contiguous. */
+int xqt_b200_kv4_append(const void* k, const void* v, void* codes, void* params, const void* slots,
+                        const long long* strides, int tokens, int heads, int dim, long long pages, int page_size,
+                        int wide_slots, int dtype, xqt_b200_stream_t stream);
+int xqt_b200_kv4_gather(const void* codes, const void* params, const void* slots, void* k_out, void* v_out, int tokens,
+                        int heads, int dim, long long pages, int page_size, int wide_slots, int dtype,
+                        xqt_b200_stream_t stream);
+
+/* Attention over that cache: out = softmax(scale * q K^T + mask) V, q and out [tokens, q_heads, dim] (out contiguous), q_heads a
+ * multiple of kv_heads (consecutive query heads share a key head).  Sequence b has the query rows
+ * query_starts[b] .. query_starts[b+1] (null: row b, tokens == batch), which are its last tokens, and seq_lens[b] keys, key i in
+ * row i % page_size of page table[b][i / page_size] (table [batch, table_width], int32, row stride strides[2]).  A query sees the keys up
+ * to its own position, with window > 0 only the last `window` of them; keys of a page number outside [0, pages) are not seen; a row that
+ * sees nothing is 0; lengths and starts are clamped to the table and to `tokens`; rows of no sequence are not written.
+ * page_size: a power of two, 16 to 4096.  strides (host): token and head stride of q in elements (multiples of 8), row stride of
+ * table.  Workspace of the given size, 16-byte aligned, any contents, not shared with a call that may overlap. */
+size_t xqt_b200_kv4_attention_workspace_bytes(int dim);
+int xqt_b200_kv4_attention(const void* q, const void* codes, const void* params, const int* table, const int* seq_lens,
+                           const int* query_starts, void* out, const long long* strides, int tokens, int batch,
+                           int q_heads, int kv_heads, int dim, long long pages, int page_size, int table_width,
+                           int window, int dtype, float scale, void* workspace, size_t workspace_bytes,
+                           unsigned int* status, xqt_b200_stream_t stream);
+
 /* Copies the status word of `workspace` to *host_status (host pointer) and synchronises `stream`.
  * No counterpart in the reference, whose kernels have no device-side waits. */
 int xqt_b200_workspace_status(const void* workspace, unsigned int* host_status,

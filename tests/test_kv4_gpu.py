@@ -1,0 +1,339 @@
+"""The 4-bit paged cache and attention over it, against the definitions in 64 bits."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from attention_reference import attention, pack, quantize, values
+from conftest import seeded
+from xqt_b200 import native
+from xqt_b200.errors import XQTBackendError
+from xqt_b200.ops.kv4 import allocate_kv4_cache, kv4_append, kv4_attention, kv4_gather
+
+pytestmark = pytest.mark.gpu
+DEVICE = torch.device("cuda", 0)
+NAN, INF = float("nan"), float("inf")
+
+
+def _vectors(tokens, heads, dim, dtype, seed, size=1.0):
+    return (torch.randn((tokens, heads, dim), generator=seeded(seed)) * size).to(dtype)
+
+
+# ---------------------------------------------------------------- writing and reading
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("wide", [torch.int32, torch.int64])
+@pytest.mark.parametrize("tokens,heads,dim,page", [(1, 1, 64, 16), (5, 3, 128, 32), (67, 2, 256, 16), (1000, 8, 128, 64), (31, 5, 64, 4096)])
+def test_append_and_gather(dtype, wide, tokens, heads, dim, page):
+    pages = tokens // page + 3
+    k, v = _vectors(tokens, heads, dim, dtype, 1), _vectors(tokens, heads, dim, dtype, 2, 30.0)
+    v[0, 0] = 3.0                                     # a constant vector: scale 1, codes 0
+    codes, params = allocate_kv4_cache(pages, heads, dim, page_size=page, dtype=dtype, device=DEVICE)
+    codes.fill_(0xA5)
+    slots = torch.randperm(pages * page, generator=seeded(3))[:tokens].to(wide)
+    want_codes, want_params = codes.cpu(), params.cpu()
+    for i, x in enumerate((k, v)):
+        c, s, m = quantize(x)
+        want_codes[slots.long() // page, i, :, slots.long() % page] = pack(c)
+        want_params[slots.long() // page, i, :, slots.long() % page] = torch.stack((s, m), -1)
+    kv4_append(k.to(DEVICE), v.to(DEVICE), codes, params, slots.to(DEVICE))
+    assert torch.equal(codes.cpu(), want_codes) and torch.equal(params.cpu(), want_params)
+    got = kv4_gather(codes, params, slots.to(DEVICE))
+    for i in (0, 1):
+        held = values(want_codes[slots.long() // page, i, :, slots.long() % page], want_params[slots.long() // page, i, :, slots.long() % page])
+        # code * scale is exact in fp32, so the sum is rounded once to fp32 and once to the type
+        assert torch.equal(got[i].cpu(), held.float().to(dtype))
+
+
+def test_append_of_strided_vectors_and_padded_rows():
+    fused = _vectors(9, 2 + 2 * 2, 128, torch.bfloat16, 4).to(DEVICE)
+    codes, params = allocate_kv4_cache(2, 2, 128, page_size=16, device=DEVICE)
+    other = [t.clone() for t in (codes, params)]
+    slots = torch.tensor([3, -1, 31, 32, 0, 7, -5, 1 << 40, 30], device=DEVICE)
+    keep = torch.tensor([0, 2, 4, 5, 8], device=DEVICE)
+    k, v = fused[:, 2:4], fused[:, 4:]
+    kv4_append(k, v, codes, params, slots)
+    kv4_append(k[keep].contiguous(), v[keep].contiguous(), *other, slots[keep])
+    assert torch.equal(codes, other[0]) and torch.equal(params, other[1])
+    shifted = torch.empty((9, 2, 131), dtype=torch.bfloat16, device=DEVICE)[:, :, 1:129]
+    shifted.copy_(k)
+    again = [torch.zeros_like(t) for t in (codes, params)]
+    kv4_append(shifted, v, *again, slots)
+    assert torch.equal(codes, again[0]) and torch.equal(params, again[1])
+    got = kv4_gather(codes, params, slots)
+    assert all(bool((x[[1, 3, 6, 7]] == 0).all()) for x in got) and bool((got[0][0] != 0).any())
+
+
+def test_vectors_that_are_not_finite():
+    x = _vectors(5, 1, 64, torch.bfloat16, 5)
+    x[1, 0, 3], x[2, 0, 9], x[3, 0, 0] = NAN, INF, -INF
+    x[4, 0, 0], x[4, 0, 1] = 3.3e38, -3.3e38           # the range overflows
+    codes, params = allocate_kv4_cache(1, 1, 64, page_size=16, device=DEVICE)
+    codes.fill_(255)
+    kv4_append(x.to(DEVICE), x.to(DEVICE), codes, params, torch.arange(5, device=DEVICE))
+    c, s, m = quantize(x)
+    assert torch.equal(codes[0, 0, 0, :5].cpu(), pack(c)[:, 0]) and bool((codes[0, :, 0, 1:5] == 0).all())
+    assert bool(torch.isnan(params[0, :, 0, 1:5]).all()) and torch.equal(params[0, 1, 0, 0].cpu(), torch.stack((s, m), -1)[0, 0])
+    assert bool(torch.isnan(kv4_gather(codes, params, torch.arange(1, 5, device=DEVICE))[1]).all())
+
+
+def test_nothing_to_append():
+    codes, params = allocate_kv4_cache(1, 2, 64, page_size=16, device=DEVICE)
+    empty = torch.empty((0, 2, 64), dtype=torch.bfloat16, device=DEVICE)
+    kv4_append(empty, empty, codes, params, torch.empty(0, dtype=torch.int64, device=DEVICE))
+    assert kv4_gather(codes, params, torch.empty(0, dtype=torch.int32, device=DEVICE))[0].shape == (0, 2, 64)
+    none = allocate_kv4_cache(0, 2, 64, page_size=16, device=DEVICE)
+    kv4_append(torch.ones((1, 2, 64), dtype=torch.bfloat16, device=DEVICE), torch.ones((1, 2, 64), dtype=torch.bfloat16, device=DEVICE), *none,
+               torch.zeros(1, dtype=torch.int64, device=DEVICE))
+    assert bool((kv4_gather(*none, torch.zeros(1, dtype=torch.int64, device=DEVICE))[0] == 0).all())
+
+
+# ---------------------------------------------------------------- attention
+
+def make_cache(lens, heads, dim, page, dtype, seed, spare=2, size=1.0):
+    """A cache whose pages hold random vectors in random order, unused rows NaN, and its table."""
+
+    per = [-(-n // page) for n in lens]
+    pages = sum(per) + spare
+    gen = seeded(seed)
+    x = (torch.randn((pages, 2, heads, page, dim), generator=gen) * size).to(dtype)
+    c, s, m = quantize(x)
+    codes, params = pack(c), torch.stack((s, m), -1)
+    order = torch.randperm(pages, generator=gen).to(torch.int32)
+    table = torch.full((len(lens), max(max(per, default=0), 1) + 1), -1, dtype=torch.int32)
+    at, unused = 0, torch.ones(pages, page, dtype=torch.bool)
+    for b, n in enumerate(per):
+        ids = order[at:at + n]
+        table[b, :n] = ids
+        at += n
+        for i, p in enumerate(ids.tolist()):
+            unused[p, :min(page, lens[b] - i * page)] = False
+    params.permute(0, 3, 1, 2, 4)[unused] = NAN
+    return codes.to(DEVICE), params.to(DEVICE), table.to(DEVICE)
+
+
+def check(q, codes, params, table, lens, counts=None, rounded=None, **options):
+    seq_lens = torch.tensor(lens, dtype=torch.int32)
+    starts = None if counts is None else torch.tensor([sum(counts[:b]) for b in range(len(counts) + 1)], dtype=torch.int32)
+    got = kv4_attention(q.to(DEVICE), codes, params, table, seq_lens.to(DEVICE), query_starts=None if starts is None else starts.to(DEVICE), **options)
+    want, bound = attention(q, codes, params, table, seq_lens, starts, rounded=rounded, **options)
+    got = got.cpu().double()
+    rows = ~torch.isnan(want).all(-1).all(-1)
+    assert bool(torch.isfinite(got[rows]).all())
+    over = (got - want).abs()[rows] - bound[rows]
+    assert bool((over <= 0).all()), f"{float(over.max())} over a bound of {float(bound[rows].max())}"
+    assert native.workspace_status(DEVICE) == 0
+    return got
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,each,dim,page", [(1, 1, 64, 16), (2, 4, 128, 64), (8, 4, 128, 16), (2, 8, 64, 32), (1, 16, 128, 128), (3, 5, 128, 32),
+                                                 (2, 7, 256, 64), (1, 12, 256, 16), (1, 33, 64, 64)])
+@pytest.mark.parametrize("lens", [[1], [0, 2, 17, 64, 65, 300], [777]])
+def test_single_tokens(dtype, heads, each, dim, page, lens):
+    codes, params, table = make_cache(lens, heads, dim, page, dtype, 11)
+    check(_vectors(len(lens), heads * each, dim, dtype, 12), codes, params, table, lens)
+
+
+@pytest.mark.parametrize("lens,heads,each,dim,page", [([20000], 1, 4, 128, 64), ([4096, 1, 9000, 0, 513], 2, 8, 64, 16), ([5000, 3001], 2, 1, 256, 128)])
+def test_long_contexts_split_over_the_gpu(lens, heads, each, dim, page):
+    codes, params, table = make_cache(lens, heads, dim, page, torch.bfloat16, 13)
+    check(_vectors(len(lens), heads * each, dim, torch.bfloat16, 14), codes, params, table, lens)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,each,dim,page", [(2, 4, 128, 64), (1, 3, 64, 16), (1, 2, 256, 32), (2, 1, 128, 16)])
+@pytest.mark.parametrize("window", [None, 1, 33, 100])
+def test_a_few_queries_of_each_sequence(dtype, heads, each, dim, page, window):
+    lens, counts = [5, 40, 300, 129, 7], [5, 3, 7, 0, 1]
+    codes, params, table = make_cache(lens, heads, dim, page, dtype, 15)
+    check(_vectors(sum(counts), heads * each, dim, dtype, 16), codes, params, table, lens, counts, window=window)
+
+
+def test_more_queries_than_keys_and_other_scale():
+    lens, counts = [3, 0, 40], [6, 2, 41]
+    codes, params, table = make_cache(lens, 2, 64, 16, torch.float16, 17)
+    got = check(_vectors(sum(counts), 4, 64, torch.float16, 18), codes, params, table, lens, counts, scale=0.3)
+    assert bool((got[:3] == 0).all()) and bool((got[6:9] == 0).all()) and bool((got[3:6] != 0).any())
+
+
+@pytest.mark.parametrize("window", [1, 63, 64, 1000, 2 ** 31 - 1])
+def test_window_of_single_tokens(window):
+    lens = [1, 63, 64, 65, 2000]
+    codes, params, table = make_cache(lens, 2, 128, 32, torch.bfloat16, 19)
+    check(_vectors(5, 8, 128, torch.bfloat16, 20), codes, params, table, lens, window=window)
+
+
+def test_large_values_and_sharp_rows():
+    """Scores far apart (one key takes all), values of very different scales, tiny and huge queries."""
+
+    lens = [500, 500, 500]
+    codes, params, table = make_cache(lens, 2, 128, 64, torch.bfloat16, 21, size=4.0)
+    params[:, 1, :, ::7] *= 1e-4
+    params[:, 1, :, 3::7] *= 1e4
+    q = _vectors(3, 8, 128, torch.bfloat16, 22)
+    q[0] *= 50
+    q[1] *= 1e-6
+    q[2, 3] = 0
+    check(q, codes, params, table, lens)
+
+
+def test_zero_and_negative_scales_are_arithmetic():
+    lens = [130]
+    codes, params, table = make_cache(lens, 1, 64, 16, torch.float16, 23)
+    params[:, 1, :, ::3, 0] = 0
+    params[:, 1, :, 1::3, 0] *= -1
+    q = _vectors(1, 2, 64, torch.float16, 24)
+    check(q, codes, params, table, lens)
+
+
+def test_empty_cache_reads_zeros():
+    codes, params = allocate_kv4_cache(3, 2, 64, page_size=16, device=DEVICE)
+    table = torch.arange(2, dtype=torch.int32, device=DEVICE).reshape(1, 2)
+    got = kv4_attention(_vectors(1, 2, 64, torch.bfloat16, 25).to(DEVICE), codes, params, table, torch.tensor([20], dtype=torch.int32, device=DEVICE))
+    assert bool((got == 0).all())
+
+
+def test_pages_that_are_not_there():
+    """Numbers outside the cache hide their keys; lengths past the table and starts outside the rows are cut."""
+
+    lens = [100, 200, 64]
+    codes, params, table = make_cache(lens, 2, 128, 16, torch.float16, 26)
+    table[0, 2], table[1, 0], table[1, 5] = -1, codes.shape[0], 2 ** 31 - 1
+    table[2] = -7
+    got = check(_vectors(3, 4, 128, torch.float16, 27), codes, params, table, lens)
+    assert bool((got[2] == 0).all())
+    check(_vectors(3, 4, 128, torch.float16, 28), codes, params, table, [100, 10 ** 9, -5])
+    q = _vectors(6, 4, 128, torch.float16, 29)
+    starts = torch.tensor([-3, 2, 1, 99], dtype=torch.int32, device=DEVICE)         # clamped: rows 0-1, none, 1-5 (not ascending: row 1 is anyone's)
+    out = kv4_attention(q.to(DEVICE), codes, params, table, torch.tensor([100, 200, 64], dtype=torch.int32, device=DEVICE), query_starts=starts)
+    assert bool((out[2:] == 0).all()) and bool((out[0] != 0).any())        # the third sequence's pages are none
+
+
+def test_rows_of_no_sequence_stay():
+    lens = [50, 20]
+    codes, params, table = make_cache(lens, 1, 64, 16, torch.bfloat16, 30)
+    q = _vectors(9, 2, 64, torch.bfloat16, 31).to(DEVICE)
+    out = torch.full_like(q, 7.0)
+    starts = torch.tensor([2, 4, 5], dtype=torch.int32, device=DEVICE)
+    seq_lens = torch.tensor(lens, dtype=torch.int32, device=DEVICE)
+    got = kv4_attention(q, codes, params, table, seq_lens, query_starts=starts, out=out)
+    assert got.data_ptr() == out.data_ptr() and bool((out[:2] == 7).all()) and bool((out[5:] == 7).all()) and not bool((out[2:5] == 7).any())
+    first = kv4_attention(q[2:5], codes, params, table, seq_lens, query_starts=starts - 2)
+    assert torch.equal(first, out[2:5])
+
+
+@pytest.mark.parametrize("counts", [None, [3, 2]])
+def test_infinities_and_nan_in_hidden_places(counts):
+    lens = [70, 90]
+    codes, params, table = make_cache(lens, 1, 128, 16, torch.bfloat16, 32)
+    q = _vectors(2 if counts is None else 5, 4, 128, torch.bfloat16, 33)
+    if counts is not None:      # the last key of sequence 0 is NaN, its values infinite: only its last query sees them
+        page, row = int(table[0, 69 // 16]), 69 % 16
+        params[page, 0, 0, row] = NAN
+        params[page, 1, 0, row] = INF
+        clean = [t.clone() for t in (codes, params)]
+        clean[1][page, :, 0, row] = 1.0
+        seq_lens, starts = (torch.tensor(x, dtype=torch.int32, device=DEVICE) for x in (lens, [0, 3, 5]))
+        got = kv4_attention(q.to(DEVICE), codes, params, table, seq_lens, query_starts=starts)
+        want = kv4_attention(q.to(DEVICE), *clean, table, seq_lens, query_starts=starts)
+        keep = [0, 1, 3, 4]
+        assert torch.equal(got[keep], want[keep]) and bool(torch.isnan(got[2]).all())
+    else:                       # outside a window
+        params[int(table[0, 0]), :, 0, 3] = NAN
+        params[int(table[1, 1]), :, 0, 0] = INF
+        check(q, codes, params, table, lens, window=20)
+    q[0, 1, 7] = INF            # a query that is not finite spoils its own row only
+    seq_lens = torch.tensor(lens, dtype=torch.int32, device=DEVICE)
+    if counts is None:
+        got = kv4_attention(q.to(DEVICE), codes, params, table, seq_lens, window=20)
+        assert bool(torch.isfinite(got[0, [0, 2, 3]]).all()) and bool(torch.isfinite(got[1]).all())
+
+
+def test_strided_queries_and_tables():
+    lens = [40, 90]
+    codes, params, table = make_cache(lens, 2, 64, 16, torch.float16, 34)
+    fused = _vectors(2, 8, 64, torch.float16, 35).to(DEVICE)
+    seq_lens = torch.tensor(lens, dtype=torch.int32, device=DEVICE)
+    want = kv4_attention(fused[:, :4].contiguous(), codes, params, table, seq_lens)
+    wide = torch.full((2, table.shape[1] + 5), -1, dtype=torch.int32, device=DEVICE)
+    wide[:, :table.shape[1]] = table
+    assert torch.equal(kv4_attention(fused[:, :4], codes, params, wide[:, :table.shape[1]], seq_lens), want)
+    turned = fused[:, :4].transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(kv4_attention(turned, codes, params, table, seq_lens), want)
+    odd = torch.empty((2, 4, 67), dtype=torch.float16, device=DEVICE)[:, :, 3:]
+    odd.copy_(fused[:, :4])
+    assert torch.equal(kv4_attention(odd, codes, params, table, seq_lens), want)
+
+
+def test_no_sequences_and_no_pages():
+    codes, params = allocate_kv4_cache(0, 2, 64, page_size=16, device=DEVICE)
+    q = torch.ones((0, 4, 64), dtype=torch.bfloat16, device=DEVICE)
+    none = torch.empty(0, dtype=torch.int32, device=DEVICE)
+    assert kv4_attention(q, codes, params, none.reshape(0, 3), none).shape == (0, 4, 64)
+    one = torch.ones((1, 4, 64), dtype=torch.bfloat16, device=DEVICE)
+    got = kv4_attention(one, codes, params, torch.zeros((1, 3), dtype=torch.int32, device=DEVICE), torch.tensor([33], dtype=torch.int32, device=DEVICE))
+    assert bool((got == 0).all())
+    got = kv4_attention(one, codes, params, torch.zeros((1, 0), dtype=torch.int32, device=DEVICE), torch.tensor([33], dtype=torch.int32, device=DEVICE))
+    assert bool((got == 0).all())
+
+
+def test_same_bits_every_time():
+    lens = [900, 33, 2100, 1, 640] * 3
+    codes, params, table = make_cache(lens, 4, 128, 64, torch.bfloat16, 36)
+    q = _vectors(len(lens), 16, 128, torch.bfloat16, 37).to(DEVICE)
+    seq_lens = torch.tensor(lens, dtype=torch.int32, device=DEVICE)
+    first = kv4_attention(q, codes, params, table, seq_lens)
+    for _ in range(5):
+        assert torch.equal(kv4_attention(q, codes, params, table, seq_lens), first)
+
+
+def test_two_streams_and_two_captured_graphs():
+    lens = [3000, 1200]
+    codes, params, table = make_cache(lens, 2, 128, 64, torch.float16, 38)
+    seq_lens = torch.tensor(lens, dtype=torch.int32, device=DEVICE)
+    qs = [_vectors(2, 8, 128, torch.float16, 39 + i).to(DEVICE) for i in range(2)]
+    want = [kv4_attention(q, codes, params, table, seq_lens) for q in qs]
+    graphs, held = [], []
+    for q in qs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held.append(kv4_attention(q, codes, params, table, seq_lens))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(held, want))
+    got = [None, None]
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i] = kv4_attention(qs[i], codes, params, table, seq_lens)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    seq_lens.copy_(torch.tensor([7, 2900], dtype=torch.int32))          # lengths live on the device
+    table[1, : table.shape[1] - 1] = table[0, : table.shape[1] - 1]
+    for graph in graphs:
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, kv4_attention(q, codes, params, table, seq_lens)) for a, q in zip(held, qs))
+
+
+def test_many_short_sequences():
+    lens = [(7 * i) % 50 for i in range(700)]
+    codes, params, table = make_cache(lens, 1, 64, 16, torch.float16, 41)
+    check(_vectors(len(lens), 2, 64, torch.float16, 42), codes, params, table, lens)
+
+
+def test_out_is_checked():
+    codes, params = allocate_kv4_cache(1, 2, 64, page_size=16, device=DEVICE)
+    q = torch.ones((1, 4, 64), dtype=torch.bfloat16, device=DEVICE)
+    table, seq_lens = torch.zeros((1, 1), dtype=torch.int32, device=DEVICE), torch.ones(1, dtype=torch.int32, device=DEVICE)
+    for bad in (q.half(), torch.ones((2, 4, 64), dtype=torch.bfloat16, device=DEVICE), torch.ones((1, 4, 128), dtype=torch.bfloat16, device=DEVICE)[..., ::2]):
+        with pytest.raises(XQTBackendError, match="out"):
+            kv4_attention(q, codes, params, table, seq_lens, out=bad)

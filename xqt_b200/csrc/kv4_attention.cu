@@ -1,0 +1,743 @@
+// Attention of few queries over a paged cache of keys and values in 4 bits (layout: kv4_cache.cu).
+//
+//   out = softmax(scale * q K^T + mask) V,   K, V = code * s + m  per (token, head)
+//
+// The queries of a sequence are its last tokens; query i sees the keys up to its own position, with a window only the last
+// `window` of them.  A row that sees nothing is 0.
+//
+// Neither K nor V is ever formed.  The matrix instructions (mma.sync m16n8k16, fp16 operands, fp32 sums) run on the codes themselves: a
+// nibble in the low bits of a half is the subnormal c * 2^-24, so one AND per two codes makes an operand, and
+//   q . K_t = s_t * sum(c q) + m_t * sum(q)          P V = sum((p_t s_t) c) + sum(p_t m_t)
+// puts scales and minima on the scores and on the probabilities.  Queries are scaled by a power of two per row so that fp16 holds them
+// to 2^-12 of each element down to 2^-26 of the row's largest; p_t s_t is rounded to fp16 against a running power of two above the scales, with
+// 2^15 of headroom, so nothing underflows; softmax statistics and all sums are fp32.
+//
+// The keys are the 16-row operand and the queries the 8-column one (transposed products), so that eight rows -- the query heads of
+// one key head -- fill a tile.  Work is cut into units of W chunks of CT keys (a chunk per warp); the units of all (sequence, row tile,
+// head) items form one list, of which each CTA takes an equal contiguous share whatever the lengths are; items that
+// CTAs share are joined by a second kernel.  Each warp fetches its own chunks with bulk copies, S of them ahead.
+//
+// Bound by HBM: (dim + 8) bytes per key and head.
+#include <math_constants.h>
+
+#include "common.cuh"
+#include "sm100.cuh"
+
+namespace xqt_b200 {
+
+namespace {
+
+using namespace sm100;
+
+struct AttnArgs {
+  const void* q;
+  const uint8_t* codes;
+  const uint8_t* params;
+  const int* table;
+  const int* seq_lens;
+  const int* query_starts;   // null: one query per sequence
+  void* out;
+  float* part_o;             // [2 * CTAs][ROWS][D]
+  float2* part_ml;           // [2 * CTAs][ROWS]
+  unsigned* status;
+  long long q_token, q_head, pages, table_stride;
+  int tokens, batch, q_heads, kv_heads, each, page_size, page_shift, table_width, window;
+  float scale;               // times log2(e)
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ float2 pair_of(uint32_t bits) {
+  const T* e = reinterpret_cast<const T*>(&bits);
+  return make_float2(to_float<T>(e[0]), to_float<T>(e[1]));
+}
+
+template <int D_, int NT_, int W_, int CT_, int S_>
+struct Shape {
+  static constexpr int D = D_, NT = NT_, W = W_, CT = CT_, S = S_;
+  static constexpr int ROWS = 8 * NT, KROW = D / 2, KWORDS = D / 32, VWORDS = D / 64, MT = CT / 16;
+  static constexpr int UNIT = W * CT;
+  static constexpr int CODE_BYTES = CT * KROW, PARAM_BYTES = CT * 4, STAGE = 2 * (CODE_BYTES + PARAM_BYTES);
+  static constexpr int MERGE_ROW = D + 4;
+  static constexpr int MERGE_BYTES = W * ROWS * MERGE_ROW * 4, STAT_BYTES = W * ROWS * 16;
+  static constexpr int SMEM = W * S * STAGE + MERGE_BYTES + STAT_BYTES + W * S * 8;
+};
+
+// A sequence as the work list sees it.
+struct Sequence {
+  int q0, nq, len, first, tiles, units;   // `first`: where its units start; units per (tile, head) item
+};
+
+template <int ROWS, int UNIT, int CT>
+__device__ __forceinline__ Sequence sequence(const AttnArgs& a, int b) {
+  Sequence s;
+  if (a.query_starts) {
+    const int lo = min(max(a.query_starts[b], 0), a.tokens);
+    s.q0 = lo;
+    s.nq = min(max(a.query_starts[b + 1], lo), a.tokens) - lo;
+  } else {
+    s.q0 = b;
+    s.nq = 1;
+  }
+  const long long most = (long long)a.table_width << a.page_shift;
+  s.len = (int)min((long long)max(a.seq_lens[b], 0), most);
+  const long long from = a.window ? (long long)s.len - s.nq + 1 - a.window : 0;
+  s.first = from > 0 ? (int)(from / CT * CT) : 0;
+  s.tiles = (int)(((long long)s.nq * a.each + ROWS - 1) / ROWS);
+  s.units = max((s.len - s.first + UNIT - 1) / UNIT, 1);   // an empty sequence still has its rows written
+  return s;
+}
+
+// All units, and the place of unit `u` in the list; every warp does it for itself.
+struct Walk {
+  int b, tile, head, unit;
+  Sequence s;
+};
+
+template <int ROWS, int UNIT, int CT>
+__device__ __forceinline__ long long count_units(const AttnArgs& a, int lane) {
+  long long sum = 0;
+  for (int b = lane; b < a.batch; b += 32) {
+    const Sequence s = sequence<ROWS, UNIT, CT>(a, b);
+    sum += (long long)s.tiles * a.kv_heads * s.units;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
+}
+
+// by_item: `u` counts items (tile, head) and not units; `before` gets the units in front of the item then
+template <int ROWS, int UNIT, int CT>
+__device__ __forceinline__ bool place(const AttnArgs& a, int lane, long long u, bool by_item, Walk& w, long long& before) {
+  long long base = 0, base_units = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 32) {
+    long long n = 0, units = 0;
+    if (b0 + lane < a.batch) {
+      const Sequence s = sequence<ROWS, UNIT, CT>(a, b0 + lane);
+      n = (long long)s.tiles * a.kv_heads;
+      units = n * s.units;
+    }
+    long long cum_units = units;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, cum_units, o);
+      if (lane >= o) cum_units += y;
+    }
+    long long cum = cum_units;
+    if (by_item) {
+      cum = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, cum, o);
+        if (lane >= o) cum += x;
+      }
+    } else {
+      n = units;
+    }
+    const unsigned over = __ballot_sync(0xffffffffu, base + cum > u);
+    if (over) {
+      const int at = __ffs(over) - 1;
+      const long long rest = u - base - __shfl_sync(0xffffffffu, cum - n, at);
+      w.b = b0 + at;
+      w.s = sequence<ROWS, UNIT, CT>(a, w.b);
+      const long long item = by_item ? rest : rest / w.s.units;
+      w.unit = by_item ? 0 : (int)(rest - item * w.s.units);
+      w.tile = (int)(item / a.kv_heads);
+      w.head = (int)(item - (long long)w.tile * a.kv_heads);
+      before = base_units + __shfl_sync(0xffffffffu, cum_units - units, at) + item * w.s.units;
+      return true;
+    }
+    base += __shfl_sync(0xffffffffu, cum, 31);
+    base_units += __shfl_sync(0xffffffffu, cum_units, 31);
+  }
+  return false;
+}
+
+template <int ROWS, int UNIT, int CT>
+__device__ __forceinline__ void advance(const AttnArgs& a, Walk& w) {
+  if (++w.unit < w.s.units) return;
+  w.unit = 0;
+  if (++w.head < a.kv_heads) return;
+  w.head = 0;
+  if (++w.tile < w.s.tiles) return;
+  w.tile = 0;
+  while (++w.b < a.batch) {
+    w.s = sequence<ROWS, UNIT, CT>(a, w.b);
+    if (w.s.tiles > 0) return;
+  }
+}
+
+__device__ __forceinline__ long long share(long long units, int i, int n) { return units * i / n; }
+
+template <typename T, typename SH>
+__global__ void __launch_bounds__(SH::W * 32) kv4_attention_kernel(const AttnArgs a) {
+  constexpr int D = SH::D, NT = SH::NT, W = SH::W, CT = SH::CT, S = SH::S, ROWS = SH::ROWS, MT = SH::MT, KROW = SH::KROW;
+  constexpr int KWORDS = SH::KWORDS, VWORDS = SH::VWORDS;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  uint8_t* const ring = smem + warp * (S * SH::STAGE);
+  float* const merge = reinterpret_cast<float*>(smem + W * S * SH::STAGE);
+  float4* const stats = reinterpret_cast<float4*>(smem + W * S * SH::STAGE + SH::MERGE_BYTES);
+  const uint32_t bars = smem_addr(smem + W * S * SH::STAGE + SH::MERGE_BYTES + SH::STAT_BYTES) + warp * (S * 8);
+  if (lane == 0) {
+    for (int s = 0; s < S; ++s) mbar_init(bars + 8 * s, 1);
+    fence_barrier_init();
+  }
+  __syncwarp();
+  grid_launch_dependents();
+  grid_dependency_wait();
+
+  const long long total = count_units<ROWS, SH::UNIT, CT>(a, lane);
+  const long long u0 = share(total, blockIdx.x, gridDim.x), u1 = share(total, blockIdx.x + 1, gridDim.x);
+  if (u0 >= u1) return;
+  Walk c;
+  long long unused;
+  if (!place<ROWS, SH::UNIT, CT>(a, lane, u0, false, c, unused)) return;
+
+  // ---- fetching
+  const int psz = min(a.page_size, CT), pieces = CT / psz;
+  const int piece = lane >> 2, kind = lane & 3;                      // kind: key codes, value codes, key parameters, value parameters
+  const int row_bytes = kind < 2 ? KROW : 4;
+  const uint8_t* const source = (kind < 2 ? a.codes : a.params) + (kind & 1) * ((long long)a.kv_heads * a.page_size * row_bytes);
+  const long long page_bytes = 2LL * a.kv_heads * a.page_size * row_bytes;
+  const uint32_t target = smem_addr(ring) + (kind == 0 ? 0 : kind == 1 ? SH::CODE_BYTES : kind == 2 ? 2 * SH::CODE_BYTES : 2 * SH::CODE_BYTES + SH::PARAM_BYTES) +
+                          piece * psz * row_bytes;
+  Walk f = c;
+  long long to_fetch = u1 - u0;
+  int next_page = -1, next_row = 0;
+  uint32_t masks = 0, phases = 0;
+  bool dead = false;
+  // the table entry of the next chunk to fetch, asked for one chunk ahead of its use
+  auto look_up = [&]() {
+    next_page = -1;
+    if (to_fetch > 0) {
+      const int tok0 = f.s.first + (f.unit * W + warp) * CT;
+      const int at = tok0 + piece * psz;
+      const int j0 = f.tile * ROWS / a.each, j1 = min(f.s.nq - 1, (f.tile * ROWS + ROWS - 1) / a.each);
+      const int last = f.s.len - f.s.nq + j1;
+      const long long lowest = a.window ? (long long)f.s.len - f.s.nq + j0 - a.window + 1 : 0;
+      if (piece < pieces && at < f.s.len && tok0 <= last && tok0 + CT > lowest) {
+        const int page = a.table[f.b * a.table_stride + (at >> a.page_shift)];
+        next_page = page >= 0 && page < a.pages ? page : -1;
+      }
+      next_row = f.head * a.page_size + (at & (a.page_size - 1));
+      --to_fetch;
+      if (to_fetch > 0) advance<ROWS, SH::UNIT, CT>(a, f);
+    }
+  };
+  auto issue = [&](int stage) {
+    const bool valid = next_page >= 0 && !dead;
+    const unsigned votes = __ballot_sync(0xffffffffu, valid);
+    unsigned mask = 0;
+#pragma unroll
+    for (int p = 0; p < MT; ++p) mask |= (votes >> (4 * p) & 1u) << p;
+    masks = (masks & ~(15u << (4 * stage))) | mask << (4 * stage);
+    if (mask) {
+      const uint32_t bar = bars + 8 * stage;
+      if (lane == 0) mbar_expect_tx(bar, (uint32_t)(__popc(mask) * psz * 2 * (KROW + 4)));
+      __syncwarp();
+      if (valid) bulk_g2s(target + stage * SH::STAGE, source + next_page * page_bytes + (long long)next_row * row_bytes, (uint32_t)(psz * row_bytes), bar);
+    }
+  };
+#pragma unroll 1
+  for (int s = 0; s < S; ++s) {
+    look_up();
+    issue(s);
+  }
+  look_up();
+
+  // ---- one item's state
+  uint32_t qf[NT][2 * KWORDS][2];
+  float qa[NT][2], qb[NT][2];
+  int hi[NT][2];
+  long long lo[NT][2];
+  float o[VWORDS * 4][NT][4];
+  float mx[NT][2], l[NT][2], lm[NT][2], sigma = 0.0f, inv_sigma = 0.0f;
+  int full_hi = 0;
+  long long full_lo = 0;
+
+  auto start_item = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      // as the operand wants it: row g of this 8-column tile, the channels that go with this lane's key words
+      const int r = c.tile * ROWS + nt * 8 + g;
+      const int j = r / a.each;
+      const bool real = j < c.s.nq;
+      const T* src = reinterpret_cast<const T*>(a.q) + (long long)(c.s.q0 + (real ? j : 0)) * a.q_token + (long long)(c.head * a.each + r - j * a.each) * a.q_head;
+      uint4 raw[KWORDS];
+      float top = 0.0f;
+#pragma unroll
+      for (int w = 0; w < KWORDS; ++w) {
+        const int ch = D <= 128 ? t * (D / 4) + 8 * w : 128 * (w >> 2) + 32 * t + 8 * (w & 3);
+        raw[w] = real ? *reinterpret_cast<const uint4*>(src + ch) : make_uint4(0, 0, 0, 0);
+        const T* e = reinterpret_cast<const T*>(&raw[w]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(to_float<T>(e[i])));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // the power of two that brings the largest to [2^12, 2^13)
+      const int e = top > 0.0f && top <= 3.402823466e38f ? min(max((int)(__float_as_uint(top) >> 23) - 127 - 12, -110), 110) : 0;
+      const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < KWORDS; ++w) {
+        const T* x = reinterpret_cast<const T*>(&raw[w]);
+        __half h[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          h[i] = __float2half_rn(to_float<T>(x[i]) * down);
+          sum += __half2float(h[i]);
+        }
+        // nibbles 0,4 | 1,5 | 2,6 | 3,7 of a word; the odd ones stand 16 times too high in their operand
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float by = i & 1 ? 0.0625f : 1.0f;
+          qf[nt][2 * w + (i >> 1)][i & 1] = pack_half2(__half2float(h[i]) * by, __half2float(h[i + 4]) * by);
+        }
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      const float per = up * a.scale;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int owner = (2 * t + i) * 4;
+        qa[nt][i] = __shfl_sync(0xffffffffu, per, owner);
+        qb[nt][i] = __shfl_sync(0xffffffffu, sum, owner) * qa[nt][i];
+        qa[nt][i] *= 16777216.0f;
+        const int row = c.tile * ROWS + nt * 8 + 2 * t + i, jj = row / a.each;
+        hi[nt][i] = jj < c.s.nq ? c.s.len - c.s.nq + jj : -1;
+        lo[nt][i] = a.window ? (long long)c.s.len - c.s.nq + jj - a.window + 1 : 0;
+        mx[nt][i] = -CUDART_INF_F;
+        l[nt][i] = lm[nt][i] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VWORDS * 4; ++i)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.0f;
+    sigma = inv_sigma = 0.0f;
+    // keys that every row of the tile sees
+    const int j0 = c.tile * ROWS / a.each, j1 = (c.tile * ROWS + ROWS - 1) / a.each;
+    full_hi = c.s.len - c.s.nq + j0;
+    full_lo = a.window ? (long long)c.s.len - c.s.nq + min(j1, c.s.nq - 1) - a.window + 1 : 0;
+  };
+
+  auto chunk = [&](const uint8_t* st, int tok0, unsigned mask) {
+    const uint8_t* const kp = st + 2 * SH::CODE_BYTES;
+    const uint8_t* const vp = kp + SH::PARAM_BYTES;
+    const bool full = mask == (1u << pieces) - 1 && tok0 + CT - 1 <= full_hi && tok0 >= full_lo;
+    const int pg = g ^ (g >> 1 & 1);                 // the key of operand row g: neighbours alternate, which spreads the value rows over the banks
+    float p[MT][NT][4];
+    float2 sv[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const int r0 = mt * 16 + pg;
+      uint32_t k0[KWORDS], k1[KWORDS];
+      if constexpr (D == 64) {
+        const uint2 x = *reinterpret_cast<const uint2*>(st + r0 * KROW + 8 * t), y = *reinterpret_cast<const uint2*>(st + (r0 + 8) * KROW + 8 * t);
+        k0[0] = x.x; k0[1] = x.y; k1[0] = y.x; k1[1] = y.y;
+      } else {
+#pragma unroll
+        for (int h = 0; h < KWORDS / 4; ++h) {
+          const uint4 x = *reinterpret_cast<const uint4*>(st + r0 * KROW + 64 * h + 16 * t), y = *reinterpret_cast<const uint4*>(st + (r0 + 8) * KROW + 64 * h + 16 * t);
+          k0[4 * h] = x.x; k0[4 * h + 1] = x.y; k0[4 * h + 2] = x.z; k0[4 * h + 3] = x.w;
+          k1[4 * h] = y.x; k1[4 * h + 1] = y.y; k1[4 * h + 2] = y.z; k1[4 * h + 3] = y.w;
+        }
+      }
+      float acc[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < KWORDS; ++w) {
+        const uint32_t x = k0[w], y = k1[w], x8 = x >> 8, y8 = y >> 8;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          mma_16816(acc[nt], x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, qf[nt][2 * w][0], qf[nt][2 * w][1]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          mma_16816(acc[nt], x8 & 0x000f000fu, y8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x00f000f0u, qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
+      }
+      const float2 s0 = pair_of<T>(*reinterpret_cast<const uint32_t*>(kp + r0 * 4)), s1 = pair_of<T>(*reinterpret_cast<const uint32_t*>(kp + (r0 + 8) * 4));
+      sv[mt][0] = pair_of<T>(*reinterpret_cast<const uint32_t*>(vp + r0 * 4));
+      sv[mt][1] = pair_of<T>(*reinterpret_cast<const uint32_t*>(vp + (r0 + 8) * 4));
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 s = i < 2 ? s0 : s1;
+          p[mt][nt][i] = fmaf(acc[nt][i], s.x * qa[nt][i & 1], s.y * qb[nt][i & 1]);
+        }
+      }
+      if (!full) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int tok = tok0 + r0 + 8 * e;
+          const bool there = mask >> ((r0 + 8 * e) / psz) & 1u;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (!there || tok > hi[nt][i] || tok < lo[nt][i]) p[mt][nt][2 * e + i] = -CUDART_INF_F;
+          if (!there || tok >= c.s.len) sv[mt][e] = make_float2(0.0f, 0.0f);     // nothing was fetched, or nothing was ever written
+        }
+      }
+    }
+    // running maxima; nothing is exchanged while no lane exceeds them
+    float top[NT][2], big = 0.0f;
+    bool grows = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        top[nt][i] = fmaxf(p[0][nt][i], p[0][nt][i + 2]);
+#pragma unroll
+        for (int mt = 1; mt < MT; ++mt) top[nt][i] = fmaxf(top[nt][i], fmaxf(p[mt][nt][i], p[mt][nt][i + 2]));
+        grows = grows || top[nt][i] > mx[nt][i];
+      }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float s = fabsf(sv[mt][e].x);
+        if (s <= 3.402823466e38f) big = fmaxf(big, s);
+      }
+    grows = grows || big > sigma;
+    if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) {
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) top[nt][i] = fmaxf(top[nt][i], __shfl_xor_sync(0xffffffffu, top[nt][i], x));
+      }
+      float by = 1.0f;
+      if (big > sigma) {
+        // a power of two above every scale so far, in [2^-100, 2^127]
+        const int e = min(max((int)(__float_as_uint(big) >> 23) + 1, 27), 254);
+        const float next = __uint_as_float((uint32_t)e << 23);
+        by = sigma == 0.0f ? 0.0f : sigma * (1.0f / next);
+        sigma = next;
+        inv_sigma = 32768.0f / next;
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float alpha[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float m = fmaxf(mx[nt][i], top[nt][i]);
+          alpha[i] = mx[nt][i] == m ? 1.0f : exp2_fast(mx[nt][i] - m);
+          mx[nt][i] = m;
+          l[nt][i] *= alpha[i];
+          lm[nt][i] *= alpha[i];
+          alpha[i] *= by;
+        }
+#pragma unroll
+        for (int i = 0; i < VWORDS * 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][nt][e] *= alpha[e & 1];
+      }
+    }
+    // probabilities, their sums, and the second operand of P V
+    uint32_t pf[MT][NT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float w[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float m = mx[nt][i] == -CUDART_INF_F ? 0.0f : mx[nt][i];
+            const float pr = exp2_fast(p[mt][nt][2 * e + i] - m);
+            const bool hidden = !full && p[mt][nt][2 * e + i] == -CUDART_INF_F;      // what it hides may be anything
+            l[nt][i] += pr;
+            lm[nt][i] = hidden ? lm[nt][i] : fmaf(pr, sv[mt][e].y, lm[nt][i]);
+            w[i] = hidden ? 0.0f : pr * (sv[mt][e].x * inv_sigma);
+          }
+          pf[mt][nt][e] = transpose8x8(pack_half2(w[0], w[1]));
+        }
+      }
+    const uint8_t* const vs = st + SH::CODE_BYTES + g * (4 * VWORDS);
+    const int x0 = 2 * t ^ (t & 1), y0 = x0 ^ 1;
+#pragma unroll
+    for (int j = 0; j < VWORDS; ++j) {
+      float part[4][NT][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) part[i][nt][0] = part[i][nt][1] = part[i][nt][2] = part[i][nt][3] = 0.0f;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const uint8_t* const at = vs + mt * 16 * KROW + 4 * j;
+        const uint32_t x = *reinterpret_cast<const uint32_t*>(at + x0 * KROW), y = *reinterpret_cast<const uint32_t*>(at + y0 * KROW);
+        const uint32_t z = *reinterpret_cast<const uint32_t*>(at + (x0 + 8) * KROW), w = *reinterpret_cast<const uint32_t*>(at + (y0 + 8) * KROW);
+        const uint32_t a01 = __byte_perm(x, y, 0x5410), a23 = __byte_perm(x, y, 0x7632), b01 = __byte_perm(z, w, 0x5410), b23 = __byte_perm(z, w, 0x7632);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t u = (i < 2 ? a01 : a23) >> (8 * (i & 1)), v = (i < 2 ? b01 : b23) >> (8 * (i & 1));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma_16816(part[i][nt], u & 0x000f000fu, u & 0x00f000f0u, v & 0x000f000fu, v & 0x00f000f0u, pf[mt][nt][0], pf[mt][nt][1]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[4 * j + i][nt][e] += part[i][nt][e];
+    }
+  };
+
+  // the warps' parts of an item joined, and written as the result or as this CTA's part of it
+  auto finish_item = [&](bool whole, int slot) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) {
+          l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], x);
+          lm[nt][i] += __shfl_xor_sync(0xffffffffu, lm[nt][i], x);
+        }
+        const int row = nt * 8 + 2 * t + i;
+        if (g == 0) stats[warp * ROWS + row] = make_float4(mx[nt][i], l[nt][i], lm[nt][i], 0.0f);
+        float* const dst = merge + (warp * ROWS + row) * SH::MERGE_ROW + g * (D / 8);
+        const float by = 512.0f * sigma;
+#pragma unroll
+        for (int j = 0; j < VWORDS * 4; ++j)
+          *reinterpret_cast<float2*>(dst + 2 * j) = make_float2(o[j][nt][i] * by, o[j][nt][2 + i] * (by * 0.0625f));
+      }
+    __syncthreads();
+    constexpr int QUADS = D / 4;
+    for (int i = tid; i < ROWS * QUADS; i += W * 32) {
+      const int row = i / QUADS, d = i % QUADS * 4;
+      const int r = c.tile * ROWS + row, j = r / a.each;
+      if (j >= c.s.nq) continue;
+      float m = -CUDART_INF_F;
+#pragma unroll
+      for (int w = 0; w < W; ++w) m = fmaxf(m, stats[w * ROWS + row].x);
+      float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      float weight = 0.0f;
+      if (m != -CUDART_INF_F) {
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const float4 st = stats[w * ROWS + row];
+          const float by = exp2_fast(st.x - m);
+          const float4 v = *reinterpret_cast<const float4*>(merge + (w * ROWS + row) * SH::MERGE_ROW + d);
+          weight = fmaf(st.y, by, weight);
+          sum.x = fmaf(v.x + st.z, by, sum.x);
+          sum.y = fmaf(v.y + st.z, by, sum.y);
+          sum.z = fmaf(v.z + st.z, by, sum.z);
+          sum.w = fmaf(v.w + st.z, by, sum.w);
+        }
+      }
+      if (whole) {
+        const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
+        T* const dst = reinterpret_cast<T*>(a.out) + ((long long)(c.s.q0 + j) * a.q_heads + c.head * a.each + r - j * a.each) * D + d;
+        T v[4] = {from_float<T>(sum.x * inv), from_float<T>(sum.y * inv), from_float<T>(sum.z * inv), from_float<T>(sum.w * inv)};
+        *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(v);
+      } else {
+        *reinterpret_cast<float4*>(a.part_o + ((long long)slot * ROWS + row) * D + d) = sum;
+        if (d == 0) a.part_ml[(long long)slot * ROWS + row] = make_float2(m, weight);
+      }
+    }
+    __syncthreads();
+  };
+
+  int stage = 0;
+  bool opens = true;
+  int from_unit = 0;
+#pragma unroll 1
+  for (long long u = u0; u < u1; ++u) {
+    if (opens) {
+      start_item();
+      from_unit = c.unit;
+      opens = false;
+    }
+    const unsigned mask = masks >> (4 * stage) & 15u;
+    if (mask) {
+      if (!mbar_wait(bars + 8 * stage, phases >> stage & 1u)) {
+        dead = true;
+        if (lane == 0 && a.status) *a.status = 1u;
+      }
+      phases ^= 1u << stage;
+      if (!dead) chunk(ring + stage * SH::STAGE, c.s.first + (c.unit * W + warp) * CT, mask);
+      __syncwarp();
+    }
+    issue(stage);
+    look_up();
+    stage = stage + 1 == S ? 0 : stage + 1;
+    const bool ends = c.unit + 1 == c.s.units;
+    if (ends || u + 1 == u1) {
+      finish_item(ends && from_unit == 0, 2 * blockIdx.x + (from_unit == 0 ? 1 : 0));
+      opens = true;
+    }
+    advance<ROWS, SH::UNIT, CT>(a, c);
+  }
+}
+
+// Joins the parts of an item that several CTAs of the kernel above worked on: one block per item and row.
+template <typename T, typename SH>
+__global__ void __launch_bounds__(128) kv4_attention_join_kernel(const AttnArgs a, int ctas) {
+  constexpr int D = SH::D, ROWS = SH::ROWS, PER = D / 32;
+  __shared__ float sums[4][D];
+  __shared__ float2 ml[4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  Walk w;
+  long long u0 = 0;
+  if (!place<ROWS, SH::UNIT, SH::CT>(a, lane, blockIdx.x, true, w, u0)) return;
+  const long long total = count_units<ROWS, SH::UNIT, SH::CT>(a, lane);
+  const int r = w.tile * ROWS + row, j = r / a.each;
+  if (j >= w.s.nq) return;
+  const long long u1 = u0 + w.s.units;
+  const int i0 = (int)(((u0 + 1) * ctas - 1) / total), i1 = (int)((u1 * ctas - 1) / total);
+  if (i0 == i1) return;                        // one CTA had it all and has written it
+  float m = -CUDART_INF_F, weight = 0.0f;
+  float sum[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) sum[e] = 0.0f;
+  for (int i = i0 + warp; i <= i1; i += 4) {
+    const long long start = share(total, i, ctas);
+    if (start == share(total, i + 1, ctas)) continue;            // fewer units than CTAs: this one had none
+    const int slot = 2 * i + (start > u0 ? 0 : 1);
+    const float2 s = a.part_ml[(long long)slot * ROWS + row];
+    float v[PER];
+    const float* src = a.part_o + ((long long)slot * ROWS + row) * D + lane * PER;
+#pragma unroll
+    for (int e = 0; e < PER; e += 2) *reinterpret_cast<float2*>(v + e) = *reinterpret_cast<const float2*>(src + e);
+    if (s.x == -CUDART_INF_F) continue;
+    const float top = fmaxf(m, s.x);
+    const float keep = m == top ? 1.0f : exp2_fast(m - top), by = exp2_fast(s.x - top);
+    m = top;
+    weight = fmaf(s.y, by, weight * keep);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) sum[e] = fmaf(v[e], by, sum[e] * keep);
+  }
+#pragma unroll
+  for (int e = 0; e < PER; ++e) sums[warp][lane * PER + e] = sum[e];
+  if (lane == 0) ml[warp] = make_float2(m, weight);
+  __syncthreads();
+  for (int d = threadIdx.x; d < D; d += 128) {
+    float top = -CUDART_INF_F, all = 0.0f, value = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, ml[i].x);
+    if (top != -CUDART_INF_F) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float by = exp2_fast(ml[i].x - top);
+        all = fmaf(ml[i].y, by, all);
+        value = fmaf(sums[i][d], by, value);
+      }
+    }
+    reinterpret_cast<T*>(a.out)[((long long)(w.s.q0 + j) * a.q_heads + w.head * a.each + r - j * a.each) * D + d] =
+        from_float<T>(all == 0.0f ? 0.0f : value / all);
+  }
+}
+
+constexpr int kCtasPerSm = 2;
+
+template <int D, int NT>
+using Few = Shape<D, NT, 4, D == 256 ? 16 : 32, 4>;
+
+template <typename T, int D, int NT>
+int run(AttnArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  using SH = Few<D, NT>;
+  static_assert(SH::SMEM <= 113 * 1024, "two CTAs per SM");
+  const int ctas = kCtasPerSm * sm_count();
+  const size_t o_bytes = (size_t)2 * ctas * SH::ROWS * D * 4;
+  XQT_REQUIRE(workspace && workspace_bytes >= o_bytes + (size_t)2 * ctas * SH::ROWS * 8 && ((uintptr_t)workspace & 15) == 0);
+  a.part_o = reinterpret_cast<float*>(workspace);
+  a.part_ml = reinterpret_cast<float2*>((uint8_t*)workspace + o_bytes);
+  XQT_SMEM_OPT_IN((kv4_attention_kernel<T, SH>), SH::SMEM);
+  int rc = launch_pdl(kv4_attention_kernel<T, SH>, dim3((unsigned)ctas), dim3(SH::W * 32), SH::SMEM, stream, a);
+  if (rc) return rc;
+  // as many items as there can be: full tiles, and one that is not full per sequence
+  const long long tiles = a.query_starts ? (long long)a.tokens * a.each / SH::ROWS + a.batch : (long long)a.batch * ceil_div(a.each, SH::ROWS);
+  XQT_REQUIRE(tiles * a.kv_heads < (1LL << 31) - 1);
+  return launch_pdl(kv4_attention_join_kernel<T, SH>, dim3((unsigned)(tiles * a.kv_heads), SH::ROWS), dim3(128), 0, stream, a, ctas);
+}
+
+template <typename T>
+int run_dim(const AttnArgs& a, int dim, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  // two 8-row tiles where eight rows do not hold a key head's queries (128 and 256 channels: the registers of one of 256)
+  const bool wide = a.each > 8 || a.query_starts;
+  if (dim == 64) return wide ? run<T, 64, 2>(a, workspace, workspace_bytes, stream) : run<T, 64, 1>(a, workspace, workspace_bytes, stream);
+  if (dim == 128) return wide ? run<T, 128, 2>(a, workspace, workspace_bytes, stream) : run<T, 128, 1>(a, workspace, workspace_bytes, stream);
+  return run<T, 256, 1>(a, workspace, workspace_bytes, stream);
+}
+
+}  // namespace
+}  // namespace xqt_b200
+
+extern "C" size_t xqt_b200_kv4_attention_workspace_bytes(int dim) {
+  using namespace xqt_b200;
+  return (size_t)2 * kCtasPerSm * sm_count() * 16 * (dim + 2) * 4;
+}
+
+extern "C" int xqt_b200_kv4_attention(const void* q, const void* codes, const void* params, const int* table, const int* seq_lens, const int* query_starts,
+                                      void* out, const long long* strides, int tokens, int batch, int q_heads, int kv_heads, int dim, long long pages,
+                                      int page_size, int table_width, int window, int dtype, float scale, void* workspace, size_t workspace_bytes,
+                                      unsigned* status, cudaStream_t stream) {
+  using namespace xqt_b200;
+  XQT_REQUIRE(tokens >= 0 && batch >= 0 && kv_heads >= 1 && kv_heads <= (1 << 16) && q_heads >= kv_heads && q_heads <= (1 << 16) && q_heads % kv_heads == 0);
+  XQT_REQUIRE(dim == 64 || dim == 128 || dim == 256);
+  XQT_REQUIRE(dtype == XQT_B200_FP16 || dtype == XQT_B200_BF16);
+  XQT_REQUIRE(page_size >= 16 && page_size <= 4096 && (page_size & (page_size - 1)) == 0);
+  XQT_REQUIRE(pages >= 0 && pages < (1LL << 31) && table_width >= 0 && (long long)table_width * page_size < (1LL << 31) - 4096);
+  XQT_REQUIRE(window >= 0 && (long long)tokens * (q_heads / kv_heads) < (1LL << 31) - 4096);
+  if (tokens == 0 || batch == 0) return 0;
+  XQT_REQUIRE(q && out && seq_lens && strides && (table_width == 0 || table) && (pages == 0 || (codes && params)));
+  XQT_REQUIRE((query_starts != nullptr) || tokens == batch);
+  XQT_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)codes | (uintptr_t)params) & 15) == 0 && ((strides[0] | strides[1]) & 7) == 0);
+  AttnArgs a = {};
+  a.q = q;
+  a.codes = (const uint8_t*)codes;
+  a.params = (const uint8_t*)params;
+  a.table = table;
+  a.seq_lens = seq_lens;
+  a.query_starts = query_starts;
+  a.out = out;
+  a.status = status;
+  a.q_token = strides[0];
+  a.q_head = strides[1];
+  a.table_stride = strides[2];
+  a.pages = pages;
+  a.tokens = tokens;
+  a.batch = batch;
+  a.q_heads = q_heads;
+  a.kv_heads = kv_heads;
+  a.each = q_heads / kv_heads;
+  a.page_size = page_size;
+  a.page_shift = __builtin_ctz((unsigned)page_size);
+  a.table_width = table_width;
+  a.window = window;
+  a.scale = scale * 1.4426950408889634f;
+  return dtype == XQT_B200_BF16 ? run_dim<__nv_bfloat16>(a, dim, workspace, workspace_bytes, stream)
+                                : run_dim<__half>(a, dim, workspace, workspace_bytes, stream);
+}

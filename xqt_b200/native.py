@@ -80,6 +80,11 @@ SIGNATURES: dict[str, tuple] = {
     "xqt_b200_w4a16_swiglu_mlp_workspace_bytes": (_Z, [_I] * 3),
     "xqt_b200_w4a16_swiglu_mlp": (_I, [_P] * 8 + [_I] * 10 + [_P, _Z, _P]),
     "xqt_b200_swiglu": (_I, [_P, _P, _I, _I, _I, _P]),
+    "xqt_b200_qk_norm_rope": (_I, [_P] * 10 + [_I] * 10 + [ctypes.c_float, _P]),
+    "xqt_b200_kv4_append": (_I, [_P] * 6 + [_I] * 3 + [ctypes.c_longlong] + [_I] * 3 + [_P]),
+    "xqt_b200_kv4_gather": (_I, [_P] * 5 + [_I] * 3 + [ctypes.c_longlong] + [_I] * 3 + [_P]),
+    "xqt_b200_kv4_attention_workspace_bytes": (_Z, [_I]),
+    "xqt_b200_kv4_attention": (_I, [_P] * 8 + [_I] * 5 + [ctypes.c_longlong] + [_I] * 4 + [ctypes.c_float, _P, _Z, _P, _P]),
     "xqt_b200_workspace_status": (_I, [_P, ctypes.POINTER(ctypes.c_uint), _P]),
 }
 

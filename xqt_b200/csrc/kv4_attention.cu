@@ -18,7 +18,10 @@
 // CTAs share are joined by a second kernel.  Each warp fetches its own chunks with bulk copies, S of them ahead.
 //
 // Bound by HBM: (dim + 8) bytes per key and head.
+#include <limits.h>
 #include <math_constants.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "sm100.cuh"
@@ -55,6 +58,11 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(a));
@@ -64,22 +72,42 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];\n" ::"l"(p)); }
+// a pair of floats as the packed instructions take it
+struct Two {
+  unsigned long long v;
+  __device__ __forceinline__ Two() {}
+  __device__ __forceinline__ Two(float a, float b) : v(f32x2_pack(a, b)) {}
+  __device__ __forceinline__ explicit Two(float a) : v(f32x2_pack(a, a)) {}
+  __device__ __forceinline__ float2 both() const {
+    float2 f;
+    f32x2_unpack(v, f.x, f.y);
+    return f;
+  }
+};
+__device__ __forceinline__ Two operator*(Two a, Two b) { Two r; r.v = f32x2_mul(a.v, b.v); return r; }
+__device__ __forceinline__ Two operator+(Two a, Two b) { Two r; r.v = f32x2_add(a.v, b.v); return r; }
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) { Two r; r.v = f32x2_fma(a.v, b.v, c.v); return r; }
 template <typename T>
 __device__ __forceinline__ float2 pair_of(uint32_t bits) {
   const T* e = reinterpret_cast<const T*>(&bits);
   return make_float2(to_float<T>(e[0]), to_float<T>(e[1]));
 }
 
-template <int D_, int NT_, int W_, int CT_, int S_>
+template <int D_, int NT_, int W_, int CT_, int S_, int PER_SM_>
 struct Shape {
-  static constexpr int D = D_, NT = NT_, W = W_, CT = CT_, S = S_;
+  static constexpr int D = D_, NT = NT_, W = W_, CT = CT_, S = S_, PER_SM = PER_SM_;
   static constexpr int ROWS = 8 * NT, KROW = D / 2, KWORDS = D / 32, VWORDS = D / 64, MT = CT / 16;
   static constexpr int UNIT = W * CT;
   static constexpr int CODE_BYTES = CT * KROW, PARAM_BYTES = CT * 4, STAGE = 2 * (CODE_BYTES + PARAM_BYTES);
-  static constexpr int MERGE_ROW = D + 4;
-  static constexpr int MERGE_BYTES = W * ROWS * MERGE_ROW * 4, STAT_BYTES = W * ROWS * 16;
+  static constexpr int MERGE_ROW = D + 8;
+  static constexpr int MERGES = W / 2;                    // buffers: the warps write them in two rounds
+  static constexpr int MERGE_BYTES = MERGES * ROWS * MERGE_ROW * 4, STAT_BYTES = W * ROWS * 16;
   static constexpr int SMEM = W * S * STAGE + MERGE_BYTES + STAT_BYTES + W * S * 8;
 };
+
+// Units that stand for an item's beginning and end (its queries read, its warps joined): they go first and have no keys.
+constexpr int kOpening = 1;
 
 // A sequence as the work list sees it.
 struct Sequence {
@@ -102,66 +130,79 @@ __device__ __forceinline__ Sequence sequence(const AttnArgs& a, int b) {
   const long long from = a.window ? (long long)s.len - s.nq + 1 - a.window : 0;
   s.first = from > 0 ? (int)(from / CT * CT) : 0;
   s.tiles = (int)(((long long)s.nq * a.each + ROWS - 1) / ROWS);
-  s.units = max((s.len - s.first + UNIT - 1) / UNIT, 1);   // an empty sequence still has its rows written
+  s.units = max((s.len - s.first + UNIT - 1) / UNIT, 0) + kOpening;   // an empty sequence still has its rows written
   return s;
 }
 
-// All units, and the place of unit `u` in the list; every warp does it for itself.
+// A place in the work list.
 struct Walk {
   int b, tile, head, unit;
   Sequence s;
 };
 
-template <int ROWS, int UNIT, int CT>
-__device__ __forceinline__ long long count_units(const AttnArgs& a, int lane) {
-  long long sum = 0;
-  for (int b = lane; b < a.batch; b += 32) {
-    const Sequence s = sequence<ROWS, UNIT, CT>(a, b);
-    sum += (long long)s.tiles * a.kv_heads * s.units;
+// The list: its units are dealt out in equal contiguous runs, the first `more` CTAs one unit longer.  32 bits: the host refuses more.
+struct Deal {
+  unsigned total, each, more;
+  __device__ __forceinline__ unsigned start(unsigned i) const { return each * i + min(i, more); }
+  __device__ __forceinline__ unsigned owner(unsigned u) const {
+    const unsigned long_run = more * (each + 1);
+    return u < long_run ? u / (each + 1) : more + (u - long_run) / max(each, 1u);
   }
+};
+
+__device__ __forceinline__ unsigned scan32(unsigned v, int lane) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return sum;
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned x = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += x;
+  }
+  return v;
 }
 
-// by_item: `u` counts items (tile, head) and not units; `before` gets the units in front of the item then
 template <int ROWS, int UNIT, int CT>
-__device__ __forceinline__ bool place(const AttnArgs& a, int lane, long long u, bool by_item, Walk& w, long long& before) {
-  long long base = 0, base_units = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 32) {
-    long long n = 0, units = 0;
+__device__ __forceinline__ Deal deal(const AttnArgs& a, int lane, unsigned ctas, Sequence& mine) {
+  Deal d = {};
+  for (int b0 = (a.batch - 1) & ~31; b0 >= 0; b0 -= 32) {      // backwards: `mine` ends as sequence `lane`
+    unsigned units = 0;
     if (b0 + lane < a.batch) {
-      const Sequence s = sequence<ROWS, UNIT, CT>(a, b0 + lane);
-      n = (long long)s.tiles * a.kv_heads;
-      units = n * s.units;
+      mine = sequence<ROWS, UNIT, CT>(a, b0 + lane);
+      units = (unsigned)mine.tiles * a.kv_heads * mine.units;
     }
-    long long cum_units = units;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, cum_units, o);
-      if (lane >= o) cum_units += y;
+    d.total += __reduce_add_sync(0xffffffffu, units);
+  }
+  d.each = d.total / ctas;
+  d.more = d.total - d.each * ctas;
+  return d;
+}
+
+// The place of unit `u`, or with by_item of item (tile, head) number `u`; `before` gets the units in front of it.
+template <int ROWS, int UNIT, int CT>
+__device__ __forceinline__ bool place(const AttnArgs& a, int lane, const Sequence& mine, unsigned u, bool by_item, Walk& w, unsigned& before) {
+  unsigned base = 0, base_units = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 32) {
+    Sequence s = mine;
+    unsigned items = 0, units = 0;
+    if (b0 + lane < a.batch) {
+      if (b0 > 0) s = sequence<ROWS, UNIT, CT>(a, b0 + lane);
+      items = (unsigned)s.tiles * a.kv_heads;
+      units = items * s.units;
     }
-    long long cum = cum_units;
-    if (by_item) {
-      cum = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, cum, o);
-        if (lane >= o) cum += x;
-      }
-    } else {
-      n = units;
-    }
+    const unsigned cum_units = scan32(units, lane), n = by_item ? items : units, cum = by_item ? scan32(items, lane) : cum_units;
     const unsigned over = __ballot_sync(0xffffffffu, base + cum > u);
     if (over) {
       const int at = __ffs(over) - 1;
-      const long long rest = u - base - __shfl_sync(0xffffffffu, cum - n, at);
+      const unsigned rest = u - base - __shfl_sync(0xffffffffu, cum - n, at);
       w.b = b0 + at;
-      w.s = sequence<ROWS, UNIT, CT>(a, w.b);
-      const long long item = by_item ? rest : rest / w.s.units;
+      w.s.q0 = __shfl_sync(0xffffffffu, s.q0, at);
+      w.s.nq = __shfl_sync(0xffffffffu, s.nq, at);
+      w.s.len = __shfl_sync(0xffffffffu, s.len, at);
+      w.s.first = __shfl_sync(0xffffffffu, s.first, at);
+      w.s.tiles = __shfl_sync(0xffffffffu, s.tiles, at);
+      w.s.units = __shfl_sync(0xffffffffu, s.units, at);
+      const unsigned item = by_item ? rest : rest / (unsigned)w.s.units;
       w.unit = by_item ? 0 : (int)(rest - item * w.s.units);
-      w.tile = (int)(item / a.kv_heads);
-      w.head = (int)(item - (long long)w.tile * a.kv_heads);
+      w.tile = (int)(item / (unsigned)a.kv_heads);
+      w.head = (int)(item - (unsigned)w.tile * a.kv_heads);
       before = base_units + __shfl_sync(0xffffffffu, cum_units - units, at) + item * w.s.units;
       return true;
     }
@@ -185,10 +226,8 @@ __device__ __forceinline__ void advance(const AttnArgs& a, Walk& w) {
   }
 }
 
-__device__ __forceinline__ long long share(long long units, int i, int n) { return units * i / n; }
-
 template <typename T, typename SH>
-__global__ void __launch_bounds__(SH::W * 32) kv4_attention_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(const AttnArgs a) {
   constexpr int D = SH::D, NT = SH::NT, W = SH::W, CT = SH::CT, S = SH::S, ROWS = SH::ROWS, MT = SH::MT, KROW = SH::KROW;
   constexpr int KWORDS = SH::KWORDS, VWORDS = SH::VWORDS;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -205,12 +244,13 @@ __global__ void __launch_bounds__(SH::W * 32) kv4_attention_kernel(const AttnArg
   grid_launch_dependents();
   grid_dependency_wait();
 
-  const long long total = count_units<ROWS, SH::UNIT, CT>(a, lane);
-  const long long u0 = share(total, blockIdx.x, gridDim.x), u1 = share(total, blockIdx.x + 1, gridDim.x);
+  Sequence mine = {};
+  const Deal d = deal<ROWS, SH::UNIT, CT>(a, lane, gridDim.x, mine);
+  const unsigned u0 = d.start(blockIdx.x), u1 = d.start(blockIdx.x + 1);
   if (u0 >= u1) return;
   Walk c;
-  long long unused;
-  if (!place<ROWS, SH::UNIT, CT>(a, lane, u0, false, c, unused)) return;
+  unsigned unused;
+  if (!place<ROWS, SH::UNIT, CT>(a, lane, mine, u0, false, c, unused)) return;
 
   // ---- fetching
   const int psz = min(a.page_size, CT), pieces = CT / psz;
@@ -221,7 +261,26 @@ __global__ void __launch_bounds__(SH::W * 32) kv4_attention_kernel(const AttnArg
   const uint32_t target = smem_addr(ring) + (kind == 0 ? 0 : kind == 1 ? SH::CODE_BYTES : kind == 2 ? 2 * SH::CODE_BYTES : 2 * SH::CODE_BYTES + SH::PARAM_BYTES) +
                           piece * psz * row_bytes;
   Walk f = c;
-  long long to_fetch = u1 - u0;
+  // of the item being fetched: its units not yet asked for, this lane's next key, the keys that some row of the tile sees, the table's row
+  int f_units = 0, f_at = 0, f_end = 0, f_begin = 0;
+  const int* f_table = nullptr;
+  auto open = [&]() {
+    const int j0 = f.tile * ROWS / a.each, j1 = min(f.s.nq - 1, (f.tile * ROWS + ROWS - 1) / a.each);
+    f_units = f.s.units - f.unit;
+    f_at = piece < pieces ? f.s.first + ((f.unit - kOpening) * W + warp) * CT + piece * psz : INT_MAX - (1 << 24);
+    f_end = f.b < a.batch ? f.s.len - f.s.nq + j1 + 1 : 0;      // (starts that do not ascend can make the list shorter than it counts)
+    f_begin = a.window ? (int)max((long long)f.s.len - f.s.nq + j0 - a.window + 1, 0LL) : 0;
+    f_table = a.table + f.b * a.table_stride;
+    // its queries, which the warps read when they come to it
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = f.tile * ROWS + nt * 8 + g, j = r / a.each;
+      if (j < f.s.nq)
+        prefetch_l1(reinterpret_cast<const T*>(a.q) + (long long)(f.s.q0 + j) * a.q_token + (long long)(f.head * a.each + r - j * a.each) * a.q_head + t * (D / 4));
+    }
+  };
+  open();
+  int to_fetch = (int)(u1 - u0);
   int next_page = -1, next_row = 0;
   uint32_t masks = 0, phases = 0;
   bool dead = false;
@@ -229,26 +288,24 @@ __global__ void __launch_bounds__(SH::W * 32) kv4_attention_kernel(const AttnArg
   auto look_up = [&]() {
     next_page = -1;
     if (to_fetch > 0) {
-      const int tok0 = f.s.first + (f.unit * W + warp) * CT;
-      const int at = tok0 + piece * psz;
-      const int j0 = f.tile * ROWS / a.each, j1 = min(f.s.nq - 1, (f.tile * ROWS + ROWS - 1) / a.each);
-      const int last = f.s.len - f.s.nq + j1;
-      const long long lowest = a.window ? (long long)f.s.len - f.s.nq + j0 - a.window + 1 : 0;
-      if (piece < pieces && at < f.s.len && tok0 <= last && tok0 + CT > lowest) {
-        const int page = a.table[f.b * a.table_stride + (at >> a.page_shift)];
-        next_page = page >= 0 && page < a.pages ? page : -1;
-      }
-      next_row = f.head * a.page_size + (at & (a.page_size - 1));
+      if (f_at < f_end && f_at + psz > f_begin) next_page = f_table[f_at >> a.page_shift];
+      next_row = f.head * a.page_size + (f_at & (a.page_size - 1));
       --to_fetch;
-      if (to_fetch > 0) advance<ROWS, SH::UNIT, CT>(a, f);
+      if (--f_units > 0) {
+        if (piece < pieces) f_at += SH::UNIT;
+      } else if (to_fetch > 0) {
+        f.unit = f.s.units - 1;
+        advance<ROWS, SH::UNIT, CT>(a, f);
+        open();
+      }
     }
   };
   auto issue = [&](int stage) {
-    const bool valid = next_page >= 0 && !dead;
+    const bool valid = (unsigned)next_page < (unsigned)a.pages && !dead;
     const unsigned votes = __ballot_sync(0xffffffffu, valid);
-    unsigned mask = 0;
-#pragma unroll
-    for (int p = 0; p < MT; ++p) mask |= (votes >> (4 * p) & 1u) << p;
+    unsigned mask = votes & 1u;
+    if constexpr (MT > 1) mask |= votes >> 3 & 2u;
+    if constexpr (MT > 2) mask |= (votes >> 6 & 4u) | (votes >> 9 & 8u);
     masks = (masks & ~(15u << (4 * stage))) | mask << (4 * stage);
     if (mask) {
       const uint32_t bar = bars + 8 * stage;
@@ -266,13 +323,14 @@ __global__ void __launch_bounds__(SH::W * 32) kv4_attention_kernel(const AttnArg
 
   // ---- one item's state
   uint32_t qf[NT][2 * KWORDS][2];
-  float qa[NT][2], qb[NT][2];
-  int hi[NT][2];
-  long long lo[NT][2];
-  float o[VWORDS * 4][NT][4];
-  float mx[NT][2], l[NT][2], lm[NT][2], sigma = 0.0f, inv_sigma = 0.0f;
-  int full_hi = 0;
-  long long full_lo = 0;
+  Two qa[NT], qb[NT];
+  int hi[NT][2], lo[NT][2];
+  Two o[VWORDS * 4][NT][2];
+  float mx[NT][2], sigma = 0.0f, inv_sigma = 0.0f;
+  Two l[NT], lm[NT], lw[NT];       // sums of p and of p * m, and what the rounding of the operands p * s took away
+  int full_hi = 0, full_lo = 0;
+  const unsigned all_pieces = (1u << pieces) - 1;
+  constexpr bool KEEP_ROUNDING = sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value;
 
   auto start_item = [&]() {
 #pragma unroll
@@ -317,39 +375,43 @@ __global__ void __launch_bounds__(SH::W * 32) kv4_attention_kernel(const AttnArg
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       const float per = up * a.scale;
+      float qs[2], qt[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int owner = (2 * t + i) * 4;
-        qa[nt][i] = __shfl_sync(0xffffffffu, per, owner);
-        qb[nt][i] = __shfl_sync(0xffffffffu, sum, owner) * qa[nt][i];
-        qa[nt][i] *= 16777216.0f;
+        qs[i] = __shfl_sync(0xffffffffu, per, owner);
+        qt[i] = __shfl_sync(0xffffffffu, sum, owner) * qs[i];
+        qs[i] *= 16777216.0f;
         const int row = c.tile * ROWS + nt * 8 + 2 * t + i, jj = row / a.each;
         hi[nt][i] = jj < c.s.nq ? c.s.len - c.s.nq + jj : -1;
-        lo[nt][i] = a.window ? (long long)c.s.len - c.s.nq + jj - a.window + 1 : 0;
+        lo[nt][i] = a.window ? (int)max((long long)c.s.len - c.s.nq + jj - a.window + 1, 0LL) : 0;
         mx[nt][i] = -CUDART_INF_F;
-        l[nt][i] = lm[nt][i] = 0.0f;
       }
+      qa[nt] = Two(qs[0], qs[1]);
+      qb[nt] = Two(qt[0], qt[1]);
+      l[nt] = lm[nt] = lw[nt] = Two(0.0f);
     }
 #pragma unroll
     for (int i = 0; i < VWORDS * 4; ++i)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.0f;
+        for (int e = 0; e < 2; ++e) o[i][nt][e] = Two(0.0f);
     sigma = inv_sigma = 0.0f;
     // keys that every row of the tile sees
     const int j0 = c.tile * ROWS / a.each, j1 = (c.tile * ROWS + ROWS - 1) / a.each;
     full_hi = c.s.len - c.s.nq + j0;
-    full_lo = a.window ? (long long)c.s.len - c.s.nq + min(j1, c.s.nq - 1) - a.window + 1 : 0;
+    full_lo = a.window ? (int)max((long long)c.s.len - c.s.nq + min(j1, c.s.nq - 1) - a.window + 1, 0LL) : 0;
   };
 
-  auto chunk = [&](const uint8_t* st, int tok0, unsigned mask) {
+  // FULL: every row sees every key of the chunk
+  auto chunk = [&](auto full_tag, const uint8_t* st, int tok0, unsigned mask) {
+    constexpr bool FULL = decltype(full_tag)::value;
     const uint8_t* const kp = st + 2 * SH::CODE_BYTES;
     const uint8_t* const vp = kp + SH::PARAM_BYTES;
-    const bool full = mask == (1u << pieces) - 1 && tok0 + CT - 1 <= full_hi && tok0 >= full_lo;
     const int pg = g ^ (g >> 1 & 1);                 // the key of operand row g: neighbours alternate, which spreads the value rows over the banks
     float p[MT][NT][4];
-    float2 sv[MT][2];
+    uint32_t vb[MT][2];                              // scale and minimum of the values
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const int r0 = mt * 16 + pg;
@@ -367,31 +429,31 @@ __global__ void __launch_bounds__(SH::W * 32) kv4_attention_kernel(const AttnArg
       }
       float acc[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.0f;
-#pragma unroll
       for (int w = 0; w < KWORDS; ++w) {
         const uint32_t x = k0[w], y = k1[w], x8 = x >> 8, y8 = y >> 8;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          mma_16816(acc[nt], x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, qf[nt][2 * w][0], qf[nt][2 * w][1]);
+        for (int nt = 0; nt < NT; ++nt) {
+          if (w == 0)
+            mma_16816_first(acc[nt], x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, qf[nt][0][0], qf[nt][0][1]);
+          else
+            mma_16816(acc[nt], x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, qf[nt][2 * w][0], qf[nt][2 * w][1]);
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
           mma_16816(acc[nt], x8 & 0x000f000fu, y8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x00f000f0u, qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
       }
-      const float2 s0 = pair_of<T>(*reinterpret_cast<const uint32_t*>(kp + r0 * 4)), s1 = pair_of<T>(*reinterpret_cast<const uint32_t*>(kp + (r0 + 8) * 4));
-      sv[mt][0] = pair_of<T>(*reinterpret_cast<const uint32_t*>(vp + r0 * 4));
-      sv[mt][1] = pair_of<T>(*reinterpret_cast<const uint32_t*>(vp + (r0 + 8) * 4));
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int e = 0; e < 2; ++e) {
+        const float2 s = pair_of<T>(*reinterpret_cast<const uint32_t*>(kp + (r0 + 8 * e) * 4));
+        vb[mt][e] = *reinterpret_cast<const uint32_t*>(vp + (r0 + 8 * e) * 4);
+        const Two s2(s.x), m2(s.y);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 s = i < 2 ? s0 : s1;
-          p[mt][nt][i] = fmaf(acc[nt][i], s.x * qa[nt][i & 1], s.y * qb[nt][i & 1]);
+        for (int nt = 0; nt < NT; ++nt) {
+          const float2 x = fma2(Two(acc[nt][2 * e], acc[nt][2 * e + 1]), s2 * qa[nt], m2 * qb[nt]).both();
+          p[mt][nt][2 * e] = x.x;
+          p[mt][nt][2 * e + 1] = x.y;
         }
-      }
-      if (!full) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
+        if constexpr (!FULL) {
           const int tok = tok0 + r0 + 8 * e;
           const bool there = mask >> ((r0 + 8 * e) / psz) & 1u;
 #pragma unroll
@@ -399,7 +461,7 @@ __global__ void __launch_bounds__(SH::W * 32) kv4_attention_kernel(const AttnArg
 #pragma unroll
             for (int i = 0; i < 2; ++i)
               if (!there || tok > hi[nt][i] || tok < lo[nt][i]) p[mt][nt][2 * e + i] = -CUDART_INF_F;
-          if (!there || tok >= c.s.len) sv[mt][e] = make_float2(0.0f, 0.0f);     // nothing was fetched, or nothing was ever written
+          if (!there || tok >= c.s.len) vb[mt][e] = 0;     // nothing was fetched, or nothing was ever written
         }
       }
     }
@@ -416,14 +478,15 @@ __global__ void __launch_bounds__(SH::W * 32) kv4_attention_kernel(const AttnArg
         grows = grows || top[nt][i] > mx[nt][i];
       }
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float s = fabsf(sv[mt][e].x);
-        if (s <= 3.402823466e38f) big = fmaxf(big, s);
-      }
+    for (int mt = 0; mt < MT; ++mt) big = fmaxf(big, fmaxf(fabsf(pair_of<T>(vb[mt][0]).x), fabsf(pair_of<T>(vb[mt][1]).x)));
     grows = grows || big > sigma;
     if (__any_sync(0xffffffffu, grows)) {
+      big = 0.0f;                                    // without infinities, which spoil only the rows that see them
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (fabsf(pair_of<T>(vb[mt][e]).x) <= 3.402823466e38f) big = fmaxf(big, fabsf(pair_of<T>(vb[mt][e]).x));
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) {
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
@@ -449,46 +512,54 @@ __global__ void __launch_bounds__(SH::W * 32) kv4_attention_kernel(const AttnArg
           const float m = fmaxf(mx[nt][i], top[nt][i]);
           alpha[i] = mx[nt][i] == m ? 1.0f : exp2_fast(mx[nt][i] - m);
           mx[nt][i] = m;
-          l[nt][i] *= alpha[i];
-          lm[nt][i] *= alpha[i];
-          alpha[i] *= by;
         }
+        const Two al(alpha[0], alpha[1]), both = al * Two(by);
+        l[nt] = l[nt] * al;
+        lm[nt] = lm[nt] * al;
+        lw[nt] = lw[nt] * both;
 #pragma unroll
-        for (int i = 0; i < VWORDS * 4; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[i][nt][e] *= alpha[e & 1];
+        for (int i = 0; i < VWORDS * 4; ++i) {
+          o[i][nt][0] = o[i][nt][0] * both;
+          o[i][nt][1] = o[i][nt][1] * both;
+        }
       }
     }
     // probabilities, their sums, and the second operand of P V
     uint32_t pf[MT][NT][2];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int nt = 0; nt < NT; ++nt) {
+      const Two minus(mx[nt][0] == -CUDART_INF_F ? 0.0f : -mx[nt][0], mx[nt][1] == -CUDART_INF_F ? 0.0f : -mx[nt][1]);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float w[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float m = mx[nt][i] == -CUDART_INF_F ? 0.0f : mx[nt][i];
-            const float pr = exp2_fast(p[mt][nt][2 * e + i] - m);
-            const bool hidden = !full && p[mt][nt][2 * e + i] == -CUDART_INF_F;      // what it hides may be anything
-            l[nt][i] += pr;
-            lm[nt][i] = hidden ? lm[nt][i] : fmaf(pr, sv[mt][e].y, lm[nt][i]);
-            w[i] = hidden ? 0.0f : pr * (sv[mt][e].x * inv_sigma);
+          const float2 x = (Two(p[mt][nt][2 * e], p[mt][nt][2 * e + 1]) + minus).both();
+          const Two pr(exp2_fast(x.x), exp2_fast(x.y));
+          l[nt] = l[nt] + pr;
+          const float2 sv = pair_of<T>(vb[mt][e]);
+          Two w2 = pr * Two(sv.x * inv_sigma), pm = pr * Two(sv.y);
+          if constexpr (FULL) {
+            lm[nt] = lm[nt] + pm;
+          } else {                                   // what a row does not see may be anything
+            const bool h0 = p[mt][nt][2 * e] == -CUDART_INF_F, h1 = p[mt][nt][2 * e + 1] == -CUDART_INF_F;
+            const float2 w = w2.both(), m = pm.both();
+            w2 = Two(h0 ? 0.0f : w.x, h1 ? 0.0f : w.y);
+            lm[nt] = lm[nt] + Two(h0 ? 0.0f : m.x, h1 ? 0.0f : m.y);
           }
-          pf[mt][nt][e] = transpose8x8(pack_half2(w[0], w[1]));
+          const float2 w = w2.both();
+          const uint32_t h = pack_half2(w.x, w.y);
+          if constexpr (KEEP_ROUNDING) {
+            const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&h));
+            lw[nt] = lw[nt] + (w2 + Two(-r.x, -r.y));
+          }
+          pf[mt][nt][e] = transpose8x8(h);
         }
-      }
+    }
     const uint8_t* const vs = st + SH::CODE_BYTES + g * (4 * VWORDS);
     const int x0 = 2 * t ^ (t & 1), y0 = x0 ^ 1;
 #pragma unroll
     for (int j = 0; j < VWORDS; ++j) {
       float part[4][NT][4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) part[i][nt][0] = part[i][nt][1] = part[i][nt][2] = part[i][nt][3] = 0.0f;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         const uint8_t* const at = vs + mt * 16 * KROW + 4 * j;
@@ -499,70 +570,105 @@ __global__ void __launch_bounds__(SH::W * 32) kv4_attention_kernel(const AttnArg
         for (int i = 0; i < 4; ++i) {
           const uint32_t u = (i < 2 ? a01 : a23) >> (8 * (i & 1)), v = (i < 2 ? b01 : b23) >> (8 * (i & 1));
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            mma_16816(part[i][nt], u & 0x000f000fu, u & 0x00f000f0u, v & 0x000f000fu, v & 0x00f000f0u, pf[mt][nt][0], pf[mt][nt][1]);
+          for (int nt = 0; nt < NT; ++nt) {
+            if (mt == 0)
+              mma_16816_first(part[i][nt], u & 0x000f000fu, u & 0x00f000f0u, v & 0x000f000fu, v & 0x00f000f0u, pf[mt][nt][0], pf[mt][nt][1]);
+            else
+              mma_16816(part[i][nt], u & 0x000f000fu, u & 0x00f000f0u, v & 0x000f000fu, v & 0x00f000f0u, pf[mt][nt][0], pf[mt][nt][1]);
+          }
         }
       }
+      // added here, rounded to nearest: the matrix unit cuts off what it adds to a running sum
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[4 * j + i][nt][e] += part[i][nt][e];
+          for (int e = 0; e < 2; ++e) o[4 * j + i][nt][e] = o[4 * j + i][nt][e] + Two(part[i][nt][2 * e], part[i][nt][2 * e + 1]);
     }
   };
 
   // the warps' parts of an item joined, and written as the result or as this CTA's part of it
   auto finish_item = [&](bool whole, int slot) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
+      const float2 l2 = l[nt].both(), m2 = lm[nt].both(), w2 = lw[nt].both();
+      float ls[2] = {l2.x, l2.y}, ms[2] = {m2.x, m2.y};
+      if constexpr (KEEP_ROUNDING) {                 // 7.5, the middle of the codes, times what was lost
+        ms[0] = fmaf(w2.x, 7.5f / 32768.0f * sigma, ms[0]);
+        ms[1] = fmaf(w2.y, 7.5f / 32768.0f * sigma, ms[1]);
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) {
-          l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], x);
-          lm[nt][i] += __shfl_xor_sync(0xffffffffu, lm[nt][i], x);
+          ls[i] += __shfl_xor_sync(0xffffffffu, ls[i], x);
+          ms[i] += __shfl_xor_sync(0xffffffffu, ms[i], x);
         }
-        const int row = nt * 8 + 2 * t + i;
-        if (g == 0) stats[warp * ROWS + row] = make_float4(mx[nt][i], l[nt][i], lm[nt][i], 0.0f);
-        float* const dst = merge + (warp * ROWS + row) * SH::MERGE_ROW + g * (D / 8);
-        const float by = 512.0f * sigma;
-#pragma unroll
-        for (int j = 0; j < VWORDS * 4; ++j)
-          *reinterpret_cast<float2*>(dst + 2 * j) = make_float2(o[j][nt][i] * by, o[j][nt][2 + i] * (by * 0.0625f));
+        if (g == 0) stats[warp * ROWS + nt * 8 + 2 * t + i] = make_float4(mx[nt][i], ls[i], ms[i], 0.0f);
       }
+    }
     __syncthreads();
+#pragma unroll 1
+    for (int round = 0; round < 2; ++round) {
+      if (warp / SH::MERGES == round) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int row = nt * 8 + 2 * t + i;
+            float m = -CUDART_INF_F;
+#pragma unroll
+            for (int w = 0; w < W; ++w) m = fmaxf(m, stats[w * ROWS + row].x);
+            const float by = m == -CUDART_INF_F ? 0.0f : 512.0f * sigma * exp2_fast(mx[nt][i] - m), by16 = by * 0.0625f;
+            float* const dst = merge + (warp % SH::MERGES * ROWS + row) * SH::MERGE_ROW + 2 * g;       // pair j of lane g's channels at 16 j + 2 g
+            float2 old[VWORDS * 4];
+#pragma unroll
+            for (int j = 0; j < VWORDS * 4; ++j) old[j] = round ? *reinterpret_cast<const float2*>(dst + 16 * j) : make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int j = 0; j < VWORDS * 4; ++j) {
+              const float2 even = o[j][nt][0].both(), odd = o[j][nt][1].both();
+              *reinterpret_cast<float2*>(dst + 16 * j) = make_float2(fmaf(i ? even.y : even.x, by, old[j].x), fmaf(i ? odd.y : odd.x, by16, old[j].y));
+            }
+          }
+      }
+      __syncthreads();
+    }
     constexpr int QUADS = D / 4;
+#pragma unroll 2
     for (int i = tid; i < ROWS * QUADS; i += W * 32) {
-      const int row = i / QUADS, d = i % QUADS * 4;
+      const int row = i / QUADS, quad = i % QUADS;   // channels 4 quad .. 4 quad + 3
       const int r = c.tile * ROWS + row, j = r / a.each;
       if (j >= c.s.nq) continue;
-      float m = -CUDART_INF_F;
+      const int at = quad % (D / 32) * 32 + quad / (D / 32) * 2;
+      float m = -CUDART_INF_F, weight = 0.0f, add = 0.0f;
 #pragma unroll
       for (int w = 0; w < W; ++w) m = fmaxf(m, stats[w * ROWS + row].x);
-      float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      float weight = 0.0f;
-      if (m != -CUDART_INF_F) {
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-          const float4 st = stats[w * ROWS + row];
-          const float by = exp2_fast(st.x - m);
-          const float4 v = *reinterpret_cast<const float4*>(merge + (w * ROWS + row) * SH::MERGE_ROW + d);
-          weight = fmaf(st.y, by, weight);
-          sum.x = fmaf(v.x + st.z, by, sum.x);
-          sum.y = fmaf(v.y + st.z, by, sum.y);
-          sum.z = fmaf(v.z + st.z, by, sum.z);
-          sum.w = fmaf(v.w + st.z, by, sum.w);
-        }
+      for (int w = 0; w < W; ++w) {
+        const float4 st = stats[w * ROWS + row];
+        const float by = m == -CUDART_INF_F ? 0.0f : exp2_fast(st.x - m);
+        weight = fmaf(st.y, by, weight);
+        add = fmaf(st.z, by, add);
+      }
+      float4 sum = make_float4(add, add, add, add);
+#pragma unroll
+      for (int w = 0; w < SH::MERGES; ++w) {
+        const float* const src = merge + (w * ROWS + row) * SH::MERGE_ROW + at;
+        const float2 u = *reinterpret_cast<const float2*>(src), v = *reinterpret_cast<const float2*>(src + 16);
+        sum.x += u.x;
+        sum.y += u.y;
+        sum.z += v.x;
+        sum.w += v.y;
       }
       if (whole) {
         const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
-        T* const dst = reinterpret_cast<T*>(a.out) + ((long long)(c.s.q0 + j) * a.q_heads + c.head * a.each + r - j * a.each) * D + d;
+        T* const dst = reinterpret_cast<T*>(a.out) + ((long long)(c.s.q0 + j) * a.q_heads + c.head * a.each + r - j * a.each) * D + 4 * quad;
         T v[4] = {from_float<T>(sum.x * inv), from_float<T>(sum.y * inv), from_float<T>(sum.z * inv), from_float<T>(sum.w * inv)};
         *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(v);
       } else {
-        *reinterpret_cast<float4*>(a.part_o + ((long long)slot * ROWS + row) * D + d) = sum;
-        if (d == 0) a.part_ml[(long long)slot * ROWS + row] = make_float2(m, weight);
+        *reinterpret_cast<float4*>(a.part_o + ((long long)slot * ROWS + row) * D + 4 * quad) = sum;
+        if (quad == 0) a.part_ml[(long long)slot * ROWS + row] = make_float2(m, weight);
       }
     }
     __syncthreads();
@@ -572,7 +678,7 @@ __global__ void __launch_bounds__(SH::W * 32) kv4_attention_kernel(const AttnArg
   bool opens = true;
   int from_unit = 0;
 #pragma unroll 1
-  for (long long u = u0; u < u1; ++u) {
+  for (unsigned u = u0; u < u1; ++u) {
     if (opens) {
       start_item();
       from_unit = c.unit;
@@ -585,7 +691,13 @@ __global__ void __launch_bounds__(SH::W * 32) kv4_attention_kernel(const AttnArg
         if (lane == 0 && a.status) *a.status = 1u;
       }
       phases ^= 1u << stage;
-      if (!dead) chunk(ring + stage * SH::STAGE, c.s.first + (c.unit * W + warp) * CT, mask);
+      const int tok0 = c.s.first + ((c.unit - kOpening) * W + warp) * CT;
+      if (!dead) {
+        if (mask == all_pieces && tok0 + CT - 1 <= full_hi && tok0 >= full_lo)
+          chunk(std::true_type(), ring + stage * SH::STAGE, tok0, mask);
+        else
+          chunk(std::false_type(), ring + stage * SH::STAGE, tok0, mask);
+      }
       __syncwarp();
     }
     issue(stage);
@@ -602,30 +714,28 @@ __global__ void __launch_bounds__(SH::W * 32) kv4_attention_kernel(const AttnArg
 
 // Joins the parts of an item that several CTAs of the kernel above worked on: one block per item and row.
 template <typename T, typename SH>
-__global__ void __launch_bounds__(128) kv4_attention_join_kernel(const AttnArgs a, int ctas) {
+__global__ void __launch_bounds__(128) kv4_attention_join_kernel(const AttnArgs a, unsigned ctas) {
   constexpr int D = SH::D, ROWS = SH::ROWS, PER = D / 32;
   __shared__ float sums[4][D];
   __shared__ float2 ml[4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y;
   grid_launch_dependents();
   grid_dependency_wait();
+  Sequence mine = {};
+  const Deal deal_ = deal<ROWS, SH::UNIT, SH::CT>(a, lane, ctas, mine);
   Walk w;
-  long long u0 = 0;
-  if (!place<ROWS, SH::UNIT, SH::CT>(a, lane, blockIdx.x, true, w, u0)) return;
-  const long long total = count_units<ROWS, SH::UNIT, SH::CT>(a, lane);
+  unsigned u0 = 0;
+  if (!place<ROWS, SH::UNIT, SH::CT>(a, lane, mine, blockIdx.x, true, w, u0)) return;
   const int r = w.tile * ROWS + row, j = r / a.each;
   if (j >= w.s.nq) return;
-  const long long u1 = u0 + w.s.units;
-  const int i0 = (int)(((u0 + 1) * ctas - 1) / total), i1 = (int)((u1 * ctas - 1) / total);
+  const int i0 = (int)deal_.owner(u0), i1 = (int)deal_.owner(u0 + w.s.units - 1);
   if (i0 == i1) return;                        // one CTA had it all and has written it
   float m = -CUDART_INF_F, weight = 0.0f;
   float sum[PER];
 #pragma unroll
   for (int e = 0; e < PER; ++e) sum[e] = 0.0f;
   for (int i = i0 + warp; i <= i1; i += 4) {
-    const long long start = share(total, i, ctas);
-    if (start == share(total, i + 1, ctas)) continue;            // fewer units than CTAs: this one had none
-    const int slot = 2 * i + (start > u0 ? 0 : 1);
+    const int slot = 2 * i + (deal_.start(i) > u0 ? 0 : 1);
     const float2 s = a.part_ml[(long long)slot * ROWS + row];
     float v[PER];
     const float* src = a.part_o + ((long long)slot * ROWS + row) * D + lane * PER;
@@ -660,16 +770,23 @@ __global__ void __launch_bounds__(128) kv4_attention_join_kernel(const AttnArgs 
   }
 }
 
-constexpr int kCtasPerSm = 2;
+constexpr int kMostPerSm = 2;      // CTAs of any shape on an SM
 
+// Two CTAs of four warps on an SM, with all the registers that leaves.  Keys per chunk: 64 for one 8-row tile of up to 128 channels (two
+// documents of 131,071 keys, 64 query heads on 8: 71 us; chunks of 32 keys with three CTAs of 168 registers: 81; with 64 keys, two CTAs of
+// two warps: 78), fewer where the sums of a chunk take more registers.
 template <int D, int NT>
-using Few = Shape<D, NT, 4, D == 256 ? 16 : 32, 4>;
+using Few = Shape<D, NT, 4, D == 256 ? 16 : NT == 1 ? 64 : 32, D * NT == 128 ? 3 : 4, 2>;
 
 template <typename T, int D, int NT>
 int run(AttnArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
   using SH = Few<D, NT>;
-  static_assert(SH::SMEM <= 113 * 1024, "two CTAs per SM");
-  const int ctas = kCtasPerSm * sm_count();
+  static_assert((SH::SMEM + 1024) * SH::PER_SM <= 228 * 1024 && SH::PER_SM <= kMostPerSm, "resident together");
+  // as many items as there can be: full tiles, and one that is not full per sequence
+  const long long tiles = a.query_starts ? (long long)a.tokens * a.each / SH::ROWS + a.batch : (long long)a.batch * ceil_div(a.each, SH::ROWS);
+  const long long items = tiles * a.kv_heads, units = items * (((long long)a.table_width << a.page_shift) / SH::UNIT + 1 + kOpening);
+  XQT_REQUIRE(items < (1LL << 31) - 1 && units < (1LL << 31));
+  const int ctas = (int)min((long long)SH::PER_SM * sm_count(), units);
   const size_t o_bytes = (size_t)2 * ctas * SH::ROWS * D * 4;
   XQT_REQUIRE(workspace && workspace_bytes >= o_bytes + (size_t)2 * ctas * SH::ROWS * 8 && ((uintptr_t)workspace & 15) == 0);
   a.part_o = reinterpret_cast<float*>(workspace);
@@ -677,10 +794,7 @@ int run(AttnArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream
   XQT_SMEM_OPT_IN((kv4_attention_kernel<T, SH>), SH::SMEM);
   int rc = launch_pdl(kv4_attention_kernel<T, SH>, dim3((unsigned)ctas), dim3(SH::W * 32), SH::SMEM, stream, a);
   if (rc) return rc;
-  // as many items as there can be: full tiles, and one that is not full per sequence
-  const long long tiles = a.query_starts ? (long long)a.tokens * a.each / SH::ROWS + a.batch : (long long)a.batch * ceil_div(a.each, SH::ROWS);
-  XQT_REQUIRE(tiles * a.kv_heads < (1LL << 31) - 1);
-  return launch_pdl(kv4_attention_join_kernel<T, SH>, dim3((unsigned)(tiles * a.kv_heads), SH::ROWS), dim3(128), 0, stream, a, ctas);
+  return launch_pdl(kv4_attention_join_kernel<T, SH>, dim3((unsigned)items, SH::ROWS), dim3(128), 0, stream, a, (unsigned)ctas);
 }
 
 template <typename T>
@@ -697,7 +811,7 @@ int run_dim(const AttnArgs& a, int dim, void* workspace, size_t workspace_bytes,
 
 extern "C" size_t xqt_b200_kv4_attention_workspace_bytes(int dim) {
   using namespace xqt_b200;
-  return (size_t)2 * kCtasPerSm * sm_count() * 16 * (dim + 2) * 4;
+  return (size_t)2 * kMostPerSm * sm_count() * 16 * (dim + 2) * 4;
 }
 
 extern "C" int xqt_b200_kv4_attention(const void* q, const void* codes, const void* params, const int* table, const int* seq_lens, const int* query_starts,
@@ -709,7 +823,7 @@ extern "C" int xqt_b200_kv4_attention(const void* q, const void* codes, const vo
   XQT_REQUIRE(dim == 64 || dim == 128 || dim == 256);
   XQT_REQUIRE(dtype == XQT_B200_FP16 || dtype == XQT_B200_BF16);
   XQT_REQUIRE(page_size >= 16 && page_size <= 4096 && (page_size & (page_size - 1)) == 0);
-  XQT_REQUIRE(pages >= 0 && pages < (1LL << 31) && table_width >= 0 && (long long)table_width * page_size < (1LL << 31) - 4096);
+  XQT_REQUIRE(pages >= 0 && pages < (1LL << 31) && table_width >= 0 && (long long)table_width * page_size <= (1LL << 30));
   XQT_REQUIRE(window >= 0 && (long long)tokens * (q_heads / kv_heads) < (1LL << 31) - 4096);
   if (tokens == 0 || batch == 0) return 0;
   XQT_REQUIRE(q && out && seq_lens && strides && (table_width == 0 || table) && (pages == 0 || (codes && params)));

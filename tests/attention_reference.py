@@ -68,63 +68,61 @@ def values(codes, params):
 
 
 def attention(q, codes, params, table, seq_lens, query_starts=None, scale=None, window=None, rounded=None):
-    """-> (result, bound): softmax attention in fp64 row by row, and how far the kernels' arithmetic may take a row.
+    """-> (result, bound): softmax attention in fp64, and how far the kernels' arithmetic may take each value; NaN for rows of no sequence.
 
-    The bound adds up: the last rounding; rounding of p * s (the probabilities times value scales) to fp16, or, with ``rounded`` (a kernel that
-    forms keys, values and probabilities in that type), of those three: independent errors of at most half a step h each, whose sum with
-    weights a_i exceeds 7 h sqrt(sum a_i^2) with a probability below 2 exp(-49 / 2) = 5e-11 (Hoeffding); and fp32 sums, 2^-20 of the sum of the sizes
-    (a score that is off by d moves the row by at most 2 d times the spread of its values)."""
+    The bound adds up: the last rounding; the rounding of p * s (the probabilities times the value scales) to fp16 or, with ``rounded`` (a kernel
+    that forms keys, values and probabilities in that type), of those three: independent errors of at most half a step h each, whose sum
+    with weights a_i exceeds 7 h sqrt(sum a_i^2) with a probability below 2 exp(-49 / 2) = 5e-11 (Hoeffding); and fp32 sums, 2^-20 of the sum of
+    the sizes (a score that is off by d moves the row by at most 2 d times the spread of its values)."""
 
+    device = q.device
     pages, _, heads, page, _ = codes.shape
     tokens, q_heads, dim = q.shape
     each, batch = q_heads // heads, table.shape[0]
-    qd, table, lens = q.detach().cpu().double(), table.cpu(), seq_lens.cpu().tolist()
-    starts = list(range(batch + 1)) if query_starts is None else query_starts.cpu().tolist()
+    table, lens = table.to(device), seq_lens.tolist()
+    starts = list(range(batch + 1)) if query_starts is None else query_starts.tolist()
     scale = dim ** -0.5 if scale is None else scale
-    held, par = unpack(codes.cpu()).double(), params.cpu().double()
-    out = torch.full(qd.shape, math.nan, dtype=torch.float64)
+    out = torch.full(q.shape, math.nan, dtype=torch.float64, device=device)
     bound = torch.zeros_like(out)
-    h = half_step(q.dtype)
-    hp = half_step(rounded or torch.float16)
-    hr = 0.0 if rounded is None else half_step(rounded)
+    h, hp = half_step(q.dtype), half_step(rounded or torch.float16)
     for b in range(batch):
         n = min(max(lens[b], 0), table.shape[1] * page)
         q0 = min(max(starts[b], 0), tokens)
         m = min(max(starts[b + 1], q0), tokens) - q0
-        at = torch.arange(n)
+        if not m:
+            continue
+        at = torch.arange(n, device=device)
         ids = table[b][at // page].long()
         there = (ids >= 0) & (ids < pages)
-        ids = ids.clamp(0, max(pages - 1, 0))
-        for i in range(m):
-            mine = n - m + i
-            seen = there & (at <= mine)
-            if window is not None:
-                seen &= at > mine - window
-            rows, pg = at[seen] % page, ids[seen]
-            for kh in range(heads):
-                sl = slice(kh * each, (kh + 1) * each)
-                if not len(pg):
-                    out[q0 + i, sl] = 0
-                    continue
-                ks, km = par[pg, 0, kh, rows, 0], par[pg, 0, kh, rows, 1]
-                vs, vm = par[pg, 1, kh, rows, 0], par[pg, 1, kh, rows, 1]
-                k = held[pg, 0, kh, rows] * ks[:, None] + km[:, None]
-                vc = held[pg, 1, kh, rows] * vs[:, None]
-                v = vc + vm[:, None]
-                x = qd[q0 + i, sl]
-                s = x @ k.T * scale
-                p = s.softmax(-1)
-                y = p @ v
-                out[q0 + i, sl] = y
-                spread = p @ v.abs() + y.abs()
-                size = scale * x.abs().sum(-1, keepdim=True) * (15 * ks + km.abs()).max()
-                bad = 2 * 2.0 ** -20 * size * spread + 2.0 ** -20 * (p @ (vc.abs() + vm.abs()[:, None])) + h * y.abs() * (1 + 2.0 ** -6) + 2.0 ** -25
-                weights = vc if rounded is None else v.abs()
-                bad = bad + 7 * hp * (p.square() @ weights.square()).sqrt()
-                if rounded is not None:
-                    # values (p_t v_t), and keys: a score moves by at most 7 hr sqrt(sum (q k)^2) scale, which moves the row by p_t (v_t - y)
-                    moved = 7 * hr * scale * (x.square() @ k.square().T).sqrt()
-                    spread2 = torch.stack([(p[e].square() * moved[e].square()) @ (v - y[e]).square() for e in range(each)]).sqrt()
-                    bad = bad + 7 * hr * (p.square() @ v.square()).sqrt() + spread2 * 2
-                bound[q0 + i, sl] = bad
+        ids, rows = ids.clamp(0, max(pages - 1, 0)), at % page
+        mine = n - m + torch.arange(m, device=device)[:, None]
+        seen = there & (at <= mine)
+        if window is not None:
+            seen = seen & (at > mine - window)
+        anything = seen.any(1)
+        used = seen.any(0)
+        seen, ids, rows = seen[:, used][:, None], ids[used], rows[used]
+        for kh in range(heads):
+            sl = slice(kh * each, (kh + 1) * each)
+            (ks, km), (vs, vm) = (params[ids, i, kh, rows].to(device).double().unbind(-1) for i in (0, 1))
+            (kc, vc) = (unpack(codes[ids, i, kh, rows].to(device)).double() for i in (0, 1))
+            k, vc = kc * ks[:, None] + km[:, None], vc * vs[:, None]
+            v = vc + vm[:, None]
+            x = q[q0:q0 + m, sl].double()
+            s = (x @ k.T * scale).masked_fill(~seen, -math.inf)
+            p = s.softmax(-1) if len(ids) else s
+            p = torch.where(anything[:, None, None] & seen, p, 0.0)
+            y = p @ v
+            out[q0:q0 + m, sl] = y
+            spread = p @ v.abs() + y.abs()
+            size = scale * x.abs().sum(-1, keepdim=True) * (15 * ks.abs() + km.abs()).max() if len(ids) else 0
+            bad = 2 * 2.0 ** -20 * abs(size) * spread + 2.0 ** -20 * (p @ (vc.abs() + vm.abs()[:, None])) + h * y.abs() * (1 + 2.0 ** -6) + 2.0 ** -25
+            weights = vc if rounded is None else torch.maximum(vc.abs(), v.abs())
+            bad = bad + 7 * hp * (p.square() @ weights.square()).sqrt()
+            if rounded is not None:
+                # values (p_t v_t), and keys: a score's error has deviations of hp sqrt(sum (q k)^2) scale, which moves the row by p_t (v_t - y)
+                moved = p.square() * (scale ** 2 * (x.square() @ k.square().T))
+                second = (moved @ v.square() - 2 * y * (moved @ v) + y.square() * moved.sum(-1, keepdim=True)).clamp(min=0).sqrt()
+                bad = bad + 7 * hp * ((p.square() @ v.square()).sqrt() + second)
+            bound[q0:q0 + m, sl] = bad
     return out, bound

@@ -18,41 +18,14 @@
 // CTAs share are joined by a second kernel.  Each warp fetches its own chunks with bulk copies, S of them ahead.
 //
 // Bound by HBM: (dim + 8) bytes per key and head.
-#include <limits.h>
-#include <math_constants.h>
-
-#include <type_traits>
-
-#include "common.cuh"
-#include "sm100.cuh"
+#include "kv4_attention.cuh"
 
 namespace xqt_b200 {
 
 namespace {
 
-using namespace sm100;
+using namespace kv4;
 
-struct AttnArgs {
-  const void* q;
-  const uint8_t* codes;
-  const uint8_t* params;
-  const int* table;
-  const int* seq_lens;
-  const int* query_starts;   // null: one query per sequence
-  void* out;
-  float* part_o;             // [2 * CTAs][ROWS][D]
-  float2* part_ml;           // [2 * CTAs][ROWS]
-  unsigned* status;
-  long long q_token, q_head, pages, table_stride;
-  int tokens, batch, q_heads, kv_heads, each, page_size, page_shift, table_width, window;
-  float scale;               // times log2(e)
-};
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -73,32 +46,13 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];\n" ::"l"(p)); }
-// a pair of floats as the packed instructions take it
-struct Two {
-  unsigned long long v;
-  __device__ __forceinline__ Two() {}
-  __device__ __forceinline__ Two(float a, float b) : v(f32x2_pack(a, b)) {}
-  __device__ __forceinline__ explicit Two(float a) : v(f32x2_pack(a, a)) {}
-  __device__ __forceinline__ float2 both() const {
-    float2 f;
-    f32x2_unpack(v, f.x, f.y);
-    return f;
-  }
-};
-__device__ __forceinline__ Two operator*(Two a, Two b) { Two r; r.v = f32x2_mul(a.v, b.v); return r; }
-__device__ __forceinline__ Two operator+(Two a, Two b) { Two r; r.v = f32x2_add(a.v, b.v); return r; }
-__device__ __forceinline__ Two fma2(Two a, Two b, Two c) { Two r; r.v = f32x2_fma(a.v, b.v, c.v); return r; }
-template <typename T>
-__device__ __forceinline__ float2 pair_of(uint32_t bits) {
-  const T* e = reinterpret_cast<const T*>(&bits);
-  return make_float2(to_float<T>(e[0]), to_float<T>(e[1]));
-}
-
 template <int D_, int NT_, int W_, int CT_, int S_, int PER_SM_>
 struct Shape {
   static constexpr int D = D_, NT = NT_, W = W_, CT = CT_, S = S_, PER_SM = PER_SM_;
   static constexpr int ROWS = 8 * NT, KROW = D / 2, KWORDS = D / 32, VWORDS = D / 64, MT = CT / 16;
   static constexpr int UNIT = W * CT;
+  static constexpr int OPENING = 1;                      // a unit for an item's beginning and end: its queries read, its warps joined
+  static constexpr bool PROMPT = false;
   static constexpr int CODE_BYTES = CT * KROW, PARAM_BYTES = CT * 4, STAGE = 2 * (CODE_BYTES + PARAM_BYTES);
   static constexpr int MERGE_ROW = D + 8;
   static constexpr int MERGES = W / 2;                    // buffers: the warps write them in two rounds
@@ -106,113 +60,7 @@ struct Shape {
   static constexpr int SMEM = W * S * STAGE + MERGE_BYTES + STAT_BYTES + W * S * 8;
 };
 
-// Units that stand for an item's beginning and end (its queries read, its warps joined): they go first and have no keys.
-constexpr int kOpening = 1;
-
-// A sequence as the work list sees it.
-struct Sequence {
-  int q0, nq, len, first, tiles, units;   // `first`: where its units start; units per (tile, head) item
-};
-
-template <int ROWS, int UNIT, int CT>
-__device__ __forceinline__ Sequence sequence(const AttnArgs& a, int b) {
-  Sequence s;
-  if (a.query_starts) {
-    const int lo = min(max(a.query_starts[b], 0), a.tokens);
-    s.q0 = lo;
-    s.nq = min(max(a.query_starts[b + 1], lo), a.tokens) - lo;
-  } else {
-    s.q0 = b;
-    s.nq = 1;
-  }
-  const long long most = (long long)a.table_width << a.page_shift;
-  s.len = (int)min((long long)max(a.seq_lens[b], 0), most);
-  const long long from = a.window ? (long long)s.len - s.nq + 1 - a.window : 0;
-  s.first = from > 0 ? (int)(from / CT * CT) : 0;
-  s.tiles = (int)(((long long)s.nq * a.each + ROWS - 1) / ROWS);
-  s.units = max((s.len - s.first + UNIT - 1) / UNIT, 0) + kOpening;   // an empty sequence still has its rows written
-  return s;
-}
-
-// A place in the work list.
-struct Walk {
-  int b, tile, head, unit;
-  Sequence s;
-};
-
-// The list: its units are dealt out in equal contiguous runs, the first `more` CTAs one unit longer.  32 bits: the host refuses more.
-struct Deal {
-  unsigned total, each, more;
-  __device__ __forceinline__ unsigned start(unsigned i) const { return each * i + min(i, more); }
-  __device__ __forceinline__ unsigned owner(unsigned u) const {
-    const unsigned long_run = more * (each + 1);
-    return u < long_run ? u / (each + 1) : more + (u - long_run) / max(each, 1u);
-  }
-};
-
-__device__ __forceinline__ unsigned scan32(unsigned v, int lane) {
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const unsigned x = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += x;
-  }
-  return v;
-}
-
-template <int ROWS, int UNIT, int CT>
-__device__ __forceinline__ Deal deal(const AttnArgs& a, int lane, unsigned ctas, Sequence& mine) {
-  Deal d = {};
-  for (int b0 = (a.batch - 1) & ~31; b0 >= 0; b0 -= 32) {      // backwards: `mine` ends as sequence `lane`
-    unsigned units = 0;
-    if (b0 + lane < a.batch) {
-      mine = sequence<ROWS, UNIT, CT>(a, b0 + lane);
-      units = (unsigned)mine.tiles * a.kv_heads * mine.units;
-    }
-    d.total += __reduce_add_sync(0xffffffffu, units);
-  }
-  d.each = d.total / ctas;
-  d.more = d.total - d.each * ctas;
-  return d;
-}
-
-// The place of unit `u`, or with by_item of item (tile, head) number `u`; `before` gets the units in front of it.
-template <int ROWS, int UNIT, int CT>
-__device__ __forceinline__ bool place(const AttnArgs& a, int lane, const Sequence& mine, unsigned u, bool by_item, Walk& w, unsigned& before) {
-  unsigned base = 0, base_units = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 32) {
-    Sequence s = mine;
-    unsigned items = 0, units = 0;
-    if (b0 + lane < a.batch) {
-      if (b0 > 0) s = sequence<ROWS, UNIT, CT>(a, b0 + lane);
-      items = (unsigned)s.tiles * a.kv_heads;
-      units = items * s.units;
-    }
-    const unsigned cum_units = scan32(units, lane), n = by_item ? items : units, cum = by_item ? scan32(items, lane) : cum_units;
-    const unsigned over = __ballot_sync(0xffffffffu, base + cum > u);
-    if (over) {
-      const int at = __ffs(over) - 1;
-      const unsigned rest = u - base - __shfl_sync(0xffffffffu, cum - n, at);
-      w.b = b0 + at;
-      w.s.q0 = __shfl_sync(0xffffffffu, s.q0, at);
-      w.s.nq = __shfl_sync(0xffffffffu, s.nq, at);
-      w.s.len = __shfl_sync(0xffffffffu, s.len, at);
-      w.s.first = __shfl_sync(0xffffffffu, s.first, at);
-      w.s.tiles = __shfl_sync(0xffffffffu, s.tiles, at);
-      w.s.units = __shfl_sync(0xffffffffu, s.units, at);
-      const unsigned item = by_item ? rest : rest / (unsigned)w.s.units;
-      w.unit = by_item ? 0 : (int)(rest - item * w.s.units);
-      w.tile = (int)(item / (unsigned)a.kv_heads);
-      w.head = (int)(item - (unsigned)w.tile * a.kv_heads);
-      before = base_units + __shfl_sync(0xffffffffu, cum_units - units, at) + item * w.s.units;
-      return true;
-    }
-    base += __shfl_sync(0xffffffffu, cum, 31);
-    base_units += __shfl_sync(0xffffffffu, cum_units, 31);
-  }
-  return false;
-}
-
-template <int ROWS, int UNIT, int CT>
+template <typename L>
 __device__ __forceinline__ void advance(const AttnArgs& a, Walk& w) {
   if (++w.unit < w.s.units) return;
   w.unit = 0;
@@ -221,7 +69,7 @@ __device__ __forceinline__ void advance(const AttnArgs& a, Walk& w) {
   if (++w.tile < w.s.tiles) return;
   w.tile = 0;
   while (++w.b < a.batch) {
-    w.s = sequence<ROWS, UNIT, CT>(a, w.b);
+    w.s = sequence<L>(a, w.b);
     if (w.s.tiles > 0) return;
   }
 }
@@ -245,12 +93,12 @@ __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(c
   grid_dependency_wait();
 
   Sequence mine = {};
-  const Deal d = deal<ROWS, SH::UNIT, CT>(a, lane, gridDim.x, mine);
+  const Deal d = deal<SH>(a, lane, gridDim.x, mine);
   const unsigned u0 = d.start(blockIdx.x), u1 = d.start(blockIdx.x + 1);
   if (u0 >= u1) return;
   Walk c;
   unsigned unused;
-  if (!place<ROWS, SH::UNIT, CT>(a, lane, mine, u0, false, c, unused)) return;
+  if (!place<SH>(a, lane, mine, u0, false, c, unused)) return;
 
   // ---- fetching
   const int psz = min(a.page_size, CT), pieces = CT / psz;
@@ -267,7 +115,7 @@ __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(c
   auto open = [&]() {
     const int j0 = f.tile * ROWS / a.each, j1 = min(f.s.nq - 1, (f.tile * ROWS + ROWS - 1) / a.each);
     f_units = f.s.units - f.unit;
-    f_at = piece < pieces ? f.s.first + ((f.unit - kOpening) * W + warp) * CT + piece * psz : INT_MAX - (1 << 24);
+    f_at = piece < pieces ? f.s.first + ((f.unit - SH::OPENING) * W + warp) * CT + piece * psz : INT_MAX - (1 << 24);
     f_end = f.b < a.batch ? f.s.len - f.s.nq + j1 + 1 : 0;      // (starts that do not ascend can make the list shorter than it counts)
     f_begin = a.window ? (int)max((long long)f.s.len - f.s.nq + j0 - a.window + 1, 0LL) : 0;
     f_table = a.table + f.b * a.table_stride;
@@ -295,7 +143,7 @@ __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(c
         if (piece < pieces) f_at += SH::UNIT;
       } else if (to_fetch > 0) {
         f.unit = f.s.units - 1;
-        advance<ROWS, SH::UNIT, CT>(a, f);
+        advance<SH>(a, f);
         open();
       }
     }
@@ -691,7 +539,7 @@ __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(c
         if (lane == 0 && a.status) *a.status = 1u;
       }
       phases ^= 1u << stage;
-      const int tok0 = c.s.first + ((c.unit - kOpening) * W + warp) * CT;
+      const int tok0 = c.s.first + ((c.unit - SH::OPENING) * W + warp) * CT;
       if (!dead) {
         if (mask == all_pieces && tok0 + CT - 1 <= full_hi && tok0 >= full_lo)
           chunk(std::true_type(), ring + stage * SH::STAGE, tok0, mask);
@@ -708,7 +556,7 @@ __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(c
       finish_item(ends && from_unit == 0, 2 * blockIdx.x + (from_unit == 0 ? 1 : 0));
       opens = true;
     }
-    advance<ROWS, SH::UNIT, CT>(a, c);
+    advance<SH>(a, c);
   }
 }
 
@@ -722,10 +570,10 @@ __global__ void __launch_bounds__(128) kv4_attention_join_kernel(const AttnArgs 
   grid_launch_dependents();
   grid_dependency_wait();
   Sequence mine = {};
-  const Deal deal_ = deal<ROWS, SH::UNIT, SH::CT>(a, lane, ctas, mine);
+  const Deal deal_ = deal<SH>(a, lane, ctas, mine);
   Walk w;
   unsigned u0 = 0;
-  if (!place<ROWS, SH::UNIT, SH::CT>(a, lane, mine, blockIdx.x, true, w, u0)) return;
+  if (!place<SH>(a, lane, mine, blockIdx.x, true, w, u0)) return;
   const int r = w.tile * ROWS + row, j = r / a.each;
   if (j >= w.s.nq) return;
   const int i0 = (int)deal_.owner(u0), i1 = (int)deal_.owner(u0 + w.s.units - 1);
@@ -784,7 +632,7 @@ int run(AttnArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream
   static_assert((SH::SMEM + 1024) * SH::PER_SM <= 228 * 1024 && SH::PER_SM <= kMostPerSm, "resident together");
   // as many items as there can be: full tiles, and one that is not full per sequence
   const long long tiles = a.query_starts ? (long long)a.tokens * a.each / SH::ROWS + a.batch : (long long)a.batch * ceil_div(a.each, SH::ROWS);
-  const long long items = tiles * a.kv_heads, units = items * (((long long)a.table_width << a.page_shift) / SH::UNIT + 1 + kOpening);
+  const long long items = tiles * a.kv_heads, units = items * (((long long)a.table_width << a.page_shift) / SH::UNIT + 1 + SH::OPENING);
   XQT_REQUIRE(items < (1LL << 31) - 1 && units < (1LL << 31));
   const int ctas = (int)min((long long)SH::PER_SM * sm_count(), units);
   const size_t o_bytes = (size_t)2 * ctas * SH::ROWS * D * 4;
@@ -852,6 +700,17 @@ extern "C" int xqt_b200_kv4_attention(const void* q, const void* codes, const vo
   a.table_width = table_width;
   a.window = window;
   a.scale = scale * 1.4426950408889634f;
+  // Which sequences go to the prompt kernel.  Its tiles of 128 rows run near the tensor core's rate where they are full and fill the SMs, and one
+  // of its CTAs takes a sequence's keys alone; this file's kernel spreads any sequence over all SMs.
+  a.few_rows = INT_MAX;
+  if (query_starts != nullptr) {
+    const int most = (long long)tokens * q_heads >= 128LL * sm_count() ? 32 : 256;
+    if ((long long)tokens * a.each > most) {
+      a.few_rows = most;
+      const int rc = kv4_prompt_launch(a, dim, dtype, stream);
+      if (rc) return rc;
+    }
+  }
   return dtype == XQT_B200_BF16 ? run_dim<__nv_bfloat16>(a, dim, workspace, workspace_bytes, stream)
                                 : run_dim<__half>(a, dim, workspace, workspace_bytes, stream);
 }

@@ -1,0 +1,171 @@
+// What the two attention kernels over the 4-bit cache share: their arguments, and the list of the work in a batch whose lengths only the
+// device knows.
+#pragma once
+
+#include <limits.h>
+#include <math_constants.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "sm100.cuh"
+
+namespace xqt_b200 {
+namespace kv4 {
+
+using namespace sm100;
+
+struct AttnArgs {
+  const void* q;
+  const uint8_t* codes;
+  const uint8_t* params;
+  const int* table;
+  const int* seq_lens;
+  const int* query_starts;   // null: one query per sequence
+  void* out;
+  float* part_o;             // [2 * CTAs][ROWS][D]
+  float2* part_ml;           // [2 * CTAs][ROWS]
+  unsigned* status;
+  long long q_token, q_head, pages, table_stride;
+  int tokens, batch, q_heads, kv_heads, each, page_size, page_shift, table_width, window, few_rows;     // few_rows: sequences with more rows for a key head go to the prompt kernel
+  float scale;               // times log2(e)
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+// a pair of floats as the packed instructions take it
+struct Two {
+  unsigned long long v;
+  __device__ __forceinline__ Two() {}
+  __device__ __forceinline__ Two(float a, float b) : v(f32x2_pack(a, b)) {}
+  __device__ __forceinline__ explicit Two(float a) : v(f32x2_pack(a, a)) {}
+  __device__ __forceinline__ float2 both() const {
+    float2 f;
+    f32x2_unpack(v, f.x, f.y);
+    return f;
+  }
+};
+__device__ __forceinline__ Two operator*(Two a, Two b) { Two r; r.v = f32x2_mul(a.v, b.v); return r; }
+__device__ __forceinline__ Two operator+(Two a, Two b) { Two r; r.v = f32x2_add(a.v, b.v); return r; }
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) { Two r; r.v = f32x2_fma(a.v, b.v, c.v); return r; }
+template <typename T>
+__device__ __forceinline__ float2 pair_of(uint32_t bits) {
+  const T* e = reinterpret_cast<const T*>(&bits);
+  return make_float2(to_float<T>(e[0]), to_float<T>(e[1]));
+}
+
+// A list's shape L: ROWS of a row tile, UNIT keys of a unit (OPENING units in front of every item have no keys), CT to which an item's first
+// key is rounded down; PROMPT: the sequences with more than few_rows rows, else those with no more.
+
+// A sequence as the work list sees it.
+struct Sequence {
+  int q0, nq, len, first, tiles, units;   // `first`: where its units start; units per (tile, head) item
+};
+
+template <typename L>
+__device__ __forceinline__ Sequence sequence(const AttnArgs& a, int b) {
+  Sequence s;
+  if (a.query_starts) {
+    const int lo = min(max(a.query_starts[b], 0), a.tokens);
+    s.q0 = lo;
+    s.nq = min(max(a.query_starts[b + 1], lo), a.tokens) - lo;
+  } else {
+    s.q0 = b;
+    s.nq = 1;
+  }
+  const long long most = (long long)a.table_width << a.page_shift;
+  s.len = (int)min((long long)max(a.seq_lens[b], 0), most);
+  const long long from = a.window ? (long long)s.len - s.nq + 1 - a.window : 0;
+  s.first = from > 0 ? (int)(from / L::CT * L::CT) : 0;
+  const long long rows = (long long)s.nq * a.each;
+  s.tiles = (L::PROMPT ? rows <= a.few_rows : rows > a.few_rows) ? 0 : (int)((rows + L::ROWS - 1) / L::ROWS);
+  s.units = max((s.len - s.first + L::UNIT - 1) / L::UNIT, 0) + L::OPENING;   // an empty sequence still has its rows written
+  return s;
+}
+
+// A place in the work list.
+struct Walk {
+  int b, tile, head, unit;
+  Sequence s;
+};
+
+// The list: its units are dealt out in equal contiguous runs, the first `more` CTAs one unit longer.  32 bits: the host refuses more.
+struct Deal {
+  unsigned total, each, more;
+  __device__ __forceinline__ unsigned start(unsigned i) const { return each * i + min(i, more); }
+  __device__ __forceinline__ unsigned owner(unsigned u) const {
+    const unsigned long_run = more * (each + 1);
+    return u < long_run ? u / (each + 1) : more + (u - long_run) / max(each, 1u);
+  }
+};
+
+__device__ __forceinline__ unsigned scan32(unsigned v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned x = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += x;
+  }
+  return v;
+}
+
+template <typename L>
+__device__ __forceinline__ Deal deal(const AttnArgs& a, int lane, unsigned ctas, Sequence& mine) {
+  Deal d = {};
+  for (int b0 = (a.batch - 1) & ~31; b0 >= 0; b0 -= 32) {      // backwards: `mine` ends as sequence `lane`
+    unsigned units = 0;
+    if (b0 + lane < a.batch) {
+      mine = sequence<L>(a, b0 + lane);
+      units = (unsigned)mine.tiles * a.kv_heads * mine.units;
+    }
+    d.total += __reduce_add_sync(0xffffffffu, units);
+  }
+  d.each = d.total / ctas;
+  d.more = d.total - d.each * ctas;
+  return d;
+}
+
+// The place of unit `u`, or with by_item of item (tile, head) number `u`; `before` gets the units in front of it.
+template <typename L>
+__device__ __forceinline__ bool place(const AttnArgs& a, int lane, const Sequence& mine, unsigned u, bool by_item, Walk& w, unsigned& before) {
+  unsigned base = 0, base_units = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 32) {
+    Sequence s = mine;
+    unsigned items = 0, units = 0;
+    if (b0 + lane < a.batch) {
+      if (b0 > 0) s = sequence<L>(a, b0 + lane);
+      items = (unsigned)s.tiles * a.kv_heads;
+      units = items * s.units;
+    }
+    const unsigned cum_units = scan32(units, lane), n = by_item ? items : units, cum = by_item ? scan32(items, lane) : cum_units;
+    const unsigned over = __ballot_sync(0xffffffffu, base + cum > u);
+    if (over) {
+      const int at = __ffs(over) - 1;
+      const unsigned rest = u - base - __shfl_sync(0xffffffffu, cum - n, at);
+      w.b = b0 + at;
+      w.s.q0 = __shfl_sync(0xffffffffu, s.q0, at);
+      w.s.nq = __shfl_sync(0xffffffffu, s.nq, at);
+      w.s.len = __shfl_sync(0xffffffffu, s.len, at);
+      w.s.first = __shfl_sync(0xffffffffu, s.first, at);
+      w.s.tiles = __shfl_sync(0xffffffffu, s.tiles, at);
+      w.s.units = __shfl_sync(0xffffffffu, s.units, at);
+      const unsigned item = by_item ? rest : rest / (unsigned)w.s.units;
+      w.unit = by_item ? 0 : (int)(rest - item * w.s.units);
+      w.tile = (int)(item / (unsigned)a.kv_heads);
+      w.head = (int)(item - (unsigned)w.tile * a.kv_heads);
+      before = base_units + __shfl_sync(0xffffffffu, cum_units - units, at) + item * w.s.units;
+      return true;
+    }
+    base += __shfl_sync(0xffffffffu, cum, 31);
+    base_units += __shfl_sync(0xffffffffu, cum_units, 31);
+  }
+  return false;
+}
+
+}  // namespace kv4
+
+int kv4_prompt_launch(const kv4::AttnArgs& a, int dim, int dtype, cudaStream_t stream);
+
+}  // namespace xqt_b200

@@ -1,0 +1,503 @@
+// Attention of many queries (prompts, chunks of prompts) over the paged 4-bit cache (layout: kv4_cache.cu; the mathematics and the rules
+// for what a query sees: kv4_attention.cu), on the tensor cores.
+//
+// A CTA takes TILES row tiles of 128 (row = query * heads of the key head + head) of one sequence and key head through the keys they see, BN at
+// a time.  Codes come in by bulk copies; four warps turn them into fp16 keys and values in shared memory (128-byte swizzle), once for all rows;
+// one thread issues S = Q K^T and O += P V (tcgen05, sums in tensor memory); four warps per row tile, a thread per row, do the softmax: P goes
+// back to tensor memory over the scores that it came from.  While one tile's scores are in the softmax the tensor core works for the other.
+//
+//   warp 0       table look-ups and bulk copies (two chunks of codes ahead)
+//   warp 1       tcgen05.mma
+//   warp 2       allocates tensor memory
+//   warps 4-7    codes -> fp16
+//   warps 8-15   softmax, rescaling of O, result
+//
+// Scales.  fp16 has the mantissa that keeps the result as exact as the inputs (bf16 operands lose 8 times more), but not the range, so all
+// three operands go in with a power of two: a query row with its own (largest element in [1, 2)), the keys of a chunk with one
+// for the chunk (largest in [2^13, 2^14)), values with one that only grows along the sequence (O is rescaled then).  The powers come back
+// in the fp32 factor of the scores and at the end.  P is formed against a running maximum that moves only when a row exceeds
+// it by 2^8, so O is rescaled rarely; P <= 2^8 fits fp16.
+//
+// A vector that is not finite counts as NaN: its key becomes NaN, its value 0, so the rows that see it are NaN and the others never
+// meet it.  Keys that are not there (no page, past the end) become 0 and are masked.
+//
+// The order of a word's codes: pairs (0,4) (1,5) (2,6) (3,7) come out of one AND each, so channels stand in shared memory as 0 4 1 5 2 6 3 7 in
+// every group of eight; queries are stored in the same order, and the result is put back when it is written.
+//
+// Bound by the tensor core and by ex2 (16 a clock and SM), which take the same time for 128 channels.
+#include "kv4_attention.cuh"
+
+namespace xqt_b200 {
+
+namespace {
+
+using namespace kv4;
+
+template <int D_, int TILES_, int BN_>
+struct PromptShape {
+  static constexpr int D = D_, TILES = TILES_, BN = BN_;
+  static constexpr int ROWS = 128 * TILES, UNIT = 1 << 20, CT = BN, OPENING = 1;
+  static constexpr bool PROMPT = true;
+  static constexpr int THREADS = 256 + 128 * TILES;
+  static constexpr int BLOCKS = D / 64;                        // 128-byte wide column blocks of an operand
+  static constexpr int Q_BYTES = ROWS * D * 2, KV_BYTES = BN * D * 2;
+  static constexpr int CODE_BYTES = BN * D / 2, PARAM_BYTES = BN * 4, RAW_BYTES = 2 * (CODE_BYTES + PARAM_BYTES);
+  static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + 2 * KV_BYTES, OFF_RAW = OFF_V + 2 * KV_BYTES, OFF_MISC = OFF_RAW + 2 * RAW_BYTES;
+  static constexpr int SMEM = OFF_MISC + 512;
+  static constexpr uint32_t O_COL = 256, P_COL = BN / 2;       // tensor memory: scores of tile i at i * BN, P over their upper half, O at 256
+  static_assert(TILES * BN <= 256 && TILES * D <= 256 && SMEM <= 227 * 1024, "tensor and shared memory");
+};
+
+// barriers, in 8-byte words behind the tiles
+enum : int { kRawFull = 0, kRawEmpty = 2, kKReady = 4, kVReady = 6, kKEmpty = 8, kVEmpty = 10, kSFull = 12, kPReady = 14, kODone = 16, kQReady = 18, kBarriers = 19 };
+
+__device__ __forceinline__ void wait_ld_dep32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                 "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]),
+                 "+r"(r[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+               "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+// Shared-memory operand whose long side is the contiguous one (values as the second operand of P V), 128-byte swizzle: 64 channels of eight
+// keys are 1024 bytes, the next eight keys follow, the next 64 channels are `block_bytes` away.
+__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t saddr, uint32_t block_bytes) {
+  return (uint64_t)((saddr & 0x3FFFF) >> 4) | (uint64_t)(block_bytes >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+__device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ __half2 bits_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }     // -126 <= e <= 127
+// e with |v| < 2^e, in [-100, 127]
+__device__ __forceinline__ int above(float v) { return min(max((int)(__float_as_uint(v) >> 23) - 126, -100), 127); }
+
+// eight codes -> c * s + m in fp16, rounded once (the codes themselves are exact: 1024 + c and 64 + c less that)
+__device__ __forceinline__ uint4 eight(uint32_t x, __half2 s, __half2 m) {
+  const __half2 k1024 = bits_half2(0x64006400u), k64 = bits_half2(0x54005400u);
+  const uint32_t y = x >> 8;
+  uint4 r;
+  r.x = half2_bits(__hfma2(__hsub2(bits_half2((x & 0x000f000fu) | 0x64006400u), k1024), s, m));
+  r.y = half2_bits(__hfma2(__hsub2(bits_half2((x & 0x00f000f0u) | 0x54005400u), k64), s, m));
+  r.z = half2_bits(__hfma2(__hsub2(bits_half2((y & 0x000f000fu) | 0x64006400u), k1024), s, m));
+  r.w = half2_bits(__hfma2(__hsub2(bits_half2((y & 0x00f000f0u) | 0x54005400u), k64), s, m));
+  return r;
+}
+
+template <typename T, typename SH>
+__global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnArgs a) {
+  constexpr int D = SH::D, TILES = SH::TILES, BN = SH::BN, BLOCKS = SH::BLOCKS;
+  const float kLowest = -CUDART_INF_F;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint8_t* const misc = smem + SH::OFF_MISC;
+  const uint32_t bar0 = smem_addr(misc);
+  auto bar = [&](int slot) { return bar0 + 8u * (uint32_t)slot; };
+  volatile uint32_t* const s_mask = reinterpret_cast<volatile uint32_t*>(misc + 160);       // [8] which 16-key groups of a chunk are there
+  volatile float* const s_key = reinterpret_cast<volatile float*>(misc + 192);               // [8] what a chunk's keys were divided by
+  volatile float* const s_value = reinterpret_cast<volatile float*>(misc + 224);             // [8] what O has to be multiplied by before it
+  volatile float* const s_last = reinterpret_cast<volatile float*>(misc + 256);              // what the values were divided by in the end
+  volatile uint32_t* const s_abort = reinterpret_cast<volatile uint32_t*>(misc + 260);
+  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(misc + 264);
+
+  grid_launch_dependents();
+  grid_dependency_wait();
+  Sequence mine = {};
+  (void)deal<SH>(a, lane, 1, mine);
+  Walk w;
+  unsigned unused;
+  if (!place<SH>(a, lane, mine, blockIdx.x, true, w, unused)) return;
+  w.tile = w.s.tiles - 1 - w.tile;                                   // the longest ones of a sequence first
+  const int row0 = w.tile * SH::ROWS, rows = w.s.nq * a.each;
+  const int pos0 = w.s.len - w.s.nq;                                 // the position of the sequence's first query
+  const int j0 = row0 / a.each, j1 = min(w.s.nq - 1, (row0 + SH::ROWS - 1) / a.each);
+  const int end = pos0 + j1 + 1;                                     // keys that some row sees: [begin, end)
+  const int begin = a.window ? (int)max((long long)pos0 + j0 - a.window + 1, 0LL) / BN * BN : 0;
+  const int chunks = end > begin ? (end - begin + BN - 1) / BN : 0;
+
+  if (tid == 0) {
+    *s_abort = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(kRawFull + i), 1);
+      mbar_init(bar(kRawEmpty + i), 4);
+      mbar_init(bar(kKReady + i), 4);
+      mbar_init(bar(kVReady + i), 4);
+      mbar_init(bar(kKEmpty + i), 1);
+      mbar_init(bar(kVEmpty + i), 1);
+      mbar_init(bar(kSFull + i), 1);
+      mbar_init(bar(kPReady + i), 4);
+      mbar_init(bar(kODone + i), 1);
+    }
+    mbar_init(bar(kQReady), 4 * TILES);
+    fence_barrier_init();
+  }
+  if (warp == 2) {
+    tmem_alloc(smem_addr(s_tmem), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  // every wait is bounded: when one runs out nothing waits any more, and the host is told
+  auto guarded = [&](uint32_t b, uint32_t parity) {
+    if (*s_abort == 0u && !mbar_wait(b, parity)) {
+      *s_abort = 1u;
+      if (a.status) *a.status = 1u;
+    }
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ codes and parameters into the raw ring
+    const int psz = min(a.page_size, BN), pieces = BN / psz, groups = psz / 16;
+    const int piece = lane >> 2, kind = lane & 3;                    // kind: key codes, value codes, key parameters, value parameters
+    const int row_bytes = kind < 2 ? D / 2 : 4;
+    const uint8_t* const source = (kind < 2 ? a.codes : a.params) + ((long long)(kind & 1) * a.kv_heads + w.head) * a.page_size * row_bytes;
+    const long long page_bytes = 2LL * a.kv_heads * a.page_size * row_bytes;
+    const uint32_t target = smem_addr(smem + SH::OFF_RAW) +
+                            (kind == 0 ? 0 : kind == 1 ? SH::CODE_BYTES : kind == 2 ? 2 * SH::CODE_BYTES : 2 * SH::CODE_BYTES + SH::PARAM_BYTES) + piece * psz * row_bytes;
+    const int* const table = a.table + w.b * a.table_stride;
+    auto look_up = [&](int i) {
+      const int at = begin + i * BN + piece * psz;
+      return i < chunks && piece < pieces && at < w.s.len ? table[at >> a.page_shift] : -1;
+    };
+    int page = look_up(0);
+    for (int i = 0; i < chunks; ++i) {
+      const int stage = i & 1, following = look_up(i + 1);
+      const bool valid = (unsigned)page < (unsigned)a.pages;
+      const unsigned votes = __ballot_sync(0xffffffffu, valid);
+      unsigned mask = 0;
+#pragma unroll
+      for (int p = 0; p < BN / 16; ++p) mask |= (votes >> (4 * (p / groups)) & 1u) << p;
+      guarded(bar(kRawEmpty + stage), (i >> 1 & 1) ^ 1);
+      if (lane == 0) {
+        s_mask[i & 7] = mask;
+        mbar_expect_tx(bar(kRawFull + stage), (uint32_t)(__popc(mask) * 16 * 2 * (D / 2 + 4)));
+      }
+      __syncwarp();
+      const int at = begin + i * BN + piece * psz;
+      if (valid && *s_abort == 0u)
+        bulk_g2s(target + stage * SH::RAW_BYTES, source + page * page_bytes + (long long)(at & (a.page_size - 1)) * row_bytes, (uint32_t)(psz * row_bytes), bar(kRawFull + stage));
+      page = following;
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ the tensor core
+    if (elect_one() && chunks > 0) {
+      constexpr uint32_t kScores = umma_idesc(kAccF32, kFmtF16, kFmtF16, 128, BN);
+      constexpr uint32_t kOut = umma_idesc(kAccF32, kFmtF16, kFmtF16, 128, D) | 1u << 16;      // second operand: long side contiguous
+      const uint32_t base = smem_addr(smem);
+      auto scores = [&](int i, int tile) {
+#pragma unroll
+        for (int kb = 0; kb < BLOCKS; ++kb) {
+          const uint64_t ad = umma_desc_sw128(base + (tile * BLOCKS + kb) * (128 * 128)), bd = umma_desc_sw128(base + SH::OFF_K + (i & 1) * SH::KV_BYTES + kb * (BN * 128));
+#pragma unroll
+          for (int s = 0; s < 4; ++s) umma_ss(tmem + tile * BN, ad + 2 * s, bd + 2 * s, kScores, kb || s ? 1u : 0u);
+        }
+        umma_commit(bar(kSFull + tile));
+      };
+      auto values = [&](int i, int tile) {
+#pragma unroll
+        for (int s = 0; s < BN / 16; ++s)
+          umma_ts_f16(tmem + SH::O_COL + tile * D, tmem + tile * BN + SH::P_COL + 8 * s,
+                      umma_desc_mn_sw128(base + SH::OFF_V + (i & 1) * SH::KV_BYTES + s * 2048, BN * 128), kOut, i || s ? 1u : 0u);
+      };
+      guarded(bar(kQReady), 0);
+      for (int i = 0; i <= chunks; ++i) {
+        if (i < chunks) guarded(bar(kKReady + (i & 1)), i >> 1 & 1);
+        if (i > 0) guarded(bar(kVReady + (i - 1 & 1)), i - 1 >> 1 & 1);
+#pragma unroll
+        for (int tile = 0; tile < TILES; ++tile) {
+          if (i > 0) {
+            guarded(bar(kPReady + tile), (i - 1) & 1);
+            tc_fence_after();
+            values(i - 1, tile);
+            if (i == chunks) umma_commit(bar(kODone + tile));
+            else if (tile == TILES - 1) umma_commit(bar(kVEmpty + (i - 1 & 1)));
+          }
+          if (i < chunks) {
+            tc_fence_after();
+            scores(i, tile);                        // in order behind the product that read P from the same columns
+            if (tile == TILES - 1) umma_commit(bar(kKEmpty + (i & 1)));
+          }
+        }
+      }
+    }
+  } else if (warp >= 4 && warp < 8) {
+    // ------------------------------------------------------------ codes -> fp16
+    constexpr int CHUNKS16 = D / 32, PER = CHUNKS16 * BN / 128;      // 16-byte pieces of a key's codes, and how many of them a thread does
+    const int t4 = tid - 128, row = t4 % BN, part = t4 / BN;
+    const int turn = D == 64 ? row >> 2 : D == 128 ? row >> 1 : row; // which piece first: spreads the rows over the banks
+    int grown = -100;                                                // values so far are below 2^grown
+    for (int i = 0; i < chunks; ++i) {
+      const int stage = i & 1;
+      const uint8_t* const raw = smem + SH::OFF_RAW + stage * SH::RAW_BYTES;
+      guarded(bar(kRawFull + stage), i >> 1 & 1);
+      const uint32_t* const kp = reinterpret_cast<const uint32_t*>(raw + 2 * SH::CODE_BYTES);
+      const uint32_t* const vp = kp + BN;
+      const uint32_t mask = s_mask[i & 7];
+      const int t0 = begin + i * BN;
+      // the chunk's largest key and value element; what is not there or not finite does not count
+      float top_k = 0.0f, top_v = 0.0f;
+#pragma unroll
+      for (int r = lane; r < BN; r += 32) {
+        if ((mask >> (r >> 4) & 1u) && t0 + r < w.s.len) {
+          const float2 k = pair_of<T>(kp[r]), v = pair_of<T>(vp[r]);
+          const float tk = fmaxf(fabsf(k.y), fabsf(fmaf(15.0f, k.x, k.y))), tv = fmaxf(fabsf(v.y), fabsf(fmaf(15.0f, v.x, v.y)));
+          if (tk <= 3.402823466e38f) top_k = fmaxf(top_k, tk);
+          if (tv <= 3.402823466e38f) top_v = fmaxf(top_v, tv);
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        top_k = fmaxf(top_k, __shfl_xor_sync(0xffffffffu, top_k, o));
+        top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, o));
+      }
+      const int ek = above(top_k), ev = max(grown, above(top_v));
+      if (t4 == 0) {
+        s_key[i & 7] = pow2(max(ek - 14, -126));
+        s_value[i & 7] = pow2(max(grown - ev, -126));
+        *s_last = pow2(max(ev - 14, -126));
+      }
+      grown = ev;
+      const bool there = (mask >> (row >> 4) & 1u) && t0 + row < w.s.len;
+      const float2 k = pair_of<T>(kp[row]), v = pair_of<T>(vp[row]);
+      const bool v_good = fabsf(v.x) <= 3.402823466e38f && fabsf(v.y) <= 3.402823466e38f;
+      const bool k_good = fabsf(k.x) <= 3.402823466e38f && fabsf(k.y) <= 3.402823466e38f && v_good;
+      const float fk = pow2(14 - ek), fv = pow2(14 - ev);
+      const float nan = __int_as_float(0x7fffffff);
+      const __half2 ks = __float2half2_rn(!there ? 0.0f : k_good ? k.x * fk : nan), km = __float2half2_rn(!there ? 0.0f : k_good ? k.y * fk : nan);
+      const __half2 vs = __float2half2_rn(there && v_good ? v.x * fv : 0.0f), vm = __float2half2_rn(there && v_good ? v.y * fv : 0.0f);
+      auto convert = [&](const uint8_t* codes, uint8_t* dst, __half2 s, __half2 m) {
+#pragma unroll
+        for (int n = 0; n < PER; ++n) {
+          const int piece = (turn + n + part * PER) % CHUNKS16;
+          const uint4 x = *reinterpret_cast<const uint4*>(codes + row * (D / 2) + piece * 16);
+          uint8_t* const to = dst + (piece >> 1) * (BN * 128) + row * 128;
+          const int first = (piece & 1) * 4, swizzle = row & 7;
+          *reinterpret_cast<uint4*>(to + (((first + 0) ^ swizzle) << 4)) = eight(x.x, s, m);
+          *reinterpret_cast<uint4*>(to + (((first + 1) ^ swizzle) << 4)) = eight(x.y, s, m);
+          *reinterpret_cast<uint4*>(to + (((first + 2) ^ swizzle) << 4)) = eight(x.z, s, m);
+          *reinterpret_cast<uint4*>(to + (((first + 3) ^ swizzle) << 4)) = eight(x.w, s, m);
+        }
+      };
+      guarded(bar(kKEmpty + stage), (i >> 1 & 1) ^ 1);
+      convert(raw, smem + SH::OFF_K + stage * SH::KV_BYTES, ks, km);
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kKReady + stage));
+      guarded(bar(kVEmpty + stage), (i >> 1 & 1) ^ 1);
+      convert(raw + SH::CODE_BYTES, smem + SH::OFF_V + stage * SH::KV_BYTES, vs, vm);
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(bar(kVReady + stage));
+        mbar_arrive(bar(kRawEmpty + stage));
+      }
+    }
+  } else if (warp >= 8) {
+    // ------------------------------------------------------------ softmax: a thread per row
+    const int tile = (warp - 8) >> 2, quarter = warp & 3, line = quarter * 32 + lane;
+    const int row = row0 + tile * 128 + line;
+    const bool real = row < rows;
+    const int j = real ? row / a.each : 0, head = w.head * a.each + (real ? row - j * a.each : 0);
+    float factor;
+    {
+      const T* const src = reinterpret_cast<const T*>(a.q) + (long long)(w.s.q0 + j) * a.q_token + (long long)head * a.q_head;
+      float top = 0.0f;
+#pragma unroll 4
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 x = real ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0, 0, 0, 0);
+        const T* e = reinterpret_cast<const T*>(&x);
+#pragma unroll
+        for (int n = 0; n < 8; ++n) top = fmaxf(top, fabsf(to_float<T>(e[n])));
+      }
+      const int e = top > 0.0f && top <= 3.402823466e38f ? min(max(above(top) - 1, -100), 100) : 0;
+      const float down = a.scale == 0.0f ? 0.0f : copysignf(pow2(-e), a.scale);
+      factor = pow2(e) * (a.scale == 0.0f ? 1.0f : fabsf(a.scale));
+      uint8_t* const dst = smem + tile * (BLOCKS * 128 * 128) + line * 128;
+#pragma unroll 4
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 x = real ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0, 0, 0, 0);
+        const T* v = reinterpret_cast<const T*>(&x);
+        uint4 y;
+        y.x = half2_bits(__floats2half2_rn(to_float<T>(v[0]) * down, to_float<T>(v[4]) * down));
+        y.y = half2_bits(__floats2half2_rn(to_float<T>(v[1]) * down, to_float<T>(v[5]) * down));
+        y.z = half2_bits(__floats2half2_rn(to_float<T>(v[2]) * down, to_float<T>(v[6]) * down));
+        y.w = half2_bits(__floats2half2_rn(to_float<T>(v[3]) * down, to_float<T>(v[7]) * down));
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * (128 * 128) + (((c & 7) ^ (line & 7)) << 4)) = y;
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kQReady));
+    }
+    const int hi = real ? pos0 + j : -1, lo = a.window ? (int)max((long long)pos0 + j - a.window + 1, 0LL) : 0;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_at = tmem + lanes + tile * BN, p_at = s_at + SH::P_COL, o_at = tmem + lanes + SH::O_COL + tile * D;
+    float m = kLowest;
+    Two l(0.0f);
+    for (int i = 0; i < chunks; ++i) {
+      guarded(bar(kSFull + tile), i & 1);
+      tc_fence_after();
+      const int t0 = begin + i * BN;
+      const float f = fminf(fmaxf(factor * s_key[i & 7], 7.5e-37f), 1.3e30f), ratio = s_value[i & 7];
+      const uint32_t there = s_mask[i & 7];
+      const bool all = there == (BN == 128 ? 0xffu : 0xfu) && t0 + BN - 1 <= hi && t0 >= lo;
+      const bool masked = __any_sync(0xffffffffu, !all);
+      // which of the 32 keys from t on this row sees
+      auto visible = [&](int n) {
+        const int t = t0 + 32 * n;
+        uint32_t bits = 0xffffffffu;
+        if (hi < t + 31) bits = hi < t ? 0u : 0xffffffffu >> (t + 31 - hi);
+        if (lo > t) bits = lo > t + 31 ? 0u : bits & 0xffffffffu << (lo - t);
+        const uint32_t two = there >> (2 * n);
+        return bits & ((two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u));
+      };
+      auto hide = [&](uint32_t (&r)[32], int n) {
+        const uint32_t bits = visible(n);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) r[e] = bits >> e & 1u ? r[e] : 0xff800000u;
+      };
+      auto largest = [](const uint32_t (&r)[32]) {
+        float x = __uint_as_float(r[0]), y = __uint_as_float(r[1]);
+#pragma unroll
+        for (int e = 2; e < 32; e += 2) {
+          x = fmaxf(x, __uint_as_float(r[e]));
+          y = fmaxf(y, __uint_as_float(r[e + 1]));
+        }
+        return fmaxf(x, y);
+      };
+      uint32_t ra[32], rb[32];
+      float top = kLowest;
+#pragma unroll
+      for (int n = 0; n < BN / 64; ++n) {            // the last pair stays in registers
+        tmem_ld_32x32(s_at + 64 * n, ra);
+        tmem_ld_32x32(s_at + 64 * n + 32, rb);
+        wait_ld_dep32(ra);
+        wait_ld_dep32(rb);
+        if (masked) {
+          hide(ra, 2 * n);
+          hide(rb, 2 * n + 1);
+        }
+        top = fmaxf(top, fmaxf(largest(ra), largest(rb)));
+      }
+      top *= f;
+      const bool moves = top > m + 8.0f || (m == kLowest && top > kLowest);
+      if (__any_sync(0xffffffffu, moves) || ratio != 1.0f) {
+        const float next = fmaxf(m, top);
+        const float alpha = m == next ? 1.0f : exp2_fast(m - next);
+        m = next;
+        l = l * Two(alpha);
+        if (i > 0) {                                 // O is complete: the scores were issued behind the product before
+          const Two by(alpha * ratio);
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t r[32];
+            tmem_ld_32x32(o_at + 32 * c, r);
+            wait_ld_dep32(r);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 v = (Two(__uint_as_float(r[e]), __uint_as_float(r[e + 1])) * by).both();
+              r[e] = __float_as_uint(v.x);
+              r[e + 1] = __float_as_uint(v.y);
+            }
+            tmem_st_32x32(o_at + 32 * c, r);
+          }
+        }
+      }
+      const Two f2(f), minus(m == kLowest ? 0.0f : -m);
+      auto weigh = [&](const uint32_t (&r)[32], int n) {
+        uint32_t h[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float2 x = fma2(Two(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), f2, minus).both();
+          const float2 p = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+          l = l + Two(p.x, p.y);
+          h[e] = half2_bits(__floats2half2_rn(p.x, p.y));
+        }
+        tmem_st_32x16(p_at + 16 * n, h);
+      };
+      weigh(ra, BN / 32 - 2);
+      weigh(rb, BN / 32 - 1);
+      if constexpr (BN == 128) {                     // the upper half of the scores has been read: P takes its place
+        tmem_ld_32x32(s_at, ra);
+        tmem_ld_32x32(s_at + 32, rb);
+        wait_ld_dep32(ra);
+        wait_ld_dep32(rb);
+        if (masked) {
+          hide(ra, 0);
+          hide(rb, 1);
+        }
+        weigh(ra, 0);
+        weigh(rb, 1);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kPReady + tile));
+    }
+    if (chunks > 0) {
+      guarded(bar(kODone + tile), 0);
+      tc_fence_after();
+    }
+    const float2 sums = l.both();
+    const float weight = sums.x + sums.y;
+    const float inv = weight == 0.0f || chunks == 0 ? 0.0f : *s_last / weight;
+    T* const out = reinterpret_cast<T*>(a.out) + ((long long)(w.s.q0 + j) * a.q_heads + head) * D;
+#pragma unroll 1
+    for (int c = 0; c < D / 32; ++c) {
+      uint32_t r[32];
+      if (chunks > 0) {
+        tmem_ld_32x32(o_at + 32 * c, r);
+        wait_ld_dep32(r);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) r[e] = 0u;
+      }
+      if (real) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          uint4 y;
+          T* const v = reinterpret_cast<T*>(&y);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = from_float<T>(__uint_as_float(r[8 * b + (e < 4 ? 2 * e : 2 * e - 7)]) * inv);
+          *reinterpret_cast<uint4*>(out + 32 * c + 8 * b) = y;
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename T, int D, int TILES, int BN>
+int run(const AttnArgs& a, cudaStream_t stream) {
+  using SH = PromptShape<D, TILES, BN>;
+  const long long items = ((long long)a.tokens * a.each / SH::ROWS + a.batch) * a.kv_heads;
+  XQT_REQUIRE(items < (1LL << 31) - 1);
+  XQT_SMEM_OPT_IN((kv4_prompt_kernel<T, SH>), SH::SMEM);
+  return launch_pdl(kv4_prompt_kernel<T, SH>, dim3((unsigned)items), dim3(SH::THREADS), SH::SMEM, stream, a);
+}
+
+template <typename T>
+int run_dim(const AttnArgs& a, int dim, cudaStream_t stream) {
+  if (dim == 64) return run<T, 64, 2, 128>(a, stream);
+  if (dim == 128) return run<T, 128, 2, 128>(a, stream);
+  return run<T, 256, 1, 64>(a, stream);
+}
+
+}  // namespace
+
+int kv4_prompt_launch(const kv4::AttnArgs& a, int dim, int dtype, cudaStream_t stream) {
+  return dtype == XQT_B200_BF16 ? run_dim<__nv_bfloat16>(a, dim, stream) : run_dim<__half>(a, dim, stream);
+}
+
+}  // namespace xqt_b200

@@ -631,7 +631,8 @@ int run(AttnArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream
   using SH = Few<D, NT>;
   static_assert((SH::SMEM + 1024) * SH::PER_SM <= 228 * 1024 && SH::PER_SM <= kMostPerSm, "resident together");
   // as many items as there can be: full tiles, and one that is not full per sequence
-  const long long tiles = a.query_starts ? (long long)a.tokens * a.each / SH::ROWS + a.batch : (long long)a.batch * ceil_div(a.each, SH::ROWS);
+  const long long most_rows = a.query_starts ? a.few_rows : a.each;
+  const long long tiles = min((long long)a.tokens * a.each / SH::ROWS + a.batch, a.batch * ((most_rows + SH::ROWS - 1) / SH::ROWS));
   const long long items = tiles * a.kv_heads, units = items * (((long long)a.table_width << a.page_shift) / SH::UNIT + 1 + SH::OPENING);
   XQT_REQUIRE(items < (1LL << 31) - 1 && units < (1LL << 31));
   const int ctas = (int)min((long long)SH::PER_SM * sm_count(), units);

@@ -4,9 +4,10 @@
 // A CTA takes TILES row tiles of 128 (row = query * heads of the key head + head) of one sequence and key head through the keys they see, BN at
 // a time.  Codes come in by bulk copies; four warps turn them into fp16 keys and values in shared memory (128-byte swizzle), once for all rows;
 // one thread issues S = Q K^T and O += P V (tcgen05, sums in tensor memory); four warps per row tile, a thread per row, do the softmax: P goes
-// back to tensor memory over the scores that it came from.  While one tile's scores are in the softmax the tensor core works for the other.
+// back to tensor memory over the scores that it came from.  Scores are double-buffered: those of the next chunk are made while the softmax
+// works on this one's.
 //
-//   warp 0       table look-ups and bulk copies (two chunks of codes ahead)
+//   warp 0       table look-ups and bulk copies
 //   warp 1       tcgen05.mma
 //   warp 2       allocates tensor memory
 //   warps 4-7    codes -> fp16
@@ -33,23 +34,37 @@ namespace {
 
 using namespace kv4;
 
-template <int D_, int TILES_, int BN_>
+template <int D_, int TILES_, int STAGES_, int RAW_>
 struct PromptShape {
-  static constexpr int D = D_, TILES = TILES_, BN = BN_;
+  static constexpr int D = D_, TILES = TILES_, STAGES = STAGES_, RAW = RAW_, BN = 64;
   static constexpr int ROWS = 128 * TILES, UNIT = 1 << 20, CT = BN, OPENING = 1;
   static constexpr bool PROMPT = true;
   static constexpr int THREADS = 256 + 128 * TILES;
   static constexpr int BLOCKS = D / 64;                        // 128-byte wide column blocks of an operand
   static constexpr int Q_BYTES = ROWS * D * 2, KV_BYTES = BN * D * 2;
   static constexpr int CODE_BYTES = BN * D / 2, PARAM_BYTES = BN * 4, RAW_BYTES = 2 * (CODE_BYTES + PARAM_BYTES);
-  static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + 2 * KV_BYTES, OFF_RAW = OFF_V + 2 * KV_BYTES, OFF_MISC = OFF_RAW + 2 * RAW_BYTES;
+  static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + STAGES * KV_BYTES, OFF_RAW = OFF_V + STAGES * KV_BYTES, OFF_MISC = OFF_RAW + RAW * RAW_BYTES;
   static constexpr int SMEM = OFF_MISC + 512;
-  static constexpr uint32_t O_COL = 256, P_COL = BN / 2;       // tensor memory: scores of tile i at i * BN, P over their upper half, O at 256
-  static_assert(TILES * BN <= 256 && TILES * D <= 256 && SMEM <= 227 * 1024, "tensor and shared memory");
+  // tensor memory: two buffers of scores per tile from column 0, P over the first half of its scores; O from 256
+  static constexpr uint32_t O_COL = 256;
+  static_assert(2 * TILES * BN <= 256 && TILES * D <= 256 && SMEM <= 227 * 1024 && STAGES <= 4 && RAW <= 4, "tensor and shared memory");
 };
 
-// barriers, in 8-byte words behind the tiles
-enum : int { kRawFull = 0, kRawEmpty = 2, kKReady = 4, kVReady = 6, kKEmpty = 8, kVEmpty = 10, kSFull = 12, kPReady = 14, kODone = 16, kQReady = 18, kBarriers = 19 };
+// Barriers, in 8-byte words behind the tiles.  The last four kinds are per tile and chunk parity: a softmax warp may be a chunk ahead of its
+// neighbours, and a wait may come two products late.
+enum : int { kRawFull = 0, kRawEmpty = 4, kKReady = 8, kVReady = 12, kKEmpty = 16, kVEmpty = 20, kSFull = 24, kPReady = 28, kODone = 32, kQReady = 36, kBarriers = 37 };
+constexpr int kRing = 16;          // chunks that loader, conversion and softmax may lie apart: more than 2 + STAGES + RAW
+
+template <int N>
+struct Ring {
+  int slot = 0, phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == N) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+};
 
 __device__ __forceinline__ void wait_ld_dep32(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;\n"
@@ -98,12 +113,12 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
   uint8_t* const misc = smem + SH::OFF_MISC;
   const uint32_t bar0 = smem_addr(misc);
   auto bar = [&](int slot) { return bar0 + 8u * (uint32_t)slot; };
-  volatile uint32_t* const s_mask = reinterpret_cast<volatile uint32_t*>(misc + 160);       // [8] which 16-key groups of a chunk are there
-  volatile float* const s_key = reinterpret_cast<volatile float*>(misc + 192);               // [8] what a chunk's keys were divided by
-  volatile float* const s_value = reinterpret_cast<volatile float*>(misc + 224);             // [8] what O has to be multiplied by before it
-  volatile float* const s_last = reinterpret_cast<volatile float*>(misc + 256);              // what the values were divided by in the end
-  volatile uint32_t* const s_abort = reinterpret_cast<volatile uint32_t*>(misc + 260);
-  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(misc + 264);
+  volatile uint32_t* const s_mask = reinterpret_cast<volatile uint32_t*>(misc + 296);       // [kRing] which 16-key groups of a chunk are there
+  volatile float* const s_key = reinterpret_cast<volatile float*>(misc + 360);               // [kRing] what a chunk's keys were divided by
+  volatile float* const s_value = reinterpret_cast<volatile float*>(misc + 424);             // [kRing] what O has to be multiplied by before it
+  volatile float* const s_last = reinterpret_cast<volatile float*>(misc + 488);              // what the values were divided by in the end
+  volatile uint32_t* const s_abort = reinterpret_cast<volatile uint32_t*>(misc + 492);
+  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(misc + 496);
 
   grid_launch_dependents();
   grid_dependency_wait();
@@ -122,7 +137,7 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
 
   if (tid == 0) {
     *s_abort = 0;
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(bar(kRawFull + i), 1);
       mbar_init(bar(kRawEmpty + i), 4);
       mbar_init(bar(kKReady + i), 4);
@@ -152,6 +167,14 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
     }
   };
 
+  // the same by polling, where the wake-up of a suspended thread would set the pace
+  auto polled = [&](uint32_t b, uint32_t parity) {
+    if (*s_abort == 0u && !mbar_spin(b, parity)) {
+      *s_abort = 1u;
+      if (a.status) *a.status = 1u;
+    }
+  };
+
   if (warp == 0) {
     // ------------------------------------------------------------ codes and parameters into the raw ring
     const int psz = min(a.page_size, BN), pieces = BN / psz, groups = psz / 16;
@@ -167,16 +190,17 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
       return i < chunks && piece < pieces && at < w.s.len ? table[at >> a.page_shift] : -1;
     };
     int page = look_up(0);
-    for (int i = 0; i < chunks; ++i) {
-      const int stage = i & 1, following = look_up(i + 1);
+    Ring<SH::RAW> ring;
+    for (int i = 0; i < chunks; ++i, ring.next()) {
+      const int stage = ring.slot, following = look_up(i + 1);
       const bool valid = (unsigned)page < (unsigned)a.pages;
       const unsigned votes = __ballot_sync(0xffffffffu, valid);
       unsigned mask = 0;
 #pragma unroll
       for (int p = 0; p < BN / 16; ++p) mask |= (votes >> (4 * (p / groups)) & 1u) << p;
-      guarded(bar(kRawEmpty + stage), (i >> 1 & 1) ^ 1);
+      guarded(bar(kRawEmpty + stage), ring.phase ^ 1);
       if (lane == 0) {
-        s_mask[i & 7] = mask;
+        s_mask[i % kRing] = mask;
         mbar_expect_tx(bar(kRawFull + stage), (uint32_t)(__popc(mask) * 16 * 2 * (D / 2 + 4)));
       }
       __syncwarp();
@@ -191,39 +215,45 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
       constexpr uint32_t kScores = umma_idesc(kAccF32, kFmtF16, kFmtF16, 128, BN);
       constexpr uint32_t kOut = umma_idesc(kAccF32, kFmtF16, kFmtF16, 128, D) | 1u << 16;      // second operand: long side contiguous
       const uint32_t base = smem_addr(smem);
-      auto scores = [&](int i, int tile) {
+      auto scores = [&](int i, int stage, int tile) {
+        const int at = 2 * tile + (i & 1);
 #pragma unroll
         for (int kb = 0; kb < BLOCKS; ++kb) {
-          const uint64_t ad = umma_desc_sw128(base + (tile * BLOCKS + kb) * (128 * 128)), bd = umma_desc_sw128(base + SH::OFF_K + (i & 1) * SH::KV_BYTES + kb * (BN * 128));
+          const uint64_t ad = umma_desc_sw128(base + (tile * BLOCKS + kb) * (128 * 128)), bd = umma_desc_sw128(base + SH::OFF_K + stage * SH::KV_BYTES + kb * (BN * 128));
 #pragma unroll
-          for (int s = 0; s < 4; ++s) umma_ss(tmem + tile * BN, ad + 2 * s, bd + 2 * s, kScores, kb || s ? 1u : 0u);
+          for (int s = 0; s < 4; ++s) umma_ss(tmem + at * BN, ad + 2 * s, bd + 2 * s, kScores, kb || s ? 1u : 0u);
         }
-        umma_commit(bar(kSFull + tile));
+        umma_commit(bar(kSFull + at));
       };
-      auto values = [&](int i, int tile) {
+      auto values = [&](int i, int stage, int tile) {
 #pragma unroll
         for (int s = 0; s < BN / 16; ++s)
-          umma_ts_f16(tmem + SH::O_COL + tile * D, tmem + tile * BN + SH::P_COL + 8 * s,
-                      umma_desc_mn_sw128(base + SH::OFF_V + (i & 1) * SH::KV_BYTES + s * 2048, BN * 128), kOut, i || s ? 1u : 0u);
+          umma_ts_f16(tmem + SH::O_COL + tile * D, tmem + (2 * tile + (i & 1)) * BN + 8 * s,
+                      umma_desc_mn_sw128(base + SH::OFF_V + stage * SH::KV_BYTES + s * 2048, BN * 128), kOut, i || s ? 1u : 0u);
+        umma_commit(bar(kODone + 2 * tile + (i & 1)));
       };
-      guarded(bar(kQReady), 0);
+      // scores run one chunk ahead; a buffer of theirs is free again behind the product that read P from it (the tensor core works in order)
+      Ring<SH::STAGES> kr, vr;
+      polled(bar(kQReady), 0);
       for (int i = 0; i <= chunks; ++i) {
-        if (i < chunks) guarded(bar(kKReady + (i & 1)), i >> 1 & 1);
-        if (i > 0) guarded(bar(kVReady + (i - 1 & 1)), i - 1 >> 1 & 1);
+        if (i < chunks) {
+          polled(bar(kKReady + kr.slot), kr.phase);
+          tc_fence_after();
 #pragma unroll
-        for (int tile = 0; tile < TILES; ++tile) {
-          if (i > 0) {
-            guarded(bar(kPReady + tile), (i - 1) & 1);
+          for (int tile = 0; tile < TILES; ++tile) scores(i, kr.slot, tile);
+          umma_commit(bar(kKEmpty + kr.slot));
+          kr.next();
+        }
+        if (i > 0) {
+          polled(bar(kVReady + vr.slot), vr.phase);
+#pragma unroll
+          for (int tile = 0; tile < TILES; ++tile) {
+            polled(bar(kPReady + 2 * tile + (i - 1 & 1)), i - 1 >> 1 & 1);
             tc_fence_after();
-            values(i - 1, tile);
-            if (i == chunks) umma_commit(bar(kODone + tile));
-            else if (tile == TILES - 1) umma_commit(bar(kVEmpty + (i - 1 & 1)));
+            values(i - 1, vr.slot, tile);
           }
-          if (i < chunks) {
-            tc_fence_after();
-            scores(i, tile);                        // in order behind the product that read P from the same columns
-            if (tile == TILES - 1) umma_commit(bar(kKEmpty + (i & 1)));
-          }
+          if (i < chunks) umma_commit(bar(kVEmpty + vr.slot));       // (nothing is left in flight behind the last product)
+          vr.next();
         }
       }
     }
@@ -233,13 +263,14 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
     const int t4 = tid - 128, row = t4 % BN, part = t4 / BN;
     const int turn = D == 64 ? row >> 2 : D == 128 ? row >> 1 : row; // which piece first: spreads the rows over the banks
     int grown = -100;                                                // values so far are below 2^grown
-    for (int i = 0; i < chunks; ++i) {
-      const int stage = i & 1;
-      const uint8_t* const raw = smem + SH::OFF_RAW + stage * SH::RAW_BYTES;
-      guarded(bar(kRawFull + stage), i >> 1 & 1);
+    Ring<SH::RAW> from;
+    Ring<SH::STAGES> to;
+    for (int i = 0; i < chunks; ++i, from.next(), to.next()) {
+      const uint8_t* const raw = smem + SH::OFF_RAW + from.slot * SH::RAW_BYTES;
+      guarded(bar(kRawFull + from.slot), from.phase);
       const uint32_t* const kp = reinterpret_cast<const uint32_t*>(raw + 2 * SH::CODE_BYTES);
       const uint32_t* const vp = kp + BN;
-      const uint32_t mask = s_mask[i & 7];
+      const uint32_t mask = s_mask[i % kRing];
       const int t0 = begin + i * BN;
       // the chunk's largest key and value element; what is not there or not finite does not count
       float top_k = 0.0f, top_v = 0.0f;
@@ -259,8 +290,8 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
       }
       const int ek = above(top_k), ev = max(grown, above(top_v));
       if (t4 == 0) {
-        s_key[i & 7] = pow2(max(ek - 14, -126));
-        s_value[i & 7] = pow2(max(grown - ev, -126));
+        s_key[i % kRing] = pow2(max(ek - 14, -126));
+        s_value[i % kRing] = pow2(max(grown - ev, -126));
         *s_last = pow2(max(ev - 14, -126));
       }
       grown = ev;
@@ -277,26 +308,26 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
         for (int n = 0; n < PER; ++n) {
           const int piece = (turn + n + part * PER) % CHUNKS16;
           const uint4 x = *reinterpret_cast<const uint4*>(codes + row * (D / 2) + piece * 16);
-          uint8_t* const to = dst + (piece >> 1) * (BN * 128) + row * 128;
+          uint8_t* const line = dst + (piece >> 1) * (BN * 128) + row * 128;
           const int first = (piece & 1) * 4, swizzle = row & 7;
-          *reinterpret_cast<uint4*>(to + (((first + 0) ^ swizzle) << 4)) = eight(x.x, s, m);
-          *reinterpret_cast<uint4*>(to + (((first + 1) ^ swizzle) << 4)) = eight(x.y, s, m);
-          *reinterpret_cast<uint4*>(to + (((first + 2) ^ swizzle) << 4)) = eight(x.z, s, m);
-          *reinterpret_cast<uint4*>(to + (((first + 3) ^ swizzle) << 4)) = eight(x.w, s, m);
+          *reinterpret_cast<uint4*>(line + (((first + 0) ^ swizzle) << 4)) = eight(x.x, s, m);
+          *reinterpret_cast<uint4*>(line + (((first + 1) ^ swizzle) << 4)) = eight(x.y, s, m);
+          *reinterpret_cast<uint4*>(line + (((first + 2) ^ swizzle) << 4)) = eight(x.z, s, m);
+          *reinterpret_cast<uint4*>(line + (((first + 3) ^ swizzle) << 4)) = eight(x.w, s, m);
         }
       };
-      guarded(bar(kKEmpty + stage), (i >> 1 & 1) ^ 1);
-      convert(raw, smem + SH::OFF_K + stage * SH::KV_BYTES, ks, km);
+      guarded(bar(kKEmpty + to.slot), to.phase ^ 1);
+      convert(raw, smem + SH::OFF_K + to.slot * SH::KV_BYTES, ks, km);
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kKReady + stage));
-      guarded(bar(kVEmpty + stage), (i >> 1 & 1) ^ 1);
-      convert(raw + SH::CODE_BYTES, smem + SH::OFF_V + stage * SH::KV_BYTES, vs, vm);
+      if (lane == 0) mbar_arrive(bar(kKReady + to.slot));
+      guarded(bar(kVEmpty + to.slot), to.phase ^ 1);
+      convert(raw + SH::CODE_BYTES, smem + SH::OFF_V + to.slot * SH::KV_BYTES, vs, vm);
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(bar(kVReady + stage));
-        mbar_arrive(bar(kRawEmpty + stage));
+        mbar_arrive(bar(kVReady + to.slot));
+        mbar_arrive(bar(kRawEmpty + from.slot));
       }
     }
   } else if (warp >= 8) {
@@ -337,16 +368,17 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
     }
     const int hi = real ? pos0 + j : -1, lo = a.window ? (int)max((long long)pos0 + j - a.window + 1, 0LL) : 0;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const uint32_t s_at = tmem + lanes + tile * BN, p_at = s_at + SH::P_COL, o_at = tmem + lanes + SH::O_COL + tile * D;
+    const uint32_t s_tile = tmem + lanes + 2 * tile * BN, o_at = tmem + lanes + SH::O_COL + tile * D;
     float m = kLowest;
     Two l(0.0f);
     for (int i = 0; i < chunks; ++i) {
-      guarded(bar(kSFull + tile), i & 1);
+      guarded(bar(kSFull + 2 * tile + (i & 1)), i >> 1 & 1);
       tc_fence_after();
+      const uint32_t s_at = s_tile + (i & 1) * BN;
       const int t0 = begin + i * BN;
-      const float f = fminf(fmaxf(factor * s_key[i & 7], 7.5e-37f), 1.3e30f), ratio = s_value[i & 7];
-      const uint32_t there = s_mask[i & 7];
-      const bool all = there == (BN == 128 ? 0xffu : 0xfu) && t0 + BN - 1 <= hi && t0 >= lo;
+      const float f = fminf(fmaxf(factor * s_key[i % kRing], 7.5e-37f), 1.3e30f), ratio = s_value[i % kRing];
+      const uint32_t there = s_mask[i % kRing];
+      const bool all = there == 0xfu && t0 + BN - 1 <= hi && t0 >= lo;
       const bool masked = __any_sync(0xffffffffu, !all);
       // which of the 32 keys from t on this row sees
       auto visible = [&](int n) {
@@ -372,19 +404,15 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
         return fmaxf(x, y);
       };
       uint32_t ra[32], rb[32];
-      float top = kLowest;
-#pragma unroll
-      for (int n = 0; n < BN / 64; ++n) {            // the last pair stays in registers
-        tmem_ld_32x32(s_at + 64 * n, ra);
-        tmem_ld_32x32(s_at + 64 * n + 32, rb);
-        wait_ld_dep32(ra);
-        wait_ld_dep32(rb);
-        if (masked) {
-          hide(ra, 2 * n);
-          hide(rb, 2 * n + 1);
-        }
-        top = fmaxf(top, fmaxf(largest(ra), largest(rb)));
+      tmem_ld_32x32(s_at, ra);
+      tmem_ld_32x32(s_at + 32, rb);
+      wait_ld_dep32(ra);
+      wait_ld_dep32(rb);
+      if (masked) {
+        hide(ra, 0);
+        hide(rb, 1);
       }
+      float top = fmaxf(largest(ra), largest(rb));
       top *= f;
       const bool moves = top > m + 8.0f || (m == kLowest && top > kLowest);
       if (__any_sync(0xffffffffu, moves) || ratio != 1.0f) {
@@ -392,7 +420,9 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
         const float alpha = m == next ? 1.0f : exp2_fast(m - next);
         m = next;
         l = l * Two(alpha);
-        if (i > 0) {                                 // O is complete: the scores were issued behind the product before
+        if (i > 0) {
+          guarded(bar(kODone + 2 * tile + (i - 1 & 1)), i - 1 >> 1 & 1);       // the product before has to be in O
+          tc_fence_after();
           const Two by(alpha * ratio);
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
@@ -419,29 +449,17 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
           l = l + Two(p.x, p.y);
           h[e] = half2_bits(__floats2half2_rn(p.x, p.y));
         }
-        tmem_st_32x16(p_at + 16 * n, h);
+        tmem_st_32x16(s_at + 16 * n, h);             // over the scores, which are all in registers
       };
-      weigh(ra, BN / 32 - 2);
-      weigh(rb, BN / 32 - 1);
-      if constexpr (BN == 128) {                     // the upper half of the scores has been read: P takes its place
-        tmem_ld_32x32(s_at, ra);
-        tmem_ld_32x32(s_at + 32, rb);
-        wait_ld_dep32(ra);
-        wait_ld_dep32(rb);
-        if (masked) {
-          hide(ra, 0);
-          hide(rb, 1);
-        }
-        weigh(ra, 0);
-        weigh(rb, 1);
-      }
+      weigh(ra, 0);
+      weigh(rb, 1);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kPReady + tile));
+      if (lane == 0) mbar_arrive(bar(kPReady + 2 * tile + (i & 1)));
     }
     if (chunks > 0) {
-      guarded(bar(kODone + tile), 0);
+      guarded(bar(kODone + 2 * tile + (chunks - 1 & 1)), chunks - 1 >> 1 & 1);
       tc_fence_after();
     }
     const float2 sums = l.both();
@@ -478,9 +496,9 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
   }
 }
 
-template <typename T, int D, int TILES, int BN>
+template <typename T, int D, int TILES, int STAGES, int RAW>
 int run(const AttnArgs& a, cudaStream_t stream) {
-  using SH = PromptShape<D, TILES, BN>;
+  using SH = PromptShape<D, TILES, STAGES, RAW>;
   const long long items = ((long long)a.tokens * a.each / SH::ROWS + a.batch) * a.kv_heads;
   XQT_REQUIRE(items < (1LL << 31) - 1);
   XQT_SMEM_OPT_IN((kv4_prompt_kernel<T, SH>), SH::SMEM);
@@ -489,9 +507,9 @@ int run(const AttnArgs& a, cudaStream_t stream) {
 
 template <typename T>
 int run_dim(const AttnArgs& a, int dim, cudaStream_t stream) {
-  if (dim == 64) return run<T, 64, 2, 128>(a, stream);
-  if (dim == 128) return run<T, 128, 2, 128>(a, stream);
-  return run<T, 256, 1, 64>(a, stream);
+  if (dim == 64) return run<T, 64, 2, 4, 4>(a, stream);
+  if (dim == 128) return run<T, 128, 2, 4, 3>(a, stream);
+  return run<T, 256, 1, 2, 2>(a, stream);
 }
 
 }  // namespace

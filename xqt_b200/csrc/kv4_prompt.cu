@@ -34,26 +34,27 @@ namespace {
 
 using namespace kv4;
 
-template <int D_, int TILES_, int STAGES_, int RAW_>
+template <int D_, int TILES_, int STAGES_>
 struct PromptShape {
-  static constexpr int D = D_, TILES = TILES_, STAGES = STAGES_, RAW = RAW_, BN = 64;
+  static constexpr int D = D_, TILES = TILES_, STAGES = STAGES_, BN = 64;     // STAGES: of codes, keys and values
+  static constexpr int GROUP_WARPS = 4 / STAGES;               // that convert one chunk
   static constexpr int ROWS = 128 * TILES, UNIT = 1 << 20, CT = BN, OPENING = 1;
   static constexpr bool PROMPT = true;
   static constexpr int THREADS = 256 + 128 * TILES;
   static constexpr int BLOCKS = D / 64;                        // 128-byte wide column blocks of an operand
   static constexpr int Q_BYTES = ROWS * D * 2, KV_BYTES = BN * D * 2;
   static constexpr int CODE_BYTES = BN * D / 2, PARAM_BYTES = BN * 4, RAW_BYTES = 2 * (CODE_BYTES + PARAM_BYTES);
-  static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + STAGES * KV_BYTES, OFF_RAW = OFF_V + STAGES * KV_BYTES, OFF_MISC = OFF_RAW + RAW * RAW_BYTES;
-  static constexpr int SMEM = OFF_MISC + 512;
+  static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + STAGES * KV_BYTES, OFF_RAW = OFF_V + STAGES * KV_BYTES, OFF_MISC = OFF_RAW + STAGES * RAW_BYTES;
+  static constexpr int SMEM = OFF_MISC + 640;
   // tensor memory: two buffers of scores per tile from column 0, P over the first half of its scores; O from 256
   static constexpr uint32_t O_COL = 256;
-  static_assert(2 * TILES * BN <= 256 && TILES * D <= 256 && SMEM <= 227 * 1024 && STAGES <= 4 && RAW <= 4, "tensor and shared memory");
+  static_assert(2 * TILES * BN <= 256 && TILES * D <= 256 && SMEM <= 227 * 1024 && (STAGES == 2 || STAGES == 4), "tensor and shared memory");
 };
 
-// Barriers, in 8-byte words behind the tiles.  The last four kinds are per tile and chunk parity: a softmax warp may be a chunk ahead of its
+// Barriers, in 8-byte words behind the tiles.  Those of scores, P and O are per tile and chunk parity: a softmax warp may be a chunk ahead of its
 // neighbours, and a wait may come two products late.
-enum : int { kRawFull = 0, kRawEmpty = 4, kKReady = 8, kVReady = 12, kKEmpty = 16, kVEmpty = 20, kSFull = 24, kPReady = 28, kODone = 32, kQReady = 36, kBarriers = 37 };
-constexpr int kRing = 16;          // chunks that loader, conversion and softmax may lie apart: more than 2 + STAGES + RAW
+enum : int { kRawFull = 0, kRawEmpty = 4, kKReady = 8, kVReady = 12, kKEmpty = 16, kVEmpty = 20, kSFull = 24, kPReady = 28, kODone = 32, kGrown = 36, kQReady = 40, kBarriers = 41 };
+constexpr int kRing = 16;          // chunks that loader, conversion and softmax may lie apart: more than 2 + 2 * STAGES
 
 template <int N>
 struct Ring {
@@ -113,12 +114,13 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
   uint8_t* const misc = smem + SH::OFF_MISC;
   const uint32_t bar0 = smem_addr(misc);
   auto bar = [&](int slot) { return bar0 + 8u * (uint32_t)slot; };
-  volatile uint32_t* const s_mask = reinterpret_cast<volatile uint32_t*>(misc + 296);       // [kRing] which 16-key groups of a chunk are there
-  volatile float* const s_key = reinterpret_cast<volatile float*>(misc + 360);               // [kRing] what a chunk's keys were divided by
-  volatile float* const s_value = reinterpret_cast<volatile float*>(misc + 424);             // [kRing] what O has to be multiplied by before it
-  volatile float* const s_last = reinterpret_cast<volatile float*>(misc + 488);              // what the values were divided by in the end
-  volatile uint32_t* const s_abort = reinterpret_cast<volatile uint32_t*>(misc + 492);
-  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(misc + 496);
+  volatile uint32_t* const s_mask = reinterpret_cast<volatile uint32_t*>(misc + 328);       // [kRing] which 16-key groups of a chunk are there
+  volatile float* const s_key = reinterpret_cast<volatile float*>(misc + 392);               // [kRing] what a chunk's keys were divided by
+  volatile float* const s_value = reinterpret_cast<volatile float*>(misc + 456);             // [kRing] what O has to be multiplied by before it
+  volatile float* const s_last = reinterpret_cast<volatile float*>(misc + 520);              // what the values were divided by in the end
+  volatile uint32_t* const s_abort = reinterpret_cast<volatile uint32_t*>(misc + 524);
+  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(misc + 528);
+  volatile int* const s_grown = reinterpret_cast<volatile int*>(misc + 532);                // [4] values so far are below 2^this
 
   grid_launch_dependents();
   grid_dependency_wait();
@@ -139,9 +141,10 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
     *s_abort = 0;
     for (int i = 0; i < 4; ++i) {
       mbar_init(bar(kRawFull + i), 1);
-      mbar_init(bar(kRawEmpty + i), 4);
-      mbar_init(bar(kKReady + i), 4);
-      mbar_init(bar(kVReady + i), 4);
+      mbar_init(bar(kRawEmpty + i), SH::GROUP_WARPS);
+      mbar_init(bar(kKReady + i), SH::GROUP_WARPS);
+      mbar_init(bar(kVReady + i), SH::GROUP_WARPS);
+      mbar_init(bar(kGrown + i), 1);
       mbar_init(bar(kKEmpty + i), 1);
       mbar_init(bar(kVEmpty + i), 1);
       mbar_init(bar(kSFull + i), 1);
@@ -190,7 +193,7 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
       return i < chunks && piece < pieces && at < w.s.len ? table[at >> a.page_shift] : -1;
     };
     int page = look_up(0);
-    Ring<SH::RAW> ring;
+    Ring<SH::STAGES> ring;
     for (int i = 0; i < chunks; ++i, ring.next()) {
       const int stage = ring.slot, following = look_up(i + 1);
       const bool valid = (unsigned)page < (unsigned)a.pages;
@@ -258,77 +261,85 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
       }
     }
   } else if (warp >= 4 && warp < 8) {
-    // ------------------------------------------------------------ codes -> fp16
-    constexpr int CHUNKS16 = D / 32, PER = CHUNKS16 * BN / 128;      // 16-byte pieces of a key's codes, and how many of them a thread does
-    const int t4 = tid - 128, row = t4 % BN, part = t4 / BN;
-    const int turn = D == 64 ? row >> 2 : D == 128 ? row >> 1 : row; // which piece first: spreads the rows over the banks
-    int grown = -100;                                                // values so far are below 2^grown
-    Ring<SH::RAW> from;
-    Ring<SH::STAGES> to;
-    for (int i = 0; i < chunks; ++i, from.next(), to.next()) {
-      const uint8_t* const raw = smem + SH::OFF_RAW + from.slot * SH::RAW_BYTES;
-      guarded(bar(kRawFull + from.slot), from.phase);
+    // ------------------------------------------------------------ codes -> fp16, chunk i by the warps of group i % STAGES
+    // (converting a chunk is a chain of waits and shuffles that a warp cannot overlap with itself; a group has a slot of each ring to itself,
+    // so the phase that it waits for is never two away)
+    constexpr int PIECES = D / 32;                                   // 16-byte pieces of a key's codes
+    constexpr int GROUP = SH::GROUP_WARPS;
+    const int slot = (warp & 3) / GROUP;
+    const uint8_t* const raw = smem + SH::OFF_RAW + slot * SH::RAW_BYTES;
+    for (int i = slot, phase = 0; i < chunks; i += SH::STAGES, phase ^= 1) {
+      guarded(bar(kRawFull + slot), phase);
       const uint32_t* const kp = reinterpret_cast<const uint32_t*>(raw + 2 * SH::CODE_BYTES);
       const uint32_t* const vp = kp + BN;
       const uint32_t mask = s_mask[i % kRing];
       const int t0 = begin + i * BN;
       // the chunk's largest key and value element; what is not there or not finite does not count
+      float2 k[2], v[2];
+      bool there[2], k_good[2], v_good[2];
       float top_k = 0.0f, top_v = 0.0f;
 #pragma unroll
-      for (int r = lane; r < BN; r += 32) {
-        if ((mask >> (r >> 4) & 1u) && t0 + r < w.s.len) {
-          const float2 k = pair_of<T>(kp[r]), v = pair_of<T>(vp[r]);
-          const float tk = fmaxf(fabsf(k.y), fabsf(fmaf(15.0f, k.x, k.y))), tv = fmaxf(fabsf(v.y), fabsf(fmaf(15.0f, v.x, v.y)));
-          if (tk <= 3.402823466e38f) top_k = fmaxf(top_k, tk);
-          if (tv <= 3.402823466e38f) top_v = fmaxf(top_v, tv);
-        }
+      for (int n = 0; n < 2; ++n) {
+        const int row = lane + 32 * n;
+        there[n] = (mask >> (row >> 4) & 1u) && t0 + row < w.s.len;
+        k[n] = pair_of<T>(kp[row]);
+        v[n] = pair_of<T>(vp[row]);
+        v_good[n] = fabsf(v[n].x) <= 3.402823466e38f && fabsf(v[n].y) <= 3.402823466e38f;
+        k_good[n] = fabsf(k[n].x) <= 3.402823466e38f && fabsf(k[n].y) <= 3.402823466e38f;
+        const float tk = fmaxf(fabsf(k[n].y), fabsf(fmaf(15.0f, k[n].x, k[n].y))), tv = fmaxf(fabsf(v[n].y), fabsf(fmaf(15.0f, v[n].x, v[n].y)));
+        if (there[n] && k_good[n]) top_k = fmaxf(top_k, fminf(tk, 3.402823466e38f));
+        if (there[n] && v_good[n]) top_v = fmaxf(top_v, fminf(tv, 3.402823466e38f));
       }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        top_k = fmaxf(top_k, __shfl_xor_sync(0xffffffffu, top_k, o));
-        top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, o));
-      }
-      const int ek = above(top_k), ev = max(grown, above(top_v));
-      if (t4 == 0) {
+      const int ek = above(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top_k))));      // (positive floats order as their bits)
+      const int own = above(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v))));
+      // values are divided by a power that only grows: the chunk before says how far it has
+      if (i > 0) guarded(bar(kGrown + (i - 1 & 3)), (i - 1) >> 2 & 1);
+      const int grown = i > 0 ? s_grown[i - 1 & 3] : -100, ev = max(grown, own);
+      __syncwarp();
+      if (lane == 0 && (warp & 3) % GROUP == 0) {
+        s_grown[i & 3] = ev;
         s_key[i % kRing] = pow2(max(ek - 14, -126));
         s_value[i % kRing] = pow2(max(grown - ev, -126));
-        *s_last = pow2(max(ev - 14, -126));
+        if (i == chunks - 1) *s_last = pow2(max(ev - 14, -126));
+        mbar_arrive(bar(kGrown + (i & 3)));
       }
-      grown = ev;
-      const bool there = (mask >> (row >> 4) & 1u) && t0 + row < w.s.len;
-      const float2 k = pair_of<T>(kp[row]), v = pair_of<T>(vp[row]);
-      const bool v_good = fabsf(v.x) <= 3.402823466e38f && fabsf(v.y) <= 3.402823466e38f;
-      const bool k_good = fabsf(k.x) <= 3.402823466e38f && fabsf(k.y) <= 3.402823466e38f && v_good;
-      const float fk = pow2(14 - ek), fv = pow2(14 - ev);
-      const float nan = __int_as_float(0x7fffffff);
-      const __half2 ks = __float2half2_rn(!there ? 0.0f : k_good ? k.x * fk : nan), km = __float2half2_rn(!there ? 0.0f : k_good ? k.y * fk : nan);
-      const __half2 vs = __float2half2_rn(there && v_good ? v.x * fv : 0.0f), vm = __float2half2_rn(there && v_good ? v.y * fv : 0.0f);
-      auto convert = [&](const uint8_t* codes, uint8_t* dst, __half2 s, __half2 m) {
-#pragma unroll
-        for (int n = 0; n < PER; ++n) {
-          const int piece = (turn + n + part * PER) % CHUNKS16;
-          const uint4 x = *reinterpret_cast<const uint4*>(codes + row * (D / 2) + piece * 16);
-          uint8_t* const line = dst + (piece >> 1) * (BN * 128) + row * 128;
-          const int first = (piece & 1) * 4, swizzle = row & 7;
-          *reinterpret_cast<uint4*>(line + (((first + 0) ^ swizzle) << 4)) = eight(x.x, s, m);
-          *reinterpret_cast<uint4*>(line + (((first + 1) ^ swizzle) << 4)) = eight(x.y, s, m);
-          *reinterpret_cast<uint4*>(line + (((first + 2) ^ swizzle) << 4)) = eight(x.z, s, m);
-          *reinterpret_cast<uint4*>(line + (((first + 3) ^ swizzle) << 4)) = eight(x.w, s, m);
+      const float fk = pow2(14 - ek), fv = pow2(14 - ev), nan = __int_as_float(0x7fffffff);
+      // K, then V: a row (or two) of this lane's in each.  One small loop body: unrolled, the four groups' places in the code evict one another
+      // from the instruction cache (8192-token prompt: 1098 us)
+#pragma unroll 1
+      for (int which = 0; which < 2; ++which) {
+        guarded(bar((which ? kVEmpty : kKEmpty) + slot), phase ^ 1);
+        const uint8_t* const codes = raw + which * SH::CODE_BYTES;
+        uint8_t* const dst = smem + (which ? SH::OFF_V : SH::OFF_K) + slot * SH::KV_BYTES;
+#pragma unroll 1
+        for (int n = GROUP == 2 ? warp & 1 : 0; n < (GROUP == 2 ? (warp & 1) + 1 : 2); ++n) {
+          const int row = lane + 32 * n;
+          const bool here = n ? there[1] : there[0], good = (n ? v_good[1] : v_good[0]) && (which || (n ? k_good[1] : k_good[0]));
+          const float2 par = which ? (n ? v[1] : v[0]) : (n ? k[1] : k[0]);
+          const float by = which ? fv : fk, bad = which ? 0.0f : nan;
+          const __half2 s = __float2half2_rn(!here ? 0.0f : good ? par.x * by : bad), m = __float2half2_rn(!here ? 0.0f : good ? par.y * by : bad);
+          const int turn = D == 64 ? row >> 2 : D == 128 ? row >> 1 : row;       // which piece first: spreads the rows over the banks
+          const uint8_t* const src = codes + row * (D / 2);
+          uint8_t* const lines = dst + row * 128;
+          uint4 x = *reinterpret_cast<const uint4*>(src + turn % PIECES * 16);
+#pragma unroll 1
+          for (int e = 0; e < PIECES; ++e) {
+            const int piece = (turn + e) % PIECES;
+            const uint4 following = *reinterpret_cast<const uint4*>(src + (turn + e + 1) % PIECES * 16);
+            uint8_t* const line = lines + (piece >> 1) * (BN * 128);
+            const int first = (piece & 1) * 4, swizzle = row & 7;
+            *reinterpret_cast<uint4*>(line + (((first + 0) ^ swizzle) << 4)) = eight(x.x, s, m);
+            *reinterpret_cast<uint4*>(line + (((first + 1) ^ swizzle) << 4)) = eight(x.y, s, m);
+            *reinterpret_cast<uint4*>(line + (((first + 2) ^ swizzle) << 4)) = eight(x.z, s, m);
+            *reinterpret_cast<uint4*>(line + (((first + 3) ^ swizzle) << 4)) = eight(x.w, s, m);
+            x = following;
+          }
         }
-      };
-      guarded(bar(kKEmpty + to.slot), to.phase ^ 1);
-      convert(raw, smem + SH::OFF_K + to.slot * SH::KV_BYTES, ks, km);
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kKReady + to.slot));
-      guarded(bar(kVEmpty + to.slot), to.phase ^ 1);
-      convert(raw + SH::CODE_BYTES, smem + SH::OFF_V + to.slot * SH::KV_BYTES, vs, vm);
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(bar(kVReady + to.slot));
-        mbar_arrive(bar(kRawEmpty + from.slot));
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar((which ? kVReady : kKReady) + slot));
       }
+      if (lane == 0) mbar_arrive(bar(kRawEmpty + slot));
     }
   } else if (warp >= 8) {
     // ------------------------------------------------------------ softmax: a thread per row
@@ -496,9 +507,9 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
   }
 }
 
-template <typename T, int D, int TILES, int STAGES, int RAW>
+template <typename T, int D, int TILES, int STAGES>
 int run(const AttnArgs& a, cudaStream_t stream) {
-  using SH = PromptShape<D, TILES, STAGES, RAW>;
+  using SH = PromptShape<D, TILES, STAGES>;
   const long long items = ((long long)a.tokens * a.each / SH::ROWS + a.batch) * a.kv_heads;
   XQT_REQUIRE(items < (1LL << 31) - 1);
   XQT_SMEM_OPT_IN((kv4_prompt_kernel<T, SH>), SH::SMEM);
@@ -507,9 +518,9 @@ int run(const AttnArgs& a, cudaStream_t stream) {
 
 template <typename T>
 int run_dim(const AttnArgs& a, int dim, cudaStream_t stream) {
-  if (dim == 64) return run<T, 64, 2, 4, 4>(a, stream);
-  if (dim == 128) return run<T, 128, 2, 4, 3>(a, stream);
-  return run<T, 256, 1, 2, 2>(a, stream);
+  if (dim == 64) return run<T, 64, 2, 4>(a, stream);
+  if (dim == 128) return run<T, 128, 2, 4>(a, stream);
+  return run<T, 256, 1, 2>(a, stream);
 }
 
 }  // namespace

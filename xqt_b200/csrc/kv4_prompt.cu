@@ -8,8 +8,9 @@
 // works on this one's.
 //
 //   warp 0       table look-ups and bulk copies
-//   warp 1       tcgen05.mma
 //   warp 2       allocates tensor memory
+//   warps 1, 3   tcgen05.mma, one issuer per row tile: an answer of a barrier takes about 200 clocks, and one thread waiting for both tiles in
+//                turn set the pace (8192-token prompt: 605 us with all other work left out)
 //   warps 4-7    codes -> fp16
 //   warps 8-15   softmax, rescaling of O, result
 //
@@ -145,8 +146,8 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
       mbar_init(bar(kKReady + i), SH::GROUP_WARPS);
       mbar_init(bar(kVReady + i), SH::GROUP_WARPS);
       mbar_init(bar(kGrown + i), 1);
-      mbar_init(bar(kKEmpty + i), 1);
-      mbar_init(bar(kVEmpty + i), 1);
+      mbar_init(bar(kKEmpty + i), TILES);
+      mbar_init(bar(kVEmpty + i), TILES);
       mbar_init(bar(kSFull + i), 1);
       mbar_init(bar(kPReady + i), 4);
       mbar_init(bar(kODone + i), 1);
@@ -176,6 +177,16 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
       *s_abort = 1u;
       if (a.status) *a.status = 1u;
     }
+  };
+
+  auto polled2 = [&](uint32_t b0, uint32_t parity0, uint32_t b1, uint32_t parity1) {
+    if (*s_abort != 0u) return;
+    for (uint32_t i = 0; i < (kSpinLimit << 3); ++i) {
+      const bool x = mbar_test_wait(b0, parity0), y = mbar_test_wait(b1, parity1);
+      if (x && y) return;
+    }
+    *s_abort = 1u;
+    if (a.status) *a.status = 1u;
   };
 
   if (warp == 0) {
@@ -212,49 +223,40 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
         bulk_g2s(target + stage * SH::RAW_BYTES, source + page * page_bytes + (long long)(at & (a.page_size - 1)) * row_bytes, (uint32_t)(psz * row_bytes), bar(kRawFull + stage));
       page = following;
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ the tensor core
+  } else if (warp == 1 || (TILES == 2 && warp == 3)) {
+    // ------------------------------------------------------------ the tensor core, for one row tile
     if (elect_one() && chunks > 0) {
       constexpr uint32_t kScores = umma_idesc(kAccF32, kFmtF16, kFmtF16, 128, BN);
       constexpr uint32_t kOut = umma_idesc(kAccF32, kFmtF16, kFmtF16, 128, D) | 1u << 16;      // second operand: long side contiguous
-      const uint32_t base = smem_addr(smem);
-      auto scores = [&](int i, int stage, int tile) {
-        const int at = 2 * tile + (i & 1);
-#pragma unroll
-        for (int kb = 0; kb < BLOCKS; ++kb) {
-          const uint64_t ad = umma_desc_sw128(base + (tile * BLOCKS + kb) * (128 * 128)), bd = umma_desc_sw128(base + SH::OFF_K + stage * SH::KV_BYTES + kb * (BN * 128));
-#pragma unroll
-          for (int s = 0; s < 4; ++s) umma_ss(tmem + at * BN, ad + 2 * s, bd + 2 * s, kScores, kb || s ? 1u : 0u);
-        }
-        umma_commit(bar(kSFull + at));
-      };
-      auto values = [&](int i, int stage, int tile) {
-#pragma unroll
-        for (int s = 0; s < BN / 16; ++s)
-          umma_ts_f16(tmem + SH::O_COL + tile * D, tmem + (2 * tile + (i & 1)) * BN + 8 * s,
-                      umma_desc_mn_sw128(base + SH::OFF_V + stage * SH::KV_BYTES + s * 2048, BN * 128), kOut, i || s ? 1u : 0u);
-        umma_commit(bar(kODone + 2 * tile + (i & 1)));
-      };
+      const int tile = warp >> 1;
+      const uint32_t base = smem_addr(smem), s_tile = tmem + 2 * tile * BN, o_tile = tmem + SH::O_COL + tile * D;
+      const uint64_t q_desc = umma_desc_sw128(base + tile * (BLOCKS * 128 * 128)), k_desc = umma_desc_sw128(base + SH::OFF_K);
+      const uint64_t v_desc = umma_desc_mn_sw128(base + SH::OFF_V, BN * 128);
       // scores run one chunk ahead; a buffer of theirs is free again behind the product that read P from it (the tensor core works in order)
       Ring<SH::STAGES> kr, vr;
       polled(bar(kQReady), 0);
+      bool k_ready = false;
       for (int i = 0; i <= chunks; ++i) {
         if (i < chunks) {
-          polled(bar(kKReady + kr.slot), kr.phase);
+          if (!k_ready) polled(bar(kKReady + kr.slot), kr.phase);
           tc_fence_after();
+          const uint64_t kd = k_desc + kr.slot * (SH::KV_BYTES >> 4);
 #pragma unroll
-          for (int tile = 0; tile < TILES; ++tile) scores(i, kr.slot, tile);
+          for (int s = 0; s < D / 16; ++s)
+            umma_ss(s_tile + (i & 1) * BN, q_desc + (s >> 2) * (128 * 128 >> 4) + 2 * (s & 3), kd + (s >> 2) * (BN * 128 >> 4) + 2 * (s & 3), kScores, s ? 1u : 0u);
+          umma_commit(bar(kSFull + 2 * tile + (i & 1)));
           umma_commit(bar(kKEmpty + kr.slot));
           kr.next();
         }
+        k_ready = i + 1 < chunks && mbar_test_wait(bar(kKReady + kr.slot), kr.phase);      // answered while the wait below goes on
         if (i > 0) {
-          polled(bar(kVReady + vr.slot), vr.phase);
+          const int last = i - 1;
+          polled2(bar(kVReady + vr.slot), vr.phase, bar(kPReady + 2 * tile + (last & 1)), last >> 1 & 1);
+          tc_fence_after();
+          const uint64_t vd = v_desc + vr.slot * (SH::KV_BYTES >> 4);
 #pragma unroll
-          for (int tile = 0; tile < TILES; ++tile) {
-            polled(bar(kPReady + 2 * tile + (i - 1 & 1)), i - 1 >> 1 & 1);
-            tc_fence_after();
-            values(i - 1, vr.slot, tile);
-          }
+          for (int s = 0; s < BN / 16; ++s) umma_ts_f16(o_tile, s_tile + (last & 1) * BN + 8 * s, vd + s * (2048 >> 4), kOut, last || s ? 1u : 0u);
+          umma_commit(bar(kODone + 2 * tile + (last & 1)));
           if (i < chunks) umma_commit(bar(kVEmpty + vr.slot));       // (nothing is left in flight behind the last product)
           vr.next();
         }
@@ -382,8 +384,9 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
     const uint32_t s_tile = tmem + lanes + 2 * tile * BN, o_at = tmem + lanes + SH::O_COL + tile * D;
     float m = kLowest;
     Two l(0.0f);
+    bool s_ready = false;
     for (int i = 0; i < chunks; ++i) {
-      guarded(bar(kSFull + 2 * tile + (i & 1)), i >> 1 & 1);
+      if (!s_ready) guarded(bar(kSFull + 2 * tile + (i & 1)), i >> 1 & 1);
       tc_fence_after();
       const uint32_t s_at = s_tile + (i & 1) * BN;
       const int t0 = begin + i * BN;
@@ -463,6 +466,7 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
         tmem_st_32x16(s_at + 16 * n, h);             // over the scores, which are all in registers
       };
       weigh(ra, 0);
+      s_ready = i + 1 < chunks && mbar_test_wait(bar(kSFull + 2 * tile + (i + 1 & 1)), i + 1 >> 1 & 1);
       weigh(rb, 1);
       tmem_wait_st();
       tc_fence_before();

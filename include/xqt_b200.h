@@ -480,7 +480,8 @@ int xqt_b200_kv4_gather(const void* codes, const void* params, const void* slots
  * sees nothing is 0; lengths and starts are clamped to the table and to `tokens`; rows of no sequence are not written.
  * page_size: a power of two, 16 to 4096.  strides (host): token and head stride of q in elements (multiples of 8), row stride of
  * table.  Workspace of the given size, 16-byte aligned, any contents, not shared with a call that may overlap. */
-size_t xqt_b200_kv4_attention_workspace_bytes(int dim);
+size_t xqt_b200_kv4_attention_workspace_bytes(int tokens, int batch, int q_heads, int kv_heads, int dim,
+                                              int has_query_starts);
 int xqt_b200_kv4_attention(const void* q, const void* codes, const void* params, const int* table, const int* seq_lens,
                            const int* query_starts, void* out, const long long* strides, int tokens, int batch,
                            int q_heads, int kv_heads, int dim, long long pages, int page_size, int table_width,

@@ -58,7 +58,7 @@ def cache_key() -> str:
 def host_cache_key() -> str:
     import torch
 
-    return _digest(HOST_FLAGS + [torch.__version__, sys.version], [HOST_SOURCE] + sorted(INCLUDE.glob("*.h")))
+    return _digest(HOST_FLAGS + [torch.__version__, sys.version], [HOST_SOURCE] + sorted(CSRC.glob("*.h")) + sorted(INCLUDE.glob("*.h")))
 
 
 def _stamped(output: pathlib.Path, stamp: pathlib.Path, key: str) -> bool:

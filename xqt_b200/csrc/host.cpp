@@ -19,6 +19,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <structmember.h>
 
+#include <cmath>
 #include <cstring>
 #include <memory>
 #include <string>
@@ -572,8 +573,16 @@ PyObject* workspace_captured(PyObject*, PyObject* args) {
   return PyBool_FromLong(captured);
 }
 
+#include "host_attention.h"
+
 PyMethodDef host_methods[] = {{"set_workspace", set_workspace, METH_VARARGS, "Mirror a buffer of the workspace pool."},
                               {"workspace_captured", workspace_captured, METH_VARARGS, "Whether a graph capture uses a buffer of the pool."},
+                              {"set_attention_entries", attention::set_entries, METH_VARARGS, "Library entries of the operators between the projections."},
+                              {"set_status_word", attention::set_status_word, METH_VARARGS, "A device's status word."},
+                              {"qk_norm_rope", XQT_FASTCALL(attention::qk_norm_rope), "Norm and rotation, or None."},
+                              {"kv4_append", XQT_FASTCALL(attention::kv4_append), "Write into the 4-bit cache, or None."},
+                              {"kv4_gather", XQT_FASTCALL(attention::kv4_gather), "Read from the 4-bit cache, or None."},
+                              {"kv4_attention", XQT_FASTCALL(attention::kv4_attention), "Attention over the 4-bit cache, or None."},
                               {nullptr, nullptr, 0, nullptr}};
 PyModuleDef host_module = {PyModuleDef_HEAD_INIT, "_host", "Native call path of the bound layers.", -1, host_methods, nullptr, nullptr, nullptr, nullptr};
 

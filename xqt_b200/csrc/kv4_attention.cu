@@ -658,7 +658,7 @@ int run_dim(const AttnArgs& a, int dim, void* workspace, size_t workspace_bytes,
 }  // namespace
 }  // namespace xqt_b200
 
-extern "C" size_t xqt_b200_kv4_attention_workspace_bytes(int dim) {
+extern "C" size_t xqt_b200_kv4_attention_workspace_bytes(int tokens, int batch, int q_heads, int kv_heads, int dim, int has_query_starts) {
   using namespace xqt_b200;
   return (size_t)2 * kMostPerSm * sm_count() * 16 * (dim + 2) * 4;
 }

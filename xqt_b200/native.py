@@ -83,7 +83,7 @@ SIGNATURES: dict[str, tuple] = {
     "xqt_b200_qk_norm_rope": (_I, [_P] * 10 + [_I] * 10 + [ctypes.c_float, _P]),
     "xqt_b200_kv4_append": (_I, [_P] * 6 + [_I] * 3 + [ctypes.c_longlong] + [_I] * 3 + [_P]),
     "xqt_b200_kv4_gather": (_I, [_P] * 5 + [_I] * 3 + [ctypes.c_longlong] + [_I] * 3 + [_P]),
-    "xqt_b200_kv4_attention_workspace_bytes": (_Z, [_I]),
+    "xqt_b200_kv4_attention_workspace_bytes": (_Z, [_I] * 6),
     "xqt_b200_kv4_attention": (_I, [_P] * 8 + [_I] * 5 + [ctypes.c_longlong] + [_I] * 4 + [ctypes.c_float, _P, _Z, _P, _P]),
     "xqt_b200_workspace_status": (_I, [_P, ctypes.POINTER(ctypes.c_uint), _P]),
 }
@@ -134,6 +134,20 @@ def host():
             raise NativeLibraryError(f"cannot load the native call path ({exc}): build it with `python -m xqt_b200.build`") from exc
         _host_module = _host
     return _host_module
+
+
+_attention_host = None
+
+
+def attention_host():
+    """:func:`host` with the library's entries of the operators between the projections made known to it."""
+
+    global _attention_host
+    if _attention_host is None:
+        names = ("xqt_b200_qk_norm_rope", "xqt_b200_kv4_append", "xqt_b200_kv4_gather", "xqt_b200_kv4_attention", "xqt_b200_kv4_attention_workspace_bytes")
+        host().set_attention_entries(*(ctypes.cast(getattr(library(), name), ctypes.c_void_p).value for name in names), check)
+        _attention_host = host()
+    return _attention_host
 
 
 def available() -> bool:
@@ -218,6 +232,7 @@ def status_word(device: torch.device) -> torch.Tensor:
     if word is None:
         word = torch.zeros(64, dtype=torch.int32, device=torch.device("cuda", index))
         _status_words[index] = word
+        host().set_status_word(index, word.data_ptr())
     return word
 
 
@@ -243,5 +258,5 @@ def workspace_status(device: torch.device) -> int:
 
 __all__ = [
     "ACT", "AUTO_INTEGER", "BF16", "DTYPE_CODE", "FP16", "FP32", "LIBRARY_PATH", "SIGNATURES", "VARIANT", "VARIANT_NAMES",
-    "available", "check", "host", "library", "ptr", "status_word", "stream_handle", "version", "workspace", "workspace_status",
+    "attention_host", "available", "check", "host", "library", "ptr", "status_word", "stream_handle", "version", "workspace", "workspace_status",
 ]

@@ -17,6 +17,7 @@ from .rotary import _rows16, _steps
 
 _Strides = ctypes.c_longlong * 4
 HEAD_DIMS = (64, 128, 256)
+_native = None             # the native call path, once a call has been made
 
 
 def allocate_kv4_cache(pages: int, kv_heads: int, head_dim: int, *, page_size: int = 64, dtype: torch.dtype = torch.bfloat16, device=None):
@@ -62,6 +63,9 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, params: to
     channels), into the cache.  ``slots[i]`` = ``page * page_size + row`` of token ``i``, distinct in one call; a slot outside the
     cache (-1 for a padded row) is skipped."""
 
+    global _native
+    if _native is not None and _native.kv4_append(k, v, codes, params, slots):
+        return
     pages, heads, page_size, dim = _cache("kv4_append", codes, params)
     tokens = _slots("kv4_append", slots, codes.device)
     for x in (k, v):
@@ -79,11 +83,17 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, params: to
             k.data_ptr(), v.data_ptr(), codes.data_ptr(), params.data_ptr(), slots.data_ptr(), _Strides(*_steps(k), *_steps(v)), tokens, heads, dim, pages,
             page_size, slots.dtype == torch.int64, native.DTYPE_CODE[params.dtype], native.stream_handle(codes.device))
     native.check(code, "xqt_b200_kv4_append")
+    _native = native.attention_host()
 
 
 def kv4_gather(codes: torch.Tensor, params: torch.Tensor, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """The keys and values that the slots hold, ``[tokens, heads, dim]`` in the type of ``params``; zeros for a slot outside the cache."""
 
+    global _native
+    if _native is not None:
+        done = _native.kv4_gather(codes, params, slots)
+        if done is not None:
+            return done
     pages, heads, page_size, dim = _cache("kv4_gather", codes, params)
     tokens = _slots("kv4_gather", slots, codes.device)
     _on_gpu("kv4_gather", codes)
@@ -95,6 +105,7 @@ def kv4_gather(codes: torch.Tensor, params: torch.Tensor, slots: torch.Tensor) -
                 codes.data_ptr(), params.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), tokens, heads, dim, pages, page_size,
                 slots.dtype == torch.int64, native.DTYPE_CODE[params.dtype], native.stream_handle(codes.device))
         native.check(code, "xqt_b200_kv4_gather")
+        _native = native.attention_host()
     return k, v
 
 
@@ -113,6 +124,11 @@ def kv4_attention(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, bl
     of ``q``.  Rows of ``q`` that belong to no sequence are not written: in a new result they hold anything, in ``out`` (contiguous)
     what they held."""
 
+    global _native
+    if _native is not None:
+        done = _native.kv4_attention(q, codes, params, block_table, seq_lens, query_starts, scale, window, out)
+        if done is not None:
+            return done
     pages, kv_heads, page_size, dim = _cache("kv4_attention", codes, params)
     device = codes.device
     if q.ndim != 3 or q.dtype != params.dtype or q.device != device or q.shape[2] != dim or q.shape[1] < 1 or q.shape[1] % kv_heads:
@@ -144,7 +160,7 @@ def kv4_attention(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, bl
             q = q.clone(memory_format=torch.contiguous_format)
         library = native.library()
         with torch.cuda.device(device):
-            need = library.xqt_b200_kv4_attention_workspace_bytes(dim)
+            need = library.xqt_b200_kv4_attention_workspace_bytes(tokens, batch, q_heads, kv_heads, dim, query_starts is not None)
             workspace = torch.empty(need, dtype=torch.uint8, device=device)      # the allocator's: each captured graph has its own
             code = library.xqt_b200_kv4_attention(
                 q.data_ptr(), codes.data_ptr(), params.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), native.ptr(query_starts), out.data_ptr(),
@@ -152,6 +168,7 @@ def kv4_attention(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, bl
                 0 if window is None else min(int(window), 2 ** 31 - 1), native.DTYPE_CODE[q.dtype], scale, workspace.data_ptr(), need,
                 native.status_word(device).data_ptr(), native.stream_handle(device))
         native.check(code, "xqt_b200_kv4_attention")
+        _native = native.attention_host()
     return out
 
 

@@ -16,6 +16,7 @@ from .. import native
 from ..errors import XQTBackendError
 
 _Strides = ctypes.c_longlong * 10
+_native = None             # the native call path, once a call has been made
 
 
 def rotary_frequencies(rotary_dim: int, *, theta: float = 10000.0, sections=None, ladders=None, device=None):
@@ -89,6 +90,11 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
 
     ``out = (q_out, k_out)``: written instead of new tensors; either may be the input itself (in place), but may not overlap an input otherwise."""
 
+    global _native
+    if _native is not None and out is None:
+        done = _native(q, k, positions, frequencies, axes, q_weight, k_weight, eps, interleaved)
+        if done is not None:
+            return done
     if q.ndim != 3 or q.dtype not in (torch.float16, torch.bfloat16):
         _bad("expects fp16/bf16 queries [tokens, heads, dim]")
     device, dtype = q.device, q.dtype
@@ -148,6 +154,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
                 positions.dtype == torch.int64, bool(interleaved), native.DTYPE_CODE[dtype], native.DTYPE_CODE[weight_dtype or torch.float32], float(eps),
                 native.stream_handle(device))
         native.check(code, "xqt_b200_qk_norm_rope")
+        _native = native.attention_host().qk_norm_rope
     return q_out, k_out
 
 

@@ -461,7 +461,7 @@ int xqt_b200_qk_norm_rope(const void* q, const void* k, void* q_out, void* k_out
  * for c * s + m.  A vector with an infinity or NaN gets s = m = NaN.
  *   codes  uint8 [pages, 2 (key, value), heads, page_size, dim / 2], low nibble = even channel
  *   params T     [pages, 2, heads, page_size, 2] = (s, m)
- * dim 64, 128 or 256.  slots [tokens] (int64 with wide_slots, else int32): page * page_size + row of each token; a slot outside
+ * dim 64, 128 or 256; page_size a power of two, 16 to 4096; tokens * heads < 2^30.  slots [tokens] (int64 with wide_slots, else int32): page * page_size + row of each token; a slot outside
  * the cache is skipped (append) or read as zeros (gather).  The slots of one append are distinct.
  * append: k, v [tokens, heads, dim]; strides (host): token and head stride of k, then of v, in elements, multiples of 8.
  * gather: k_out, v_out [tokens, heads, dim] contiguous. */
@@ -478,7 +478,7 @@ int xqt_b200_kv4_gather(const void* codes, const void* params, const void* slots
  * row i % page_size of page table[b][i / page_size] (table [batch, table_width], int32, row stride strides[2]).  A query sees the keys up
  * to its own position, with window > 0 only the last `window` of them; keys of a page number outside [0, pages) are not seen; a row that
  * sees nothing is 0; lengths and starts are clamped to the table and to `tokens`; rows of no sequence are not written.
- * page_size: a power of two, 16 to 4096.  strides (host): token and head stride of q in elements (multiples of 8), row stride of
+ * strides (host): token and head stride of q in elements (multiples of 8), row stride of
  * table.  Workspace of the given size, 16-byte aligned, any contents, not shared with a call that may overlap. */
 size_t xqt_b200_kv4_attention_workspace_bytes(int tokens, int batch, int q_heads, int kv_heads, int dim,
                                               int has_query_starts);

@@ -7,8 +7,7 @@
 
 #include <type_traits>
 
-#include "common.cuh"
-#include "sm100.cuh"
+#include "pairs.cuh"
 
 namespace xqt_b200 {
 namespace kv4 {
@@ -36,21 +35,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
 }
-// a pair of floats as the packed instructions take it
-struct Two {
-  unsigned long long v;
-  __device__ __forceinline__ Two() {}
-  __device__ __forceinline__ Two(float a, float b) : v(f32x2_pack(a, b)) {}
-  __device__ __forceinline__ explicit Two(float a) : v(f32x2_pack(a, a)) {}
-  __device__ __forceinline__ float2 both() const {
-    float2 f;
-    f32x2_unpack(v, f.x, f.y);
-    return f;
-  }
-};
-__device__ __forceinline__ Two operator*(Two a, Two b) { Two r; r.v = f32x2_mul(a.v, b.v); return r; }
-__device__ __forceinline__ Two operator+(Two a, Two b) { Two r; r.v = f32x2_add(a.v, b.v); return r; }
-__device__ __forceinline__ Two fma2(Two a, Two b, Two c) { Two r; r.v = f32x2_fma(a.v, b.v, c.v); return r; }
 template <typename T>
 __device__ __forceinline__ float2 pair_of(uint32_t bits) {
   const T* e = reinterpret_cast<const T*>(&bits);

@@ -7,14 +7,17 @@
 // The angle is kept as a 64-bit fixed-point fraction of a turn: position * fraction wraps exactly modulo one turn, so a far
 // position loses nothing (fp32 angles are off by 2^-24 of the angle itself: 0.006 rad at position 100,000).
 //
-// Bound by HBM: every channel is read and written once.  A lane group of `dim / 16` (padded to a power of two) lanes holds one
-// head, 16 channels a lane, chosen so that both channels of a pair are in one lane; it computes the cosines of its 8 pairs
-// once and goes through `heads_per_group` heads of its token.
-#include "common.cuh"
+// Bound by HBM: every channel is read and written once.  A block makes the cosines of up to 16 tokens in shared memory, then its lane groups go
+// through the heads of those tokens: dim / 16 lanes (padded to a power of two) hold one head, 16 channels a lane, chosen so that both
+// channels of a pair are in one lane.
+#include "pairs.cuh"
 
 namespace xqt_b200 {
 
 namespace {
+
+using sm100::Two;
+using sm100::fma2;
 
 struct RopeArgs {
   const void* x[2];        // queries, keys
@@ -27,130 +30,170 @@ struct RopeArgs {
   const double* frequencies;   // [rotary / 2], radians per position
   const int* axes;             // [rotary / 2] or null (all 0)
   int axis_count, wide_positions, weight_dtype;
-  int tokens, dim, rotary, heads_per_group, chunks;
+  int tokens, dim, rotary, block_tokens;
   float eps;
 };
 
-template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& v, float* f) {
-  const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = to_float<T>(e[i]);
+// eight channels as packed pairs, and back (one conversion per pair)
+__device__ __forceinline__ Two unpack2(uint32_t v, __half) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+  return Two(f.x, f.y);
+}
+__device__ __forceinline__ Two unpack2(uint32_t v, __nv_bfloat16) { return Two(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
+__device__ __forceinline__ uint32_t pack2(Two v, __half) {
+  const float2 f = v.both();
+  const __half2 h = __floats2half2_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(Two v, __nv_bfloat16) {
+  const float2 f = v.both();
+  const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 template <typename T>
-__device__ __forceinline__ uint4 pack8(const float* f) {
-  uint4 v;
-  T* e = reinterpret_cast<T*>(&v);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = from_float<T>(f[i]);
-  return v;
+__device__ __forceinline__ void unpack8(const uint4& v, Two (&f)[4]) {
+  f[0] = unpack2(v.x, T());
+  f[1] = unpack2(v.y, T());
+  f[2] = unpack2(v.z, T());
+  f[3] = unpack2(v.w, T());
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const Two (&f)[4]) {
+  return make_uint4(pack2(f[0], T()), pack2(f[1], T()), pack2(f[2], T()), pack2(f[3], T()));
+}
+
+constexpr int kThreads = 256, kMostTokens = 16;
+
+// The two runs of 8 channels of lane l.
+template <bool INTERLEAVED>
+__device__ __forceinline__ void runs(const RopeArgs& a, int l, int& c0, int& c1) {
+  if (INTERLEAVED || a.rotary == 0) {
+    c0 = 16 * l;
+    c1 = c0 + 8;
+  } else if (l < a.rotary / 16) {
+    c0 = 8 * l;
+    c1 = c0 + a.rotary / 2;
+  } else {
+    c0 = a.rotary + 8 * (l - a.rotary / 16);
+    c1 = c0 + (a.dim - a.rotary) / 2;
+  }
 }
 
 // LANES: lanes of a head, a power of two; lanes past dim / 16 only take part in the sums.
 template <typename T, int LANES, bool INTERLEAVED>
-__global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
-  const long long group = ((long long)blockIdx.x * 256 + threadIdx.x) / LANES;
-  const int lane = threadIdx.x % LANES;
-  const bool in_grid = group < (long long)a.tokens * a.chunks;
-  const int token = in_grid ? (int)(group / a.chunks) : 0;
-  const int head0 = in_grid ? (int)(group % a.chunks) * a.heads_per_group : 0;
-  const int all_heads = a.heads[0] + a.heads[1];
-  const bool active = in_grid && lane < a.dim / 16;
-  const bool turns = active && lane < a.rotary / 16;
-  // the lane's two runs of 8 channels
-  int c0, c1;
-  if (INTERLEAVED || a.rotary == 0) {
-    c0 = 16 * lane;
-    c1 = c0 + 8;
-  } else if (lane < a.rotary / 16) {
-    c0 = 8 * lane;
-    c1 = c0 + a.rotary / 2;
-  } else {
-    c0 = a.rotary + 8 * (lane - a.rotary / 16);
-    c1 = c0 + (a.dim - a.rotary) / 2;
+__global__ void __launch_bounds__(kThreads, 4) rope_kernel(const RopeArgs a) {
+  // four floats of every lane side by side, so that a quarter warp reads 128 contiguous bytes: pair 8 l + 4 h + i at 4 (l + 16 h) + i, and the
+  // lane's channel e of run r at 4 (l + 16 (2 r + e / 4)) + e % 4
+  __shared__ __align__(16) float s_cos[kMostTokens][128], s_sin[kMostTokens][128], s_weight[2][256];
+  const int pairs = a.rotary / 2, token0 = blockIdx.x * a.block_tokens, block_tokens = min(a.block_tokens, a.tokens - token0);
+  for (int i = threadIdx.x; i < block_tokens * pairs; i += kThreads) {
+    const int token = i / pairs, pair = i - token * pairs, spot = 4 * ((pair >> 3) + 16 * (pair >> 2 & 1)) + (pair & 3);
+    int axis = a.axes ? a.axes[pair] : 0;
+    axis = axis < 0 ? 0 : (axis >= a.axis_count ? a.axis_count - 1 : axis);
+    const long long at = axis * a.p_axis + (token0 + token) * a.p_token;
+    const long long position = a.wide_positions ? reinterpret_cast<const long long*>(a.positions)[at] : (long long)reinterpret_cast<const int*>(a.positions)[at];
+    double turn = a.frequencies[pair] * 0.15915494309189533577;   // 1 / (2 pi)
+    turn -= floor(turn);
+    const unsigned long long fraction = __double2ull_rn(turn * 18446744073709551616.0);
+    const unsigned long long angle = fraction * (unsigned long long)position;
+    sincospif((float)(int)(angle >> 32) * 4.656612873077393e-10f, &s_sin[token][spot], &s_cos[token][spot]);   // 2^-31: half turns
   }
-  float cosine[8], sine[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    cosine[i] = 1.0f;
-    sine[i] = 0.0f;
-    if (turns) {
-      const int pair = 8 * lane + i;
-      int axis = a.axes ? a.axes[pair] : 0;
-      axis = axis < 0 ? 0 : (axis >= a.axis_count ? a.axis_count - 1 : axis);
-      const long long at = axis * a.p_axis + token * a.p_token;
-      const long long position = a.wide_positions ? reinterpret_cast<const long long*>(a.positions)[at] : (long long)reinterpret_cast<const int*>(a.positions)[at];
-      double turn = a.frequencies[pair] * 0.15915494309189533577;   // 1 / (2 pi)
-      turn -= floor(turn);
-      const unsigned long long fraction = __double2ull_rn(turn * 18446744073709551616.0);
-      const unsigned long long angle = fraction * (unsigned long long)position;
-      sincospif((float)(int)(angle >> 32) * 4.656612873077393e-10f, &sine[i], &cosine[i]);   // 2^-31: half turns
+  const bool normed = a.weight[0] != nullptr || a.weight[1] != nullptr;     // uniform: then every lane of a warp takes part in the sums
+  if (normed) {
+    for (int i = threadIdx.x; i < 2 * a.dim; i += kThreads) {
+      const int which = i >= a.dim, at = which ? i - a.dim : i, owner = at >> 4, run = at >> 3 & 1, e = at & 7;
+      const void* weight = which ? a.weight[1] : a.weight[0];
+      int c0, c1;
+      runs<INTERLEAVED>(a, owner, c0, c1);
+      s_weight[which][4 * (owner + 16 * (2 * run + (e >> 2))) + (e & 3)] = weight != nullptr ? load_param(weight, a.weight_dtype, (run ? c1 : c0) + e) : 1.0f;
     }
   }
+  __syncthreads();
+
+  constexpr int kGroups = kThreads / LANES, kBatch = 2;      // heads of a group loaded before the first is worked on
+  const int lane = threadIdx.x % LANES, all = a.heads[0] + a.heads[1];
+  const bool active = lane < a.dim / 16, turns = lane < a.rotary / 16;
+  int c0, c1;
+  runs<INTERLEAVED>(a, lane, c0, c1);
   const float inv_dim = 1.0f / (float)a.dim;
-  constexpr int kBatch = 2;      // heads loaded before the first is worked on
-  for (int first = 0; first < a.heads_per_group; first += kBatch) {
+  int token = 0, head = threadIdx.x / LANES;
+  for (int item = 0; item < block_tokens * all; item += kBatch * kGroups) {
     uint4 raw[kBatch][2];
+    T* dst[kBatch];
+    int of[kBatch], which[kBatch];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      const int head = head0 + first + b;
+      while (head >= all) {
+        head -= all;
+        ++token;
+      }
+      of[b] = token;
+      which[b] = head >= a.heads[0];
       raw[b][0] = raw[b][1] = make_uint4(0, 0, 0, 0);
-      if (active && first + b < a.heads_per_group && head < all_heads) {
-        const int which = head < a.heads[0] ? 0 : 1;
-        const T* src = which ? reinterpret_cast<const T*>(a.x[1]) + token * a.x_token[1] + (head - a.heads[0]) * a.x_head[1]
-                             : reinterpret_cast<const T*>(a.x[0]) + token * a.x_token[0] + head * a.x_head[0];
+      dst[b] = nullptr;
+      if (active && token < block_tokens) {
+        const long long row = token0 + token, h = which[b] ? head - a.heads[0] : head;
+        const T* src = which[b] ? reinterpret_cast<const T*>(a.x[1]) + row * a.x_token[1] + h * a.x_head[1]
+                                : reinterpret_cast<const T*>(a.x[0]) + row * a.x_token[0] + h * a.x_head[0];
+        dst[b] = which[b] ? reinterpret_cast<T*>(a.out[1]) + row * a.o_token[1] + h * a.o_head[1]
+                          : reinterpret_cast<T*>(a.out[0]) + row * a.o_token[0] + h * a.o_head[0];
         raw[b][0] = *reinterpret_cast<const uint4*>(src + c0);
         raw[b][1] = *reinterpret_cast<const uint4*>(src + c1);
       }
+      head += kGroups;
     }
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      const int head = head0 + first + b;
-      const bool mine = first + b < a.heads_per_group && head < all_heads;
-      const int which = head < a.heads[0] ? 0 : 1;
-      float u[8], v[8];
+      Two u[4], v[4];
       unpack8<T>(raw[b][0], u);
       unpack8<T>(raw[b][1], v);
-      const void* weight = which ? a.weight[1] : a.weight[0];
-      if (a.weight[0] != nullptr || a.weight[1] != nullptr) {   // uniform: every lane of the warp takes part in the sums
-        float sum = 0.0f;
+      if (normed) {
+        Two squares(0.0f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum = fmaf(u[i], u[i], fmaf(v[i], v[i], sum));
+        for (int i = 0; i < 4; ++i) squares = fma2(u[i], u[i], fma2(v[i], v[i], squares));
+        float sum = squares.both().x + squares.both().y;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (active && mine && weight != nullptr) {
-          const float r = rsqrtf(sum * inv_dim + a.eps);
+        if (dst[b] != nullptr && (which[b] ? a.weight[1] : a.weight[0]) != nullptr) {
+          const Two r(rsqrtf(sum * inv_dim + a.eps));
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            u[i] = u[i] * r * load_param(weight, a.weight_dtype, c0 + i);
-            v[i] = v[i] * r * load_param(weight, a.weight_dtype, c1 + i);
+          for (int h = 0; h < 2; ++h) {
+            const float4 w0 = *reinterpret_cast<const float4*>(&s_weight[which[b]][4 * (lane + 16 * h)]), w1 = *reinterpret_cast<const float4*>(&s_weight[which[b]][4 * (lane + 16 * (2 + h))]);
+            u[2 * h] = u[2 * h] * (r * Two(w0.x, w0.y));
+            u[2 * h + 1] = u[2 * h + 1] * (r * Two(w0.z, w0.w));
+            v[2 * h] = v[2 * h] * (r * Two(w1.x, w1.y));
+            v[2 * h + 1] = v[2 * h + 1] * (r * Two(w1.z, w1.w));
           }
         }
       }
-      if (active && mine) {
+      if (dst[b] != nullptr) {
         if (turns) {
-          if (INTERLEAVED) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float x0 = u[2 * i], x1 = u[2 * i + 1], z0 = v[2 * i], z1 = v[2 * i + 1];
-              u[2 * i] = fmaf(x0, cosine[i], -(x1 * sine[i]));
-              u[2 * i + 1] = fmaf(x0, sine[i], x1 * cosine[i]);
-              v[2 * i] = fmaf(z0, cosine[4 + i], -(z1 * sine[4 + i]));
-              v[2 * i + 1] = fmaf(z0, sine[4 + i], z1 * cosine[4 + i]);
-            }
-          } else {
+          for (int h = 0; h < 2; ++h) {      // pairs 8 lane + 4 h .. + 3
+            const float4 c = *reinterpret_cast<const float4*>(&s_cos[of[b]][4 * (lane + 16 * h)]), s = *reinterpret_cast<const float4*>(&s_sin[of[b]][4 * (lane + 16 * h)]);
+            if (INTERLEAVED) {
+              auto turn = [](Two x, float cs, float sn) {
+                const float2 f = x.both();
+                return fma2(Two(f.x), Two(cs, sn), Two(f.y) * Two(-sn, cs));
+              };
+              Two* const x = h ? v : u;
+              x[0] = turn(x[0], c.x, s.x);
+              x[1] = turn(x[1], c.y, s.y);
+              x[2] = turn(x[2], c.z, s.z);
+              x[3] = turn(x[3], c.w, s.w);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float x0 = u[i], x1 = v[i];
-              u[i] = fmaf(x0, cosine[i], -(x1 * sine[i]));
-              v[i] = fmaf(x0, sine[i], x1 * cosine[i]);
+              for (int i = 0; i < 2; ++i) {
+                const Two cs = i ? Two(c.z, c.w) : Two(c.x, c.y), sn = i ? Two(s.z, s.w) : Two(s.x, s.y), neg = i ? Two(-s.z, -s.w) : Two(-s.x, -s.y);
+                const Two x0 = u[2 * h + i], x1 = v[2 * h + i];
+                u[2 * h + i] = fma2(x0, cs, x1 * neg);
+                v[2 * h + i] = fma2(x0, sn, x1 * cs);
+              }
             }
           }
         }
-        T* dst = which ? reinterpret_cast<T*>(a.out[1]) + token * a.o_token[1] + (head - a.heads[0]) * a.o_head[1]
-                       : reinterpret_cast<T*>(a.out[0]) + token * a.o_token[0] + head * a.o_head[0];
-        *reinterpret_cast<uint4*>(dst + c0) = pack8<T>(u);
-        *reinterpret_cast<uint4*>(dst + c1) = pack8<T>(v);
+        *reinterpret_cast<uint4*>(dst[b] + c0) = pack8<T>(u);
+        *reinterpret_cast<uint4*>(dst[b] + c1) = pack8<T>(v);
       }
     }
   }
@@ -158,12 +201,11 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
 
 template <typename T, int LANES>
 int launch(const RopeArgs& a, bool interleaved, cudaStream_t stream) {
-  const long long threads = (long long)a.tokens * a.chunks * LANES;
-  const unsigned grid = (unsigned)((threads + 255) / 256);
+  const unsigned grid = (unsigned)ceil_div(a.tokens, a.block_tokens);
   if (interleaved)
-    rope_kernel<T, LANES, true><<<grid, 256, 0, stream>>>(a);
+    rope_kernel<T, LANES, true><<<grid, kThreads, 0, stream>>>(a);
   else
-    rope_kernel<T, LANES, false><<<grid, 256, 0, stream>>>(a);
+    rope_kernel<T, LANES, false><<<grid, kThreads, 0, stream>>>(a);
   return launch_status();
 }
 
@@ -218,13 +260,9 @@ extern "C" int xqt_b200_qk_norm_rope(const void* q, const void* k, void* q_out, 
   a.dim = dim;
   a.rotary = rotary;
   a.eps = eps;
-  // Heads per lane group: more heads share the cosines, fewer fill the SMs when there are few tokens.  Halved until the
-  // groups fill about two blocks of every SM.
-  const int all = q_heads + k_heads, lanes = dim <= 64 ? 4 : dim <= 128 ? 8 : 16;
-  int per = 8;
-  while (per > 1 && (long long)tokens * ceil_div(all, per) * lanes < 2LL * 256 * sm_count()) per >>= 1;
-  a.heads_per_group = per;
-  a.chunks = ceil_div(all, per);
-  XQT_REQUIRE((long long)tokens * a.chunks * lanes / 256 < (1LL << 31) - 1);
+  // Tokens of a block: their cosines are made together, so more of them fill its threads; fewer fill the SMs.  Halved until there are two
+  // blocks for each SM.
+  a.block_tokens = kMostTokens;
+  while (a.block_tokens > 1 && ceil_div(tokens, a.block_tokens) < 2 * sm_count()) a.block_tokens >>= 1;
   return dtype == XQT_B200_BF16 ? launch_lanes<__nv_bfloat16>(a, interleaved != 0, stream) : launch_lanes<__half>(a, interleaved != 0, stream);
 }

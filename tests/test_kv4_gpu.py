@@ -326,11 +326,18 @@ def test_two_streams_and_two_captured_graphs():
     assert all(torch.equal(a, kv4_attention(q, codes, params, table, seq_lens)) for a, q in zip(held, qs))
 
 
+def wide(table, page):
+    """The table with room for a million keys: then a call counts as much work, and sequences with more than 32 rows go to the prompt kernel."""
+
+    return torch.nn.functional.pad(table, (0, (1 << 20) // page), value=-1)
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("heads,each,dim,page", [(2, 4, 128, 64), (1, 8, 64, 16), (2, 2, 256, 128), (1, 3, 128, 32), (4, 1, 64, 256), (1, 5, 256, 16)])
 @pytest.mark.parametrize("lens,counts,window", [([300], [300], None), ([129, 700, 1000, 5], [129, 257, 300, 5], None), ([513, 1300], [512, 301], 200), ([900], [899], 1)])
 def test_prompts(dtype, heads, each, dim, page, lens, counts, window):
     codes, params, table = make_cache(lens, heads, dim, page, dtype, 50)
+    table = wide(table, page)
     check(_vectors(sum(counts), heads * each, dim, dtype, 51), codes, params, table, lens, counts, window=window)
 
 
@@ -338,12 +345,14 @@ def test_prompts(dtype, heads, each, dim, page, lens, counts, window):
 def test_prompts_of_many_sequences_beside_single_tokens(dim):
     lens, counts = [40, 700, 33, 1, 512, 90, 0, 2000] * 3, [40, 1, 9, 1, 512, 33, 3, 700] * 3
     codes, params, table = make_cache(lens, 2, dim, 32, torch.bfloat16, 52)
+    table = wide(table, 32)
     check(_vectors(sum(counts), 16, dim, torch.bfloat16, 53), codes, params, table, lens, counts)
 
 
 def test_prompt_with_more_queries_than_keys_and_other_scales():
     lens, counts = [100, 0, 300], [400, 300, 300]
     codes, params, table = make_cache(lens, 1, 128, 16, torch.bfloat16, 54)
+    table = wide(table, 16)
     for scale in (0.5, -0.125, 0.0):
         got = check(_vectors(1000, 4, 128, torch.bfloat16, 55), codes, params, table, lens, counts, scale=scale)
         assert bool((got[:300] == 0).all()) and bool((got[400:700] == 0).all()) and bool((got[300:400] != 0).any())
@@ -352,6 +361,7 @@ def test_prompt_with_more_queries_than_keys_and_other_scales():
 def test_prompt_over_pages_that_are_not_there():
     lens, counts = [600, 400], [300, 400]
     codes, params, table = make_cache(lens, 2, 64, 16, torch.float16, 56)
+    table = wide(table, 16)
     table[0, 0], table[0, 7], table[0, 36], table[1, 3:8], table[1, 24] = -1, codes.shape[0], 2 ** 31 - 1, -1, -2 ** 31
     check(_vectors(700, 8, 64, torch.float16, 57), codes, params, table, lens, counts)
     table[1] = -1
@@ -363,6 +373,7 @@ def test_prompt_over_pages_that_are_not_there():
 def test_prompt_with_large_and_unequal_values(dim):
     lens, counts = [700], [700]
     codes, params, table = make_cache(lens, 1, dim, 64, torch.bfloat16, 58, size=4.0)
+    table = wide(table, 64)
     position = torch.empty(codes.shape[0], 64, dtype=torch.long)
     for i, p in enumerate(table[0, :11].tolist()):
         position[p] = torch.arange(64) + 64 * i
@@ -381,6 +392,7 @@ def test_prompt_rows_do_not_meet_what_they_do_not_see():
 
     lens, counts = [500], [400]
     codes, params, table = make_cache(lens, 2, 128, 64, torch.bfloat16, 60)
+    table = wide(table, 64)
     q = _vectors(400, 8, 128, torch.bfloat16, 61).to(DEVICE)
     q[7, 3, 5] = INF
     clean = params.clone()
@@ -402,6 +414,7 @@ def test_prompt_in_place_of_rows_and_graph():
 
     lens, counts = [400, 350], [300, 260]
     codes, params, table = make_cache(lens, 2, 128, 32, torch.float16, 62)
+    table = wide(table, 32)
     fused = _vectors(600, 12, 128, torch.float16, 63).to(DEVICE)
     q = fused[:, :8]
     seq_lens, starts = torch.tensor(lens, dtype=torch.int32, device=DEVICE), torch.tensor([10, 310, 570], dtype=torch.int32, device=DEVICE)
@@ -418,6 +431,26 @@ def test_prompt_in_place_of_rows_and_graph():
     graph.replay()
     want = kv4_attention(q, codes, params, table, seq_lens, query_starts=starts)
     assert torch.equal(held[:345], want[:345]) and native.workspace_status(DEVICE) == 0
+
+
+@pytest.mark.parametrize("lens,counts", [([3000], [70]), ([700, 2000, 64], [65, 300, 9]), ([100] * 40, [60] * 40)])
+def test_prompt_kernel_beside_the_other_one(lens, counts):
+    """The same call by either kernel (the width of the table chooses): both within their bounds; items that several CTAs share among them."""
+
+    codes, params, table = make_cache(lens, 2, 128, 64, torch.bfloat16, 64)
+    q = _vectors(sum(counts), 8, 128, torch.bfloat16, 65)
+    for t in (table, wide(table, 64)):
+        check(q, codes, params, t, lens, counts)
+
+
+def test_same_prompt_bits_every_time():
+    lens, counts = [1500, 900, 300], [700, 900, 20]
+    codes, params, table = make_cache(lens, 2, 128, 64, torch.bfloat16, 66)
+    q = _vectors(sum(counts), 8, 128, torch.bfloat16, 67).to(DEVICE)
+    seq_lens, starts = torch.tensor(lens, dtype=torch.int32, device=DEVICE), torch.tensor([0, 700, 1600, 1620], dtype=torch.int32, device=DEVICE)
+    first = kv4_attention(q, codes, params, wide(table, 64), seq_lens, query_starts=starts)
+    for _ in range(10):
+        assert torch.equal(kv4_attention(q, codes, params, wide(table, 64), seq_lens, query_starts=starts), first)
 
 
 def test_many_short_sequences():

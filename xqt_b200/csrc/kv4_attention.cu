@@ -589,7 +589,7 @@ __global__ void __launch_bounds__(128) kv4_attention_join_kernel(const AttnArgs 
     const float* src = a.part_o + ((long long)slot * ROWS + row) * D + lane * PER;
 #pragma unroll
     for (int e = 0; e < PER; e += 2) *reinterpret_cast<float2*>(v + e) = *reinterpret_cast<const float2*>(src + e);
-    if (s.x == -CUDART_INF_F) continue;
+    if (s.y == 0.0f) continue;                 // it saw nothing (a NaN has no maximum, but a weight)
     const float top = fmaxf(m, s.x);
     const float keep = m == top ? 1.0f : exp2_fast(m - top), by = exp2_fast(s.x - top);
     m = top;
@@ -618,6 +618,7 @@ __global__ void __launch_bounds__(128) kv4_attention_join_kernel(const AttnArgs 
   }
 }
 
+constexpr int kFewRows = 32;      // rows for a key head up to which a sequence stays with this file's kernel
 constexpr int kMostPerSm = 2;      // CTAs of any shape on an SM
 
 // Two CTAs of four warps on an SM, with all the registers that leaves.  Keys per chunk: 64 for one 8-row tile of up to 128 channels (two
@@ -660,7 +661,12 @@ int run_dim(const AttnArgs& a, int dim, void* workspace, size_t workspace_bytes,
 
 extern "C" size_t xqt_b200_kv4_attention_workspace_bytes(int tokens, int batch, int q_heads, int kv_heads, int dim, int has_query_starts) {
   using namespace xqt_b200;
-  return (size_t)2 * kMostPerSm * sm_count() * 16 * (dim + 2) * 4;
+  (void)batch;
+  const size_t few = (size_t)2 * kMostPerSm * sm_count() * 16 * (dim + 2) * 4;
+  // the two kernels run one after the other and share it
+  if (!has_query_starts || kv_heads < 1 || (long long)tokens * (q_heads / kv_heads) <= kFewRows) return few;
+  const size_t prompt = kv4_prompt_workspace_bytes(dim);
+  return few > prompt ? few : prompt;
 }
 
 extern "C" int xqt_b200_kv4_attention(const void* q, const void* codes, const void* params, const int* table, const int* seq_lens, const int* query_starts,
@@ -703,14 +709,15 @@ extern "C" int xqt_b200_kv4_attention(const void* q, const void* codes, const vo
   a.scale = scale * 1.4426950408889634f;
   // Which sequences go to the prompt kernel.  Its tiles of 128 rows run near the tensor core's rate where they are full and fill the SMs, and one
   // of its CTAs takes a sequence's keys alone; this file's kernel spreads any sequence over all SMs.
+  // Sequences with more rows go to the prompt kernel, unless the whole call is so little work that its two launches more are not worth it (keys: as
+  // many as the table holds).  Both sides measured, this kernel for all | prompt kernel above 32 rows: one sequence, 40 queries of 32 heads on 2000
+  // keys 25 | 33 us, 64 queries 31 | 36, 16 queries on 30,000 keys 62 | 66; 64 sequences of 16 queries on 2000 keys 332 | 275, of 9 queries 249 | 273.
   a.few_rows = INT_MAX;
-  if (query_starts != nullptr) {
-    const int most = (long long)tokens * q_heads >= 128LL * sm_count() ? 32 : 256;
-    if ((long long)tokens * a.each > most) {
-      a.few_rows = most;
-      const int rc = kv4_prompt_launch(a, dim, dtype, stream);
-      if (rc) return rc;
-    }
+  if (query_starts != nullptr && (long long)tokens * a.each > kFewRows &&
+      (double)tokens * q_heads * table_width * page_size * dim > 768e6) {
+    a.few_rows = kFewRows;
+    const int rc = kv4_prompt_launch(a, dim, dtype, workspace, workspace_bytes, stream);
+    if (rc) return rc;
   }
   return dtype == XQT_B200_BF16 ? run_dim<__nv_bfloat16>(a, dim, workspace, workspace_bytes, stream)
                                 : run_dim<__half>(a, dim, workspace, workspace_bytes, stream);

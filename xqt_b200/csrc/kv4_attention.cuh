@@ -24,6 +24,7 @@ struct AttnArgs {
   void* out;
   float* part_o;             // [2 * CTAs][ROWS][D]
   float2* part_ml;           // [2 * CTAs][ROWS]
+  int4* plan;                // prompt kernel: where each CTA begins
   unsigned* status;
   long long q_token, q_head, pages, table_stride;
   int tokens, batch, q_heads, kv_heads, each, page_size, page_shift, table_width, window, few_rows;     // few_rows: sequences with more rows for a key head go to the prompt kernel
@@ -150,6 +151,7 @@ __device__ __forceinline__ bool place(const AttnArgs& a, int lane, const Sequenc
 
 }  // namespace kv4
 
-int kv4_prompt_launch(const kv4::AttnArgs& a, int dim, int dtype, cudaStream_t stream);
+int kv4_prompt_launch(const kv4::AttnArgs& a, int dim, int dtype, void* workspace, size_t bytes, cudaStream_t stream);
+size_t kv4_prompt_workspace_bytes(int dim);
 
 }  // namespace xqt_b200

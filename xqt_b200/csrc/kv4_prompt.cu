@@ -1,14 +1,14 @@
 // Attention of many queries (prompts, chunks of prompts) over the paged 4-bit cache (layout: kv4_cache.cu; the mathematics and the rules
 // for what a query sees: kv4_attention.cu), on the tensor cores.
 //
-// A CTA takes TILES row tiles of 128 (row = query * heads of the key head + head) of one sequence and key head through the keys they see, BN at
-// a time.  Codes come in by bulk copies; four warps turn them into fp16 keys and values in shared memory (128-byte swizzle), once for all rows;
+// An item is TILES row tiles of 128 (row = query * heads of the key head + head) of one sequence and key head, and the keys they see, BN at
+// a time; the chunks of all items form one list, dealt out evenly to one CTA per SM, and items that CTAs share are joined by a second kernel.  Codes come in by bulk copies; four warps turn them into fp16 keys and values in shared memory (128-byte swizzle), once for all rows;
 // one thread issues S = Q K^T and O += P V (tcgen05, sums in tensor memory); four warps per row tile, a thread per row, do the softmax: P goes
 // back to tensor memory over the scores that it came from.  Scores are double-buffered: those of the next chunk are made while the softmax
 // works on this one's.
 //
 //   warp 0       table look-ups and bulk copies
-//   warp 2       allocates tensor memory
+//   warp 2       allocates tensor memory, prefetches queries
 //   warps 1, 3   tcgen05.mma, one issuer per row tile: an answer of a barrier takes about 200 clocks, and one thread waiting for both tiles in
 //                turn set the pace (8192-token prompt: 605 us with all other work left out)
 //   warps 4-7    codes -> fp16
@@ -39,14 +39,15 @@ template <int D_, int TILES_, int STAGES_>
 struct PromptShape {
   static constexpr int D = D_, TILES = TILES_, STAGES = STAGES_, BN = 64;     // STAGES: of codes, keys and values
   static constexpr int GROUP_WARPS = 4 / STAGES;               // that convert one chunk
-  static constexpr int ROWS = 128 * TILES, UNIT = 1 << 20, CT = BN, OPENING = 1;
+  static constexpr int ROWS = 128 * TILES, UNIT = BN, CT = BN;
+  static constexpr int OPENING = 7;                            // what an item costs besides its chunks, in chunks
   static constexpr bool PROMPT = true;
   static constexpr int THREADS = 256 + 128 * TILES;
   static constexpr int BLOCKS = D / 64;                        // 128-byte wide column blocks of an operand
   static constexpr int Q_BYTES = ROWS * D * 2, KV_BYTES = BN * D * 2;
   static constexpr int CODE_BYTES = BN * D / 2, PARAM_BYTES = BN * 4, RAW_BYTES = 2 * (CODE_BYTES + PARAM_BYTES);
   static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + STAGES * KV_BYTES, OFF_RAW = OFF_V + STAGES * KV_BYTES, OFF_MISC = OFF_RAW + STAGES * RAW_BYTES;
-  static constexpr int SMEM = OFF_MISC + 640;
+  static constexpr int SMEM = OFF_MISC + 768;
   // tensor memory: two buffers of scores per tile from column 0, P over the first half of its scores; O from 256
   static constexpr uint32_t O_COL = 256;
   static_assert(2 * TILES * BN <= 256 && TILES * D <= 256 && SMEM <= 227 * 1024 && (STAGES == 2 || STAGES == 4), "tensor and shared memory");
@@ -54,7 +55,7 @@ struct PromptShape {
 
 // Barriers, in 8-byte words behind the tiles.  Those of scores, P and O are per tile and chunk parity: a softmax warp may be a chunk ahead of its
 // neighbours, and a wait may come two products late.
-enum : int { kRawFull = 0, kRawEmpty = 4, kKReady = 8, kVReady = 12, kKEmpty = 16, kVEmpty = 20, kSFull = 24, kPReady = 28, kODone = 32, kGrown = 36, kQReady = 40, kBarriers = 41 };
+enum : int { kRawFull = 0, kRawEmpty = 4, kKReady = 8, kVReady = 12, kKEmpty = 16, kVEmpty = 20, kSFull = 24, kPReady = 28, kODone = 32, kGrown = 36, kQReady = 40, kBarriers = 42 };
 constexpr int kRing = 16;          // chunks that loader, conversion and softmax may lie apart: more than 2 + 2 * STAGES
 
 template <int N>
@@ -106,6 +107,202 @@ __device__ __forceinline__ uint4 eight(uint32_t x, __half2 s, __half2 m) {
   return r;
 }
 
+// Both functions below are not inlined: their registers would crowd those of the softmax loop, and they run once per item.
+//
+// The 32 query rows of a warp, each lane its own (or null), to shared memory: scaled by a power of two per row, fp16, channels in the order of
+// the codes, 128-byte swizzle.  Returns what the lane's scores have to be multiplied by.
+template <typename T, int D>
+__device__ __noinline__ float load_queries(const T* src, uint8_t* dst, float scale) {
+  const int lane = threadIdx.x & 31;
+  float factor = 0.0f;
+  // D / 8 lanes read a row together (a row per lane would touch 32 lines with every load): its largest, then scaled and stored
+  constexpr int LPR = D / 8, RPR = 32 / LPR, BATCH = LPR < 8 ? LPR : 8;
+  const float sign = scale == 0.0f ? 0.0f : copysignf(1.0f, scale), size = scale == 0.0f ? 1.0f : fabsf(scale);
+  const int c = lane % LPR;
+#pragma unroll 1
+  for (int first = 0; first < LPR; first += BATCH) {
+    uint4 x[BATCH];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const T* const from_row = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), (first + k) * RPR + lane / LPR));
+      x[k] = from_row != nullptr ? *reinterpret_cast<const uint4*>(from_row + 8 * c) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const T* const v = reinterpret_cast<const T*>(&x[k]);
+      // magnitudes order as their bits
+      uint32_t most = __vmaxu2(__vmaxu2(x[k].x & 0x7fff7fffu, x[k].y & 0x7fff7fffu), __vmaxu2(x[k].z & 0x7fff7fffu, x[k].w & 0x7fff7fffu));
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, o));
+      const float2 most2 = pair_of<T>(most);
+      const float top = fmaxf(most2.x, most2.y);
+      const int e = top > 0.0f && top <= 3.402823466e38f ? min(max(above(top) - 1, -100), 100) : 0;
+      const float down = pow2(-e) * sign, of_owner = __shfl_sync(0xffffffffu, pow2(e) * size, lane % RPR * LPR);
+      if (lane / RPR == first + k) factor = of_owner;
+      uint4 y;
+      y.x = half2_bits(__floats2half2_rn(to_float<T>(v[0]) * down, to_float<T>(v[4]) * down));
+      y.y = half2_bits(__floats2half2_rn(to_float<T>(v[1]) * down, to_float<T>(v[5]) * down));
+      y.z = half2_bits(__floats2half2_rn(to_float<T>(v[2]) * down, to_float<T>(v[6]) * down));
+      y.w = half2_bits(__floats2half2_rn(to_float<T>(v[3]) * down, to_float<T>(v[7]) * down));
+      const int at = (first + k) * RPR + lane / LPR;
+      *reinterpret_cast<uint4*>(dst + (c >> 3) * (128 * 128) + at * 128 + (((c & 7) ^ (at & 7)) << 4)) = y;
+    }
+  }
+  return factor;
+}
+
+// The 32 rows of a warp from tensor memory, times `by`, to their addresses (or null): as T, or as fp32 parts.
+template <typename T, int D>
+__device__ __noinline__ void store_rows(uint32_t o_at, unsigned long long mine, float by, bool whole) {
+  const int lane = threadIdx.x & 31;
+  // Four lanes write 64 bytes of a row together (a lane alone would touch a line of its own with every store): they exchange 16-byte pieces,
+  // piece i of row k for piece k of row i.
+  unsigned long long rows_at[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) rows_at[k] = __shfl_sync(0xffffffffu, mine, (lane & 28) + k);
+  auto exchange_and_store = [&](uint4 (&x)[4], int offset) {
+    auto swap = [](uint4& keep_low, uint4& keep_high, bool upper, int o) {
+      uint4 give = upper ? keep_low : keep_high;
+      give.x = __shfl_xor_sync(0xffffffffu, give.x, o);
+      give.y = __shfl_xor_sync(0xffffffffu, give.y, o);
+      give.z = __shfl_xor_sync(0xffffffffu, give.z, o);
+      give.w = __shfl_xor_sync(0xffffffffu, give.w, o);
+      if (upper) keep_low = give;
+      else keep_high = give;
+    };
+    swap(x[0], x[1], lane & 1, 1);
+    swap(x[2], x[3], lane & 1, 1);
+    swap(x[0], x[2], lane & 2, 2);
+    swap(x[1], x[3], lane & 2, 2);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (rows_at[k] != 0) *reinterpret_cast<uint4*>(rows_at[k] + offset + 16 * (lane & 3)) = x[k];
+  };
+#pragma unroll 1
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t r[32];
+    tmem_ld_32x32(o_at + 32 * c, r);
+    wait_ld_dep32(r);
+    auto value = [&](int e) { return __uint_as_float(r[(e & ~7) + ((e & 7) < 4 ? 2 * (e & 7) : 2 * (e & 7) - 7)]) * by; };      // channel e of these 32
+    uint4 x[4];
+    if (whole) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        T* const t = reinterpret_cast<T*>(&x[b]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = from_float<T>(value(8 * b + e));
+      }
+      exchange_and_store(x, 64 * c);
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          x[b] = make_uint4(__float_as_uint(value(16 * h + 4 * b)), __float_as_uint(value(16 * h + 4 * b + 1)), __float_as_uint(value(16 * h + 4 * b + 2)),
+                            __float_as_uint(value(16 * h + 4 * b + 3)));
+        exchange_and_store(x, 128 * c + 64 * h);
+      }
+    }
+  }
+}
+
+// An item of the list and a unit of it: SH::OPENING units stand for its queries and its result, the others are its chunks.
+struct PromptItem {
+  int b, tile, head, unit, begin, chunks;
+  Sequence s;
+};
+
+// the keys that some row of a tile sees start in chunk begin / BN; how many chunks
+template <typename SH>
+__device__ __forceinline__ int prompt_chunks(const AttnArgs& a, const Sequence& s, int tile, int& begin) {
+  const int pos0 = s.len - s.nq;                                       // the position of the sequence's first query
+  const int j0 = tile * SH::ROWS / a.each, j1 = min(s.nq - 1, (tile * SH::ROWS + SH::ROWS - 1) / a.each);
+  const int end = pos0 + j1 + 1;
+  begin = a.window ? (int)max((long long)pos0 + j0 - a.window + 1, 0LL) / SH::BN * SH::BN : 0;
+  return end > begin ? (end - begin + SH::BN - 1) / SH::BN : 0;
+}
+
+__device__ __forceinline__ Sequence sequence_of(const Sequence& s, int lane) {
+  Sequence r;
+  r.q0 = __shfl_sync(0xffffffffu, s.q0, lane);
+  r.nq = __shfl_sync(0xffffffffu, s.nq, lane);
+  r.len = __shfl_sync(0xffffffffu, s.len, lane);
+  r.first = __shfl_sync(0xffffffffu, s.first, lane);
+  r.tiles = __shfl_sync(0xffffffffu, s.tiles, lane);
+  r.units = __shfl_sync(0xffffffffu, s.units, lane);
+  return r;
+}
+
+// Goes through the tiles of all sequences, 32 at a time, and calls visit(b, sequence, first tile, this lane's units) until it says to stop;
+// one warp.
+template <typename SH, typename V>
+__device__ __forceinline__ void prompt_tiles(const AttnArgs& a, int lane, V visit) {
+  for (int b0 = 0; b0 < a.batch; b0 += 32) {
+    Sequence mine = {};
+    if (b0 + lane < a.batch) mine = sequence<SH>(a, b0 + lane);
+    for (unsigned some = __ballot_sync(0xffffffffu, mine.tiles > 0); some; some &= some - 1) {
+      const int at = __ffs(some) - 1;
+      const Sequence s = sequence_of(mine, at);
+      for (int t0 = 0; t0 < s.tiles; t0 += 32) {
+        int begin;
+        const unsigned units = t0 + lane < s.tiles ? (unsigned)a.kv_heads * (prompt_chunks<SH>(a, s, t0 + lane, begin) + SH::OPENING) : 0u;
+        if (!visit(b0 + at, s, t0, units)) return;
+      }
+    }
+  }
+}
+
+template <typename SH>
+__device__ __forceinline__ Deal prompt_deal(const AttnArgs& a, int lane, unsigned ctas) {
+  Deal d = {};
+  unsigned sum = 0;
+  prompt_tiles<SH>(a, lane, [&](int, const Sequence&, int, unsigned units) {
+    sum += units;
+    return true;
+  });
+  d.total = __reduce_add_sync(0xffffffffu, sum);
+  d.each = d.total / ctas;
+  d.more = d.total - d.each * ctas;
+  return d;
+}
+
+template <typename SH>
+__device__ __forceinline__ void prompt_place(const AttnArgs& a, int lane, unsigned u, PromptItem& w) {
+  unsigned base = 0;
+  prompt_tiles<SH>(a, lane, [&](int b, const Sequence& s, int t0, unsigned units) {
+    const unsigned cum = scan32(units, lane), over = __ballot_sync(0xffffffffu, base + cum > u);
+    if (over) {
+      const int at = __ffs(over) - 1;
+      const unsigned rest = u - base - __shfl_sync(0xffffffffu, cum - units, at);
+      w.b = b;
+      w.s = s;
+      w.tile = t0 + at;
+      w.chunks = prompt_chunks<SH>(a, s, w.tile, w.begin);
+      w.head = (int)(rest / (unsigned)(w.chunks + SH::OPENING));
+      w.unit = (int)(rest - (unsigned)w.head * (w.chunks + SH::OPENING));
+      return false;
+    }
+    base += __shfl_sync(0xffffffffu, cum, 31);
+    return true;
+  });
+}
+
+// the item behind w
+template <typename SH>
+__device__ __forceinline__ void prompt_next(const AttnArgs& a, PromptItem& w) {
+  w.unit = 0;
+  if (++w.head < a.kv_heads) return;
+  w.head = 0;
+  if (++w.tile >= w.s.tiles) {
+    w.tile = 0;
+    while (++w.b < a.batch) {
+      w.s = sequence<SH>(a, w.b);
+      if (w.s.tiles > 0) break;
+    }
+  }
+  w.chunks = w.b < a.batch ? prompt_chunks<SH>(a, w.s, w.tile, w.begin) : 0;      // (starts that do not ascend can make the list shorter than it counts)
+}
+
 template <typename T, typename SH>
 __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnArgs a) {
   constexpr int D = SH::D, TILES = SH::TILES, BN = SH::BN, BLOCKS = SH::BLOCKS;
@@ -115,29 +312,31 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
   uint8_t* const misc = smem + SH::OFF_MISC;
   const uint32_t bar0 = smem_addr(misc);
   auto bar = [&](int slot) { return bar0 + 8u * (uint32_t)slot; };
-  volatile uint32_t* const s_mask = reinterpret_cast<volatile uint32_t*>(misc + 328);       // [kRing] which 16-key groups of a chunk are there
-  volatile float* const s_key = reinterpret_cast<volatile float*>(misc + 392);               // [kRing] what a chunk's keys were divided by
-  volatile float* const s_value = reinterpret_cast<volatile float*>(misc + 456);             // [kRing] what O has to be multiplied by before it
-  volatile float* const s_last = reinterpret_cast<volatile float*>(misc + 520);              // what the values were divided by in the end
-  volatile uint32_t* const s_abort = reinterpret_cast<volatile uint32_t*>(misc + 524);
-  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(misc + 528);
-  volatile int* const s_grown = reinterpret_cast<volatile int*>(misc + 532);                // [4] values so far are below 2^this
+  volatile uint32_t* const s_mask = reinterpret_cast<volatile uint32_t*>(misc + 336);       // [kRing] which 16-key groups of a chunk are there
+  volatile float* const s_key = reinterpret_cast<volatile float*>(misc + 400);               // [kRing] what a chunk's keys were divided by
+  volatile float* const s_value = reinterpret_cast<volatile float*>(misc + 464);             // [kRing] what O has to be multiplied by before it
+  volatile float* const s_scale = reinterpret_cast<volatile float*>(misc + 528);             // [kRing] what its values were divided by
+  volatile int* const s_grown = reinterpret_cast<volatile int*>(misc + 592);                 // [4] values so far are below 2^this
+  volatile uint32_t* const s_abort = reinterpret_cast<volatile uint32_t*>(misc + 608);
+  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(misc + 612);
+  PromptItem* const s_start = reinterpret_cast<PromptItem*>(misc + 616);
+  unsigned* const s_range = reinterpret_cast<unsigned*>(misc + 616 + sizeof(PromptItem));    // [2]
 
   grid_launch_dependents();
   grid_dependency_wait();
-  Sequence mine = {};
-  (void)deal<SH>(a, lane, 1, mine);
-  Walk w;
-  unsigned unused;
-  if (!place<SH>(a, lane, mine, blockIdx.x, true, w, unused)) return;
-  w.tile = w.s.tiles - 1 - w.tile;                                   // the longest ones of a sequence first
-  const int row0 = w.tile * SH::ROWS, rows = w.s.nq * a.each;
-  const int pos0 = w.s.len - w.s.nq;                                 // the position of the sequence's first query
-  const int j0 = row0 / a.each, j1 = min(w.s.nq - 1, (row0 + SH::ROWS - 1) / a.each);
-  const int end = pos0 + j1 + 1;                                     // keys that some row sees: [begin, end)
-  const int begin = a.window ? (int)max((long long)pos0 + j0 - a.window + 1, 0LL) / BN * BN : 0;
-  const int chunks = end > begin ? (end - begin + BN - 1) / BN : 0;
-
+  if (warp == 0) {
+    const Deal d = prompt_deal<SH>(a, lane, gridDim.x);
+    const unsigned u0 = d.start(blockIdx.x), u1 = d.start(blockIdx.x + 1);
+    PromptItem first = {};
+    if (u0 < u1) prompt_place<SH>(a, lane, u0, first);
+    if (lane == 0) {
+      *s_start = first;
+      s_range[0] = u0;
+      s_range[1] = u1;
+      a.plan[blockIdx.x] = make_int4((int)d.total, first.unit, first.chunks + SH::OPENING, first.head);
+      a.plan[gridDim.x + blockIdx.x] = make_int4(first.b, first.tile, first.s.q0, first.s.nq);
+    }
+  }
   if (tid == 0) {
     *s_abort = 0;
     for (int i = 0; i < 4; ++i) {
@@ -152,7 +351,7 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
       mbar_init(bar(kPReady + i), 4);
       mbar_init(bar(kODone + i), 1);
     }
-    mbar_init(bar(kQReady), 4 * TILES);
+    for (int i = 0; i < 2; ++i) mbar_init(bar(kQReady + i), 4);
     fence_barrier_init();
   }
   if (warp == 2) {
@@ -163,6 +362,21 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
+  // The CTA's part of the list: `body` gets an item, its chunks [lo, hi) that are this CTA's, whether that is all of it and whether it is its
+  // beginning, and how many chunks the CTA has had before.  Every role goes through it for itself.
+  auto segments = [&](auto body) {
+    PromptItem w = *s_start;
+    unsigned left = s_range[1] - s_range[0];
+    int before = 0;
+    while (left > 0) {
+      const unsigned units = (unsigned)(w.chunks + SH::OPENING), take = min(units - w.unit, left);
+      const int lo = max(w.unit - SH::OPENING, 0), hi = max((int)(w.unit + take) - SH::OPENING, 0);
+      body(w, lo, hi, w.unit == 0 && take == units, w.unit == 0, before);
+      before += hi - lo;
+      left -= take;
+      if (left > 0) prompt_next<SH>(a, w);
+    }
+  };
   // every wait is bounded: when one runs out nothing waits any more, and the host is told
   auto guarded = [&](uint32_t b, uint32_t parity) {
     if (*s_abort == 0u && !mbar_wait(b, parity)) {
@@ -194,38 +408,40 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
     const int psz = min(a.page_size, BN), pieces = BN / psz, groups = psz / 16;
     const int piece = lane >> 2, kind = lane & 3;                    // kind: key codes, value codes, key parameters, value parameters
     const int row_bytes = kind < 2 ? D / 2 : 4;
-    const uint8_t* const source = (kind < 2 ? a.codes : a.params) + ((long long)(kind & 1) * a.kv_heads + w.head) * a.page_size * row_bytes;
     const long long page_bytes = 2LL * a.kv_heads * a.page_size * row_bytes;
     const uint32_t target = smem_addr(smem + SH::OFF_RAW) +
                             (kind == 0 ? 0 : kind == 1 ? SH::CODE_BYTES : kind == 2 ? 2 * SH::CODE_BYTES : 2 * SH::CODE_BYTES + SH::PARAM_BYTES) + piece * psz * row_bytes;
-    const int* const table = a.table + w.b * a.table_stride;
-    auto look_up = [&](int i) {
-      const int at = begin + i * BN + piece * psz;
-      return i < chunks && piece < pieces && at < w.s.len ? table[at >> a.page_shift] : -1;
-    };
-    int page = look_up(0);
     Ring<SH::STAGES> ring;
-    for (int i = 0; i < chunks; ++i, ring.next()) {
-      const int stage = ring.slot, following = look_up(i + 1);
-      const bool valid = (unsigned)page < (unsigned)a.pages;
-      const unsigned votes = __ballot_sync(0xffffffffu, valid);
-      unsigned mask = 0;
+    segments([&](const PromptItem& w, int lo, int hi, bool, bool, int before) {
+      const uint8_t* const source = (kind < 2 ? a.codes : a.params) + ((long long)(kind & 1) * a.kv_heads + w.head) * a.page_size * row_bytes;
+      const int* const table = a.table + w.b * a.table_stride;
+      auto look_up = [&](int i) {
+        const int at = w.begin + i * BN + piece * psz;
+        return i < hi && piece < pieces && at < w.s.len ? table[at >> a.page_shift] : -1;
+      };
+      int page = look_up(lo);
+      for (int i = lo; i < hi; ++i, ring.next()) {
+        const int stage = ring.slot, following = look_up(i + 1);
+        const bool valid = (unsigned)page < (unsigned)a.pages;
+        const unsigned votes = __ballot_sync(0xffffffffu, valid);
+        unsigned mask = 0;
 #pragma unroll
-      for (int p = 0; p < BN / 16; ++p) mask |= (votes >> (4 * (p / groups)) & 1u) << p;
-      guarded(bar(kRawEmpty + stage), ring.phase ^ 1);
-      if (lane == 0) {
-        s_mask[i % kRing] = mask;
-        mbar_expect_tx(bar(kRawFull + stage), (uint32_t)(__popc(mask) * 16 * 2 * (D / 2 + 4)));
+        for (int p = 0; p < BN / 16; ++p) mask |= (votes >> (4 * (p / groups)) & 1u) << p;
+        guarded(bar(kRawEmpty + stage), ring.phase ^ 1);
+        if (lane == 0) {
+          s_mask[(before + i - lo) % kRing] = mask;
+          mbar_expect_tx(bar(kRawFull + stage), (uint32_t)(__popc(mask) * 16 * 2 * (D / 2 + 4)));
+        }
+        __syncwarp();
+        const int at = w.begin + i * BN + piece * psz;
+        if (valid && *s_abort == 0u)
+          bulk_g2s(target + stage * SH::RAW_BYTES, source + page * page_bytes + (long long)(at & (a.page_size - 1)) * row_bytes, (uint32_t)(psz * row_bytes), bar(kRawFull + stage));
+        page = following;
       }
-      __syncwarp();
-      const int at = begin + i * BN + piece * psz;
-      if (valid && *s_abort == 0u)
-        bulk_g2s(target + stage * SH::RAW_BYTES, source + page * page_bytes + (long long)(at & (a.page_size - 1)) * row_bytes, (uint32_t)(psz * row_bytes), bar(kRawFull + stage));
-      page = following;
-    }
+    });
   } else if (warp == 1 || (TILES == 2 && warp == 3)) {
     // ------------------------------------------------------------ the tensor core, for one row tile
-    if (elect_one() && chunks > 0) {
+    if (elect_one()) {
       constexpr uint32_t kScores = umma_idesc(kAccF32, kFmtF16, kFmtF16, 128, BN);
       constexpr uint32_t kOut = umma_idesc(kAccF32, kFmtF16, kFmtF16, 128, D) | 1u << 16;      // second operand: long side contiguous
       const int tile = warp >> 1;
@@ -234,34 +450,52 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
       const uint64_t v_desc = umma_desc_mn_sw128(base + SH::OFF_V, BN * 128);
       // scores run one chunk ahead; a buffer of theirs is free again behind the product that read P from it (the tensor core works in order)
       Ring<SH::STAGES> kr, vr;
-      polled(bar(kQReady), 0);
-      bool k_ready = false;
-      for (int i = 0; i <= chunks; ++i) {
-        if (i < chunks) {
-          if (!k_ready) polled(bar(kKReady + kr.slot), kr.phase);
-          tc_fence_after();
-          const uint64_t kd = k_desc + kr.slot * (SH::KV_BYTES >> 4);
+      uint32_t q_phase = 0;
+      segments([&](const PromptItem&, int lo, int hi, bool, bool, int before) {
+        if (hi == lo) return;
+        polled(bar(kQReady + tile), q_phase);
+        q_phase ^= 1;
+        bool k_ready = false;
+        const int n_end = before + hi - lo;
+        for (int n = before; n <= n_end; ++n) {
+          if (n < n_end) {
+            if (!k_ready) polled(bar(kKReady + kr.slot), kr.phase);
+            tc_fence_after();
+            const uint64_t kd = k_desc + kr.slot * (SH::KV_BYTES >> 4);
 #pragma unroll
-          for (int s = 0; s < D / 16; ++s)
-            umma_ss(s_tile + (i & 1) * BN, q_desc + (s >> 2) * (128 * 128 >> 4) + 2 * (s & 3), kd + (s >> 2) * (BN * 128 >> 4) + 2 * (s & 3), kScores, s ? 1u : 0u);
-          umma_commit(bar(kSFull + 2 * tile + (i & 1)));
-          umma_commit(bar(kKEmpty + kr.slot));
-          kr.next();
-        }
-        k_ready = i + 1 < chunks && mbar_test_wait(bar(kKReady + kr.slot), kr.phase);      // answered while the wait below goes on
-        if (i > 0) {
-          const int last = i - 1;
-          polled2(bar(kVReady + vr.slot), vr.phase, bar(kPReady + 2 * tile + (last & 1)), last >> 1 & 1);
-          tc_fence_after();
-          const uint64_t vd = v_desc + vr.slot * (SH::KV_BYTES >> 4);
+            for (int s = 0; s < D / 16; ++s)
+              umma_ss(s_tile + (n & 1) * BN, q_desc + (s >> 2) * (128 * 128 >> 4) + 2 * (s & 3), kd + (s >> 2) * (BN * 128 >> 4) + 2 * (s & 3), kScores, s ? 1u : 0u);
+            umma_commit(bar(kSFull + 2 * tile + (n & 1)));
+            umma_commit(bar(kKEmpty + kr.slot));
+            kr.next();
+          }
+          k_ready = n + 1 < n_end && mbar_test_wait(bar(kKReady + kr.slot), kr.phase);      // answered while the wait below goes on
+          if (n > before) {
+            const int last = n - 1;
+            polled2(bar(kVReady + vr.slot), vr.phase, bar(kPReady + 2 * tile + (last & 1)), last >> 1 & 1);
+            tc_fence_after();
+            const uint64_t vd = v_desc + vr.slot * (SH::KV_BYTES >> 4);
 #pragma unroll
-          for (int s = 0; s < BN / 16; ++s) umma_ts_f16(o_tile, s_tile + (last & 1) * BN + 8 * s, vd + s * (2048 >> 4), kOut, last || s ? 1u : 0u);
-          umma_commit(bar(kODone + 2 * tile + (last & 1)));
-          if (i < chunks) umma_commit(bar(kVEmpty + vr.slot));       // (nothing is left in flight behind the last product)
-          vr.next();
+            for (int s = 0; s < BN / 16; ++s) umma_ts_f16(o_tile, s_tile + (last & 1) * BN + 8 * s, vd + s * (2048 >> 4), kOut, last > before || s ? 1u : 0u);
+            umma_commit(bar(kVEmpty + vr.slot));
+            umma_commit(bar(kODone + 2 * tile + (last & 1)));      // the last of what is in flight: the softmax waits for it
+            vr.next();
+          }
         }
-      }
+      });
     }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------ the queries of all the CTA's items into L2, ahead of their use
+    segments([&](const PromptItem& w, int lo, int hi, bool, bool, int) {
+      if (hi == lo) return;
+      for (int r = lane; r < SH::ROWS; r += 32) {
+        const int row = w.tile * SH::ROWS + r, j = row / a.each;
+        if (j >= w.s.nq) return;
+        const T* const src = reinterpret_cast<const T*>(a.q) + (long long)(w.s.q0 + j) * a.q_token + (long long)(w.head * a.each + row - j * a.each) * a.q_head;
+#pragma unroll
+        for (int c = 0; c < D; c += 64) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(src + c));
+      }
+    });
   } else if (warp >= 4 && warp < 8) {
     // ------------------------------------------------------------ codes -> fp16, chunk i by the warps of group i % STAGES
     // (converting a chunk is a chain of waits and shuffles that a warp cannot overlap with itself; a group has a slot of each ring to itself,
@@ -270,238 +504,225 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
     constexpr int GROUP = SH::GROUP_WARPS;
     const int slot = (warp & 3) / GROUP;
     const uint8_t* const raw = smem + SH::OFF_RAW + slot * SH::RAW_BYTES;
-    for (int i = slot, phase = 0; i < chunks; i += SH::STAGES, phase ^= 1) {
-      guarded(bar(kRawFull + slot), phase);
-      const uint32_t* const kp = reinterpret_cast<const uint32_t*>(raw + 2 * SH::CODE_BYTES);
-      const uint32_t* const vp = kp + BN;
-      const uint32_t mask = s_mask[i % kRing];
-      const int t0 = begin + i * BN;
-      // the chunk's largest key and value element; what is not there or not finite does not count
-      float2 k[2], v[2];
-      bool there[2], k_good[2], v_good[2];
-      float top_k = 0.0f, top_v = 0.0f;
+    segments([&](const PromptItem& w, int lo, int hi, bool, bool, int before) {
+      for (int n = before + (slot - before % SH::STAGES + SH::STAGES) % SH::STAGES; n < before + hi - lo; n += SH::STAGES) {
+        const int i = lo + n - before;
+        const uint32_t phase = n / SH::STAGES & 1;
+        guarded(bar(kRawFull + slot), phase);
+        const uint32_t* const kp = reinterpret_cast<const uint32_t*>(raw + 2 * SH::CODE_BYTES);
+        const uint32_t* const vp = kp + BN;
+        const uint32_t mask = s_mask[n % kRing];
+        const int t0 = w.begin + i * BN;
+        // the chunk's largest key and value element; what is not there or not finite does not count
+        float2 k[2], v[2];
+        bool there[2], k_good[2], v_good[2];
+        float top_k = 0.0f, top_v = 0.0f;
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int row = lane + 32 * n;
-        there[n] = (mask >> (row >> 4) & 1u) && t0 + row < w.s.len;
-        k[n] = pair_of<T>(kp[row]);
-        v[n] = pair_of<T>(vp[row]);
-        v_good[n] = fabsf(v[n].x) <= 3.402823466e38f && fabsf(v[n].y) <= 3.402823466e38f;
-        k_good[n] = fabsf(k[n].x) <= 3.402823466e38f && fabsf(k[n].y) <= 3.402823466e38f;
-        const float tk = fmaxf(fabsf(k[n].y), fabsf(fmaf(15.0f, k[n].x, k[n].y))), tv = fmaxf(fabsf(v[n].y), fabsf(fmaf(15.0f, v[n].x, v[n].y)));
-        if (there[n] && k_good[n]) top_k = fmaxf(top_k, fminf(tk, 3.402823466e38f));
-        if (there[n] && v_good[n]) top_v = fmaxf(top_v, fminf(tv, 3.402823466e38f));
-      }
-      const int ek = above(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top_k))));      // (positive floats order as their bits)
-      const int own = above(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v))));
-      // values are divided by a power that only grows: the chunk before says how far it has
-      if (i > 0) guarded(bar(kGrown + (i - 1 & 3)), (i - 1) >> 2 & 1);
-      const int grown = i > 0 ? s_grown[i - 1 & 3] : -100, ev = max(grown, own);
-      __syncwarp();
-      if (lane == 0 && (warp & 3) % GROUP == 0) {
-        s_grown[i & 3] = ev;
-        s_key[i % kRing] = pow2(max(ek - 14, -126));
-        s_value[i % kRing] = pow2(max(grown - ev, -126));
-        if (i == chunks - 1) *s_last = pow2(max(ev - 14, -126));
-        mbar_arrive(bar(kGrown + (i & 3)));
-      }
-      const float fk = pow2(14 - ek), fv = pow2(14 - ev), nan = __int_as_float(0x7fffffff);
-      // K, then V: a row (or two) of this lane's in each.  One small loop body: unrolled, the four groups' places in the code evict one another
-      // from the instruction cache (8192-token prompt: 1098 us)
-#pragma unroll 1
-      for (int which = 0; which < 2; ++which) {
-        guarded(bar((which ? kVEmpty : kKEmpty) + slot), phase ^ 1);
-        const uint8_t* const codes = raw + which * SH::CODE_BYTES;
-        uint8_t* const dst = smem + (which ? SH::OFF_V : SH::OFF_K) + slot * SH::KV_BYTES;
-#pragma unroll 1
-        for (int n = GROUP == 2 ? warp & 1 : 0; n < (GROUP == 2 ? (warp & 1) + 1 : 2); ++n) {
-          const int row = lane + 32 * n;
-          const bool here = n ? there[1] : there[0], good = (n ? v_good[1] : v_good[0]) && (which || (n ? k_good[1] : k_good[0]));
-          const float2 par = which ? (n ? v[1] : v[0]) : (n ? k[1] : k[0]);
-          const float by = which ? fv : fk, bad = which ? 0.0f : nan;
-          const __half2 s = __float2half2_rn(!here ? 0.0f : good ? par.x * by : bad), m = __float2half2_rn(!here ? 0.0f : good ? par.y * by : bad);
-          const int turn = D == 64 ? row >> 2 : D == 128 ? row >> 1 : row;       // which piece first: spreads the rows over the banks
-          const uint8_t* const src = codes + row * (D / 2);
-          uint8_t* const lines = dst + row * 128;
-          uint4 x = *reinterpret_cast<const uint4*>(src + turn % PIECES * 16);
-#pragma unroll 1
-          for (int e = 0; e < PIECES; ++e) {
-            const int piece = (turn + e) % PIECES;
-            const uint4 following = *reinterpret_cast<const uint4*>(src + (turn + e + 1) % PIECES * 16);
-            uint8_t* const line = lines + (piece >> 1) * (BN * 128);
-            const int first = (piece & 1) * 4, swizzle = row & 7;
-            *reinterpret_cast<uint4*>(line + (((first + 0) ^ swizzle) << 4)) = eight(x.x, s, m);
-            *reinterpret_cast<uint4*>(line + (((first + 1) ^ swizzle) << 4)) = eight(x.y, s, m);
-            *reinterpret_cast<uint4*>(line + (((first + 2) ^ swizzle) << 4)) = eight(x.z, s, m);
-            *reinterpret_cast<uint4*>(line + (((first + 3) ^ swizzle) << 4)) = eight(x.w, s, m);
-            x = following;
-          }
+        for (int h = 0; h < 2; ++h) {
+          const int row = lane + 32 * h;
+          there[h] = (mask >> (row >> 4) & 1u) && t0 + row < w.s.len;
+          k[h] = pair_of<T>(kp[row]);
+          v[h] = pair_of<T>(vp[row]);
+          v_good[h] = fabsf(v[h].x) <= 3.402823466e38f && fabsf(v[h].y) <= 3.402823466e38f;
+          k_good[h] = fabsf(k[h].x) <= 3.402823466e38f && fabsf(k[h].y) <= 3.402823466e38f;
+          const float tk = fmaxf(fabsf(k[h].y), fabsf(fmaf(15.0f, k[h].x, k[h].y))), tv = fmaxf(fabsf(v[h].y), fabsf(fmaf(15.0f, v[h].x, v[h].y)));
+          if (there[h] && k_good[h]) top_k = fmaxf(top_k, fminf(tk, 3.402823466e38f));
+          if (there[h] && v_good[h]) top_v = fmaxf(top_v, fminf(tv, 3.402823466e38f));
         }
-        fence_proxy_async();
+        const int ek = above(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top_k))));      // (positive floats order as their bits)
+        const int own = above(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v))));
+        // values are divided by a power that only grows along an item: the chunk before says how far it has
+        if (n > 0) guarded(bar(kGrown + (n - 1 & 3)), (n - 1) >> 2 & 1);
+        // (an item's first chunk leaves a factor of four for later ones, so that O is hardly ever rescaled for them)
+        const int grown = i > lo ? s_grown[n - 1 & 3] : min(own + 2, 127), ev = max(grown, own);
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar((which ? kVReady : kKReady) + slot));
+        if (lane == 0 && (warp & 3) % GROUP == 0) {
+          s_grown[n & 3] = ev;
+          s_key[n % kRing] = pow2(max(ek - 14, -126));
+          s_value[n % kRing] = pow2(max(grown - ev, -126));
+          s_scale[n % kRing] = pow2(max(ev - 14, -126));
+          mbar_arrive(bar(kGrown + (n & 3)));
+        }
+        const float fk = pow2(14 - ek), fv = pow2(14 - ev), nan = __int_as_float(0x7fffffff);
+        // K, then V: a row (or two) of this lane's in each.  One small loop body: unrolled, the four groups' places in the code evict one another
+        // from the instruction cache (8192-token prompt: 1098 us)
+#pragma unroll 1
+        for (int which = 0; which < 2; ++which) {
+          guarded(bar((which ? kVEmpty : kKEmpty) + slot), phase ^ 1);
+          const uint8_t* const codes = raw + which * SH::CODE_BYTES;
+          uint8_t* const dst = smem + (which ? SH::OFF_V : SH::OFF_K) + slot * SH::KV_BYTES;
+#pragma unroll 1
+          for (int h = GROUP == 2 ? warp & 1 : 0; h < (GROUP == 2 ? (warp & 1) + 1 : 2); ++h) {
+            const int row = lane + 32 * h;
+            const bool here = h ? there[1] : there[0], good = (h ? v_good[1] : v_good[0]) && (which || (h ? k_good[1] : k_good[0]));
+            const float2 par = which ? (h ? v[1] : v[0]) : (h ? k[1] : k[0]);
+            const float by = which ? fv : fk, bad = which ? 0.0f : nan;
+            const __half2 s = __float2half2_rn(!here ? 0.0f : good ? par.x * by : bad), m = __float2half2_rn(!here ? 0.0f : good ? par.y * by : bad);
+            const int turn = D == 64 ? row >> 2 : D == 128 ? row >> 1 : row;       // which piece first: spreads the rows over the banks
+            const uint8_t* const src = codes + row * (D / 2);
+            uint8_t* const lines = dst + row * 128;
+            uint4 x = *reinterpret_cast<const uint4*>(src + turn % PIECES * 16);
+#pragma unroll 1
+            for (int e = 0; e < PIECES; ++e) {
+              const int piece = (turn + e) % PIECES;
+              const uint4 following = *reinterpret_cast<const uint4*>(src + (turn + e + 1) % PIECES * 16);
+              uint8_t* const line = lines + (piece >> 1) * (BN * 128);
+              const int first = (piece & 1) * 4, swizzle = row & 7;
+              *reinterpret_cast<uint4*>(line + (((first + 0) ^ swizzle) << 4)) = eight(x.x, s, m);
+              *reinterpret_cast<uint4*>(line + (((first + 1) ^ swizzle) << 4)) = eight(x.y, s, m);
+              *reinterpret_cast<uint4*>(line + (((first + 2) ^ swizzle) << 4)) = eight(x.z, s, m);
+              *reinterpret_cast<uint4*>(line + (((first + 3) ^ swizzle) << 4)) = eight(x.w, s, m);
+              x = following;
+            }
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar((which ? kVReady : kKReady) + slot));
+        }
+        if (lane == 0) mbar_arrive(bar(kRawEmpty + slot));
       }
-      if (lane == 0) mbar_arrive(bar(kRawEmpty + slot));
-    }
+    });
   } else if (warp >= 8) {
     // ------------------------------------------------------------ softmax: a thread per row
     const int tile = (warp - 8) >> 2, quarter = warp & 3, line = quarter * 32 + lane;
-    const int row = row0 + tile * 128 + line;
-    const bool real = row < rows;
-    const int j = real ? row / a.each : 0, head = w.head * a.each + (real ? row - j * a.each : 0);
-    float factor;
-    {
-      const T* const src = reinterpret_cast<const T*>(a.q) + (long long)(w.s.q0 + j) * a.q_token + (long long)head * a.q_head;
-      float top = 0.0f;
-#pragma unroll 4
-      for (int c = 0; c < D / 8; ++c) {
-        const uint4 x = real ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0, 0, 0, 0);
-        const T* e = reinterpret_cast<const T*>(&x);
-#pragma unroll
-        for (int n = 0; n < 8; ++n) top = fmaxf(top, fabsf(to_float<T>(e[n])));
-      }
-      const int e = top > 0.0f && top <= 3.402823466e38f ? min(max(above(top) - 1, -100), 100) : 0;
-      const float down = a.scale == 0.0f ? 0.0f : copysignf(pow2(-e), a.scale);
-      factor = pow2(e) * (a.scale == 0.0f ? 1.0f : fabsf(a.scale));
-      uint8_t* const dst = smem + tile * (BLOCKS * 128 * 128) + line * 128;
-#pragma unroll 4
-      for (int c = 0; c < D / 8; ++c) {
-        const uint4 x = real ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0, 0, 0, 0);
-        const T* v = reinterpret_cast<const T*>(&x);
-        uint4 y;
-        y.x = half2_bits(__floats2half2_rn(to_float<T>(v[0]) * down, to_float<T>(v[4]) * down));
-        y.y = half2_bits(__floats2half2_rn(to_float<T>(v[1]) * down, to_float<T>(v[5]) * down));
-        y.z = half2_bits(__floats2half2_rn(to_float<T>(v[2]) * down, to_float<T>(v[6]) * down));
-        y.w = half2_bits(__floats2half2_rn(to_float<T>(v[3]) * down, to_float<T>(v[7]) * down));
-        *reinterpret_cast<uint4*>(dst + (c >> 3) * (128 * 128) + (((c & 7) ^ (line & 7)) << 4)) = y;
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kQReady));
-    }
-    const int hi = real ? pos0 + j : -1, lo = a.window ? (int)max((long long)pos0 + j - a.window + 1, 0LL) : 0;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_tile = tmem + lanes + 2 * tile * BN, o_at = tmem + lanes + SH::O_COL + tile * D;
-    float m = kLowest;
-    Two l(0.0f);
-    bool s_ready = false;
-    for (int i = 0; i < chunks; ++i) {
-      if (!s_ready) guarded(bar(kSFull + 2 * tile + (i & 1)), i >> 1 & 1);
+    // a finished segment whose O is still in tensor memory: it is written when the queries of the next one are on their way
+    T* out = nullptr;
+    float* part = nullptr;
+    float out_by = 0.0f;
+    int out_n = -1;
+    bool out_whole = false;
+    auto flush = [&]() {
+      if (out_n < 0) return;
+      guarded(bar(kODone + 2 * tile + (out_n & 1)), out_n >> 1 & 1);
       tc_fence_after();
-      const uint32_t s_at = s_tile + (i & 1) * BN;
-      const int t0 = begin + i * BN;
-      const float f = fminf(fmaxf(factor * s_key[i % kRing], 7.5e-37f), 1.3e30f), ratio = s_value[i % kRing];
-      const uint32_t there = s_mask[i % kRing];
-      const bool all = there == 0xfu && t0 + BN - 1 <= hi && t0 >= lo;
-      const bool masked = __any_sync(0xffffffffu, !all);
-      // which of the 32 keys from t on this row sees
-      auto visible = [&](int n) {
-        const int t = t0 + 32 * n;
-        uint32_t bits = 0xffffffffu;
-        if (hi < t + 31) bits = hi < t ? 0u : 0xffffffffu >> (t + 31 - hi);
-        if (lo > t) bits = lo > t + 31 ? 0u : bits & 0xffffffffu << (lo - t);
-        const uint32_t two = there >> (2 * n);
-        return bits & ((two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u));
-      };
-      auto hide = [&](uint32_t (&r)[32], int n) {
-        const uint32_t bits = visible(n);
-#pragma unroll
-        for (int e = 0; e < 32; ++e) r[e] = bits >> e & 1u ? r[e] : 0xff800000u;
-      };
-      auto largest = [](const uint32_t (&r)[32]) {
-        float x = __uint_as_float(r[0]), y = __uint_as_float(r[1]);
-#pragma unroll
-        for (int e = 2; e < 32; e += 2) {
-          x = fmaxf(x, __uint_as_float(r[e]));
-          y = fmaxf(y, __uint_as_float(r[e + 1]));
-        }
-        return fmaxf(x, y);
-      };
-      uint32_t ra[32], rb[32];
-      tmem_ld_32x32(s_at, ra);
-      tmem_ld_32x32(s_at + 32, rb);
-      wait_ld_dep32(ra);
-      wait_ld_dep32(rb);
-      if (masked) {
-        hide(ra, 0);
-        hide(rb, 1);
+      out_n = -1;
+      const unsigned long long mine = part != nullptr ? reinterpret_cast<unsigned long long>(part) : reinterpret_cast<unsigned long long>(out);
+      store_rows<T, D>(o_at, mine, out_by, out_whole);
+    };
+    segments([&](const PromptItem& w, int lo, int hi, bool whole, bool opens, int before) {
+      const int row = w.tile * SH::ROWS + tile * 128 + line;
+      const bool real = row < w.s.nq * a.each;
+      const int j = real ? row / a.each : 0, head = w.head * a.each + (real ? row - j * a.each : 0);
+      const int hi_key = real ? w.s.len - w.s.nq + j : -1, from = a.window ? (int)max((long long)w.s.len - w.s.nq + j - a.window + 1, 0LL) : 0;
+      const int n_end = before + hi - lo;
+      float factor = 0.0f, m = kLowest;
+      Two l(0.0f);
+      if (hi > lo) {
+        const T* const src = real ? reinterpret_cast<const T*>(a.q) + (long long)(w.s.q0 + j) * a.q_token + (long long)head * a.q_head : nullptr;
+        factor = load_queries<T, D>(src, smem + tile * (BLOCKS * 128 * 128) + quarter * 32 * 128, a.scale);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kQReady + tile));
       }
-      float top = fmaxf(largest(ra), largest(rb));
-      top *= f;
-      const bool moves = top > m + 8.0f || (m == kLowest && top > kLowest);
-      if (__any_sync(0xffffffffu, moves) || ratio != 1.0f) {
-        const float next = fmaxf(m, top);
-        const float alpha = m == next ? 1.0f : exp2_fast(m - next);
-        m = next;
-        l = l * Two(alpha);
-        if (i > 0) {
-          guarded(bar(kODone + 2 * tile + (i - 1 & 1)), i - 1 >> 1 & 1);       // the product before has to be in O
-          tc_fence_after();
-          const Two by(alpha * ratio);
-#pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t r[32];
-            tmem_ld_32x32(o_at + 32 * c, r);
-            wait_ld_dep32(r);
+      flush();
+      bool s_ready = false;
+      for (int n = before; n < n_end; ++n) {
+        if (!s_ready) guarded(bar(kSFull + 2 * tile + (n & 1)), n >> 1 & 1);
+        tc_fence_after();
+        const uint32_t s_at = s_tile + (n & 1) * BN;
+        const int t0 = w.begin + (lo + n - before) * BN;
+        const float f = fminf(fmaxf(factor * s_key[n % kRing], 7.5e-37f), 1.3e30f), ratio = s_value[n % kRing];
+        const uint32_t there = s_mask[n % kRing];
+        const bool all = there == 0xfu && t0 + BN - 1 <= hi_key && t0 >= from;
+        const bool masked = __any_sync(0xffffffffu, !all);
+        // which of the 32 keys from t on this row sees
+        auto visible = [&](int h) {
+          const int t = t0 + 32 * h;
+          uint32_t bits = 0xffffffffu;
+          if (hi_key < t + 31) bits = hi_key < t ? 0u : 0xffffffffu >> (t + 31 - hi_key);
+          if (from > t) bits = from > t + 31 ? 0u : bits & 0xffffffffu << (from - t);
+          const uint32_t two = there >> (2 * h);
+          return bits & ((two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u));
+        };
+        auto hide = [&](uint32_t (&r)[32], int h) {
+          const uint32_t bits = visible(h);
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float2 v = (Two(__uint_as_float(r[e]), __uint_as_float(r[e + 1])) * by).both();
-              r[e] = __float_as_uint(v.x);
-              r[e + 1] = __float_as_uint(v.y);
+          for (int e = 0; e < 32; ++e) r[e] = bits >> e & 1u ? r[e] : 0xff800000u;
+        };
+        auto largest = [](const uint32_t (&r)[32]) {
+          float x = __uint_as_float(r[0]), y = __uint_as_float(r[1]);
+#pragma unroll
+          for (int e = 2; e < 32; e += 2) {
+            x = fmaxf(x, __uint_as_float(r[e]));
+            y = fmaxf(y, __uint_as_float(r[e + 1]));
+          }
+          return fmaxf(x, y);
+        };
+        uint32_t ra[32], rb[32];
+        tmem_ld_32x32(s_at, ra);
+        tmem_ld_32x32(s_at + 32, rb);
+        wait_ld_dep32(ra);
+        wait_ld_dep32(rb);
+        if (masked) {
+          hide(ra, 0);
+          hide(rb, 1);
+        }
+        float top = fmaxf(largest(ra), largest(rb));
+        top *= f;
+        const bool moves = top > m + 8.0f || (m == kLowest && top > kLowest);
+        if (__any_sync(0xffffffffu, moves) || ratio != 1.0f) {
+          const float next = fmaxf(m, top);
+          const float alpha = m == next ? 1.0f : exp2_fast(m - next);
+          m = next;
+          l = l * Two(alpha);
+          if (n > before) {
+            guarded(bar(kODone + 2 * tile + (n - 1 & 1)), n - 1 >> 1 & 1);       // the product before has to be in O
+            tc_fence_after();
+            const Two by(alpha * ratio);
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t r[32];
+              tmem_ld_32x32(o_at + 32 * c, r);
+              wait_ld_dep32(r);
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                const float2 v = (Two(__uint_as_float(r[e]), __uint_as_float(r[e + 1])) * by).both();
+                r[e] = __float_as_uint(v.x);
+                r[e + 1] = __float_as_uint(v.y);
+              }
+              tmem_st_32x32(o_at + 32 * c, r);
             }
-            tmem_st_32x32(o_at + 32 * c, r);
           }
         }
+        const Two f2(f), minus(m == kLowest ? 0.0f : -m);
+        auto weigh = [&](const uint32_t (&r)[32], int at) {
+          uint32_t h[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float2 x = fma2(Two(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), f2, minus).both();
+            const float2 p = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+            l = l + Two(p.x, p.y);
+            h[e] = half2_bits(__floats2half2_rn(p.x, p.y));
+          }
+          tmem_st_32x16(s_at + 16 * at, h);             // over the scores, which are all in registers
+        };
+        weigh(ra, 0);
+        s_ready = n + 1 < n_end && mbar_test_wait(bar(kSFull + 2 * tile + (n + 1 & 1)), n + 1 >> 1 & 1);
+        weigh(rb, 1);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kPReady + 2 * tile + (n & 1)));
       }
-      const Two f2(f), minus(m == kLowest ? 0.0f : -m);
-      auto weigh = [&](const uint32_t (&r)[32], int n) {
-        uint32_t h[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float2 x = fma2(Two(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), f2, minus).both();
-          const float2 p = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-          l = l + Two(p.x, p.y);
-          h[e] = half2_bits(__floats2half2_rn(p.x, p.y));
-        }
-        tmem_st_32x16(s_at + 16 * n, h);             // over the scores, which are all in registers
-      };
-      weigh(ra, 0);
-      s_ready = i + 1 < chunks && mbar_test_wait(bar(kSFull + 2 * tile + (i + 1 & 1)), i + 1 >> 1 & 1);
-      weigh(rb, 1);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kPReady + 2 * tile + (i & 1)));
-    }
-    if (chunks > 0) {
-      guarded(bar(kODone + 2 * tile + (chunks - 1 & 1)), chunks - 1 >> 1 & 1);
-      tc_fence_after();
-    }
-    const float2 sums = l.both();
-    const float weight = sums.x + sums.y;
-    const float inv = weight == 0.0f || chunks == 0 ? 0.0f : *s_last / weight;
-    T* const out = reinterpret_cast<T*>(a.out) + ((long long)(w.s.q0 + j) * a.q_heads + head) * D;
-#pragma unroll 1
-    for (int c = 0; c < D / 32; ++c) {
-      uint32_t r[32];
-      if (chunks > 0) {
-        tmem_ld_32x32(o_at + 32 * c, r);
-        wait_ld_dep32(r);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 32; ++e) r[e] = 0u;
+      const float2 sums = l.both();
+      const float weight = sums.x + sums.y;
+      const long long slot_row = (long long)(2 * blockIdx.x + (opens ? 1 : 0)) * SH::ROWS + tile * 128 + line;
+      T* const row_out = real ? reinterpret_cast<T*>(a.out) + ((long long)(w.s.q0 + j) * a.q_heads + head) * D : nullptr;
+      if (!whole && real) a.part_ml[slot_row] = make_float2(m, weight);
+      if (hi > lo) {
+        const float scale = s_scale[(n_end - 1) % kRing];
+        out_n = n_end - 1;
+        out_whole = whole;
+        out = whole ? row_out : nullptr;
+        part = whole || !real ? nullptr : a.part_o + slot_row * D;
+        out_by = !whole ? scale : weight == 0.0f ? 0.0f : scale / weight;
+      } else if (whole && real) {                    // no keys at all
+        for (int c = 0; c < D / 8; ++c) reinterpret_cast<uint4*>(row_out)[c] = make_uint4(0, 0, 0, 0);
       }
-      if (real) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          uint4 y;
-          T* const v = reinterpret_cast<T*>(&y);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = from_float<T>(__uint_as_float(r[8 * b + (e < 4 ? 2 * e : 2 * e - 7)]) * inv);
-          *reinterpret_cast<uint4*>(out + 32 * c + 8 * b) = y;
-        }
-      }
-    }
+    });
+    flush();
   }
   tc_fence_before();
   __syncthreads();
@@ -511,26 +732,87 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
   }
 }
 
-template <typename T, int D, int TILES, int STAGES>
-int run(const AttnArgs& a, cudaStream_t stream) {
-  using SH = PromptShape<D, TILES, STAGES>;
+// Joins the items that a boundary between two CTAs runs through: block x for boundary x + 1, if it is the first in its item; a row per warp.
+template <typename T, typename SH>
+__global__ void __launch_bounds__(256) kv4_prompt_join_kernel(const AttnArgs a, unsigned ctas) {
+  constexpr int D = SH::D, PER = D / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int4 p = a.plan[blockIdx.x + 1], w = a.plan[ctas + blockIdx.x + 1];       // total, unit, units, head | sequence, tile, first query, queries
+  if (p.y == 0) return;
+  Deal d;
+  d.total = (unsigned)p.x;
+  d.each = d.total / ctas;
+  d.more = d.total - d.each * ctas;
+  const unsigned u0 = d.start(blockIdx.x + 1) - (unsigned)p.y;                    // the item's first unit
+  const unsigned i0 = d.owner(u0), i1 = d.owner(u0 + (unsigned)p.z - 1);
+  if (i0 != blockIdx.x) return;
+  {
+    const int line = blockIdx.y * 8 + warp, row = w.y * SH::ROWS + line, j = row / a.each;
+    if (j >= w.w) return;
+    float m = -CUDART_INF_F, weight = 0.0f, sum[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) sum[e] = 0.0f;
+    for (unsigned i = i0; i <= i1; ++i) {
+      const long long at = (2LL * i + (d.start(i) > u0 ? 0 : 1)) * SH::ROWS + line;
+      const float2 s = a.part_ml[at];
+      if (s.y == 0.0f) continue;                     // it saw nothing, and may have written nothing else
+      const float top = fmaxf(m, s.x), keep = m == top ? 1.0f : exp2_fast(m - top), by = exp2_fast(s.x - top);
+      m = top;
+      weight = fmaf(s.y, by, weight * keep);
+      const float* const src = a.part_o + at * D + lane * PER;
+#pragma unroll
+      for (int e = 0; e < PER; e += 2) {
+        const float2 v = *reinterpret_cast<const float2*>(src + e);
+        sum[e] = fmaf(v.x, by, sum[e] * keep);
+        sum[e + 1] = fmaf(v.y, by, sum[e + 1] * keep);
+      }
+    }
+    const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
+    T* const out = reinterpret_cast<T*>(a.out) + ((long long)(w.z + j) * a.q_heads + p.w * a.each + row - j * a.each) * D + lane * PER;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) out[e] = from_float<T>(sum[e] * inv);
+  }
+}
+
+// CTAs, and the bytes behind each other in the workspace: sums, their maxima and weights, the CTAs' beginnings
+template <typename SH>
+long long prompt_units(const AttnArgs& a) {
   const long long items = ((long long)a.tokens * a.each / SH::ROWS + a.batch) * a.kv_heads;
-  XQT_REQUIRE(items < (1LL << 31) - 1);
+  return items * (((long long)a.table_width << a.page_shift) / SH::BN + 1 + SH::OPENING);
+}
+size_t prompt_bytes(int ctas, int rows, int dim) { return (size_t)2 * ctas * rows * (dim * 4 + 8) + (size_t)2 * ctas * 16; }
+
+template <typename T, int D, int TILES, int STAGES>
+int run(AttnArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  using SH = PromptShape<D, TILES, STAGES>;
+  const long long units = prompt_units<SH>(a);
+  XQT_REQUIRE(units < (1LL << 31));
+  const int ctas = (int)min((long long)sm_count(), units);
+  XQT_REQUIRE(workspace && workspace_bytes >= prompt_bytes(ctas, SH::ROWS, D) && ((uintptr_t)workspace & 15) == 0);
+  a.part_o = reinterpret_cast<float*>(workspace);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)2 * ctas * SH::ROWS * D);
+  a.plan = reinterpret_cast<int4*>(a.part_ml + (size_t)2 * ctas * SH::ROWS);
   XQT_SMEM_OPT_IN((kv4_prompt_kernel<T, SH>), SH::SMEM);
-  return launch_pdl(kv4_prompt_kernel<T, SH>, dim3((unsigned)items), dim3(SH::THREADS), SH::SMEM, stream, a);
+  const int rc = launch_pdl(kv4_prompt_kernel<T, SH>, dim3((unsigned)ctas), dim3(SH::THREADS), SH::SMEM, stream, a);
+  if (rc || ctas == 1) return rc;
+  return launch_pdl(kv4_prompt_join_kernel<T, SH>, dim3((unsigned)ctas - 1, SH::ROWS / 8), dim3(256), 0, stream, a, (unsigned)ctas);
 }
 
 template <typename T>
-int run_dim(const AttnArgs& a, int dim, cudaStream_t stream) {
-  if (dim == 64) return run<T, 64, 2, 4>(a, stream);
-  if (dim == 128) return run<T, 128, 2, 4>(a, stream);
-  return run<T, 256, 1, 2>(a, stream);
+int run_dim(const AttnArgs& a, int dim, void* workspace, size_t bytes, cudaStream_t stream) {
+  if (dim == 64) return run<T, 64, 2, 4>(a, workspace, bytes, stream);
+  if (dim == 128) return run<T, 128, 2, 4>(a, workspace, bytes, stream);
+  return run<T, 256, 1, 2>(a, workspace, bytes, stream);
 }
 
 }  // namespace
 
-int kv4_prompt_launch(const kv4::AttnArgs& a, int dim, int dtype, cudaStream_t stream) {
-  return dtype == XQT_B200_BF16 ? run_dim<__nv_bfloat16>(a, dim, stream) : run_dim<__half>(a, dim, stream);
+int kv4_prompt_launch(const kv4::AttnArgs& a, int dim, int dtype, void* workspace, size_t bytes, cudaStream_t stream) {
+  return dtype == XQT_B200_BF16 ? run_dim<__nv_bfloat16>(a, dim, workspace, bytes, stream) : run_dim<__half>(a, dim, workspace, bytes, stream);
 }
+
+size_t kv4_prompt_workspace_bytes(int dim) { return prompt_bytes(sm_count(), dim == 256 ? 128 : 256, dim); }
 
 }  // namespace xqt_b200

@@ -206,6 +206,12 @@ B200_KERNELS = (
     KernelSpec("quantization.int8_mma_linear", KernelBackend.CUSTOM_CUDA, "xqt_b200.ops.w8a8:int8_mma_linear", SM100,
                "per-tensor dynamic W8A8 (Int8MmaLinear semantics) on tcgen05 kind::i8"),
     KernelSpec("quantization.swiglu", KernelBackend.CUSTOM_CUDA, "xqt_b200.ops.mlp:swiglu", SM100, "fused SwiGLU gating"),
+    KernelSpec("attention.qk_norm_rope", KernelBackend.CUSTOM_CUDA, "xqt_b200.ops.rotary:qk_norm_rope", SM100,
+               "RMS norm of query and key heads and the position rotation (one or several axes) in one pass"),
+    KernelSpec("attention.kv4_append", KernelBackend.CUSTOM_CUDA, "xqt_b200.ops.kv4:kv4_append", SM100, "keys and values into a paged 4-bit cache"),
+    KernelSpec("attention.kv4_gather", KernelBackend.CUSTOM_CUDA, "xqt_b200.ops.kv4:kv4_gather", SM100, "keys and values out of a paged 4-bit cache"),
+    KernelSpec("attention.kv4_attention", KernelBackend.CUSTOM_CUDA, "xqt_b200.ops.kv4:kv4_attention", SM100,
+               "attention over a paged 4-bit cache: single tokens, drafted tokens, prompts"),
 )
 for _spec in B200_KERNELS:
     register_kernel(_spec)

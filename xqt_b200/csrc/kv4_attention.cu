@@ -56,7 +56,7 @@ struct Shape {
   static constexpr int CODE_BYTES = CT * KROW, PARAM_BYTES = CT * 4, STAGE = 2 * (CODE_BYTES + PARAM_BYTES);
   static constexpr int MERGE_ROW = D + 8;
   static constexpr int MERGES = W / 2;                    // buffers: the warps write them in two rounds
-  static constexpr int MERGE_BYTES = MERGES * ROWS * MERGE_ROW * 4, STAT_BYTES = W * ROWS * 16;
+  static constexpr int MERGE_BYTES = MERGES * ROWS * MERGE_ROW * 4, STAT_BYTES = (2 * W + 1) * ROWS * 16;      // the warps' statistics twice: an item's are written while the last one's are read
   static constexpr int SMEM = W * S * STAGE + MERGE_BYTES + STAT_BYTES + W * S * 8;
 };
 
@@ -74,7 +74,14 @@ __device__ __forceinline__ void advance(const AttnArgs& a, Walk& w) {
   }
 }
 
-template <typename T, typename SH>
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t caddr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "r"(caddr) : "memory");
+  return v;
+}
+
+// CLUSTER: single tokens; a cluster of CTAs takes one item, each an equal run of its units, and joins it through distributed shared memory.
+template <typename T, typename SH, bool CLUSTER>
 __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(const AttnArgs a) {
   constexpr int D = SH::D, NT = SH::NT, W = SH::W, CT = SH::CT, S = SH::S, ROWS = SH::ROWS, MT = SH::MT, KROW = SH::KROW;
   constexpr int KWORDS = SH::KWORDS, VWORDS = SH::VWORDS;
@@ -82,7 +89,9 @@ __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(c
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   uint8_t* const ring = smem + warp * (S * SH::STAGE);
   float* const merge = reinterpret_cast<float*>(smem + W * S * SH::STAGE);
-  float4* const stats = reinterpret_cast<float4*>(smem + W * S * SH::STAGE + SH::MERGE_BYTES);
+  float4* stats = reinterpret_cast<float4*>(smem + W * S * SH::STAGE + SH::MERGE_BYTES);
+  float4* const stats0 = stats;
+  float4* const cta_ml = stats + 2 * W * ROWS;             // CLUSTER: of the CTA's part
   const uint32_t bars = smem_addr(smem + W * S * SH::STAGE + SH::MERGE_BYTES + SH::STAT_BYTES) + warp * (S * 8);
   if (lane == 0) {
     for (int s = 0; s < S; ++s) mbar_init(bars + 8 * s, 1);
@@ -92,13 +101,30 @@ __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(c
   grid_launch_dependents();
   grid_dependency_wait();
 
-  Sequence mine = {};
-  const Deal d = deal<SH>(a, lane, gridDim.x, mine);
-  const unsigned u0 = d.start(blockIdx.x), u1 = d.start(blockIdx.x + 1);
-  if (u0 >= u1) return;
   Walk c;
-  unsigned unused;
-  if (!place<SH>(a, lane, mine, u0, false, c, unused)) return;
+  unsigned u0 = 0, u1;
+  if constexpr (CLUSTER) {
+    const unsigned rank = cluster_ctarank(), size = cluster_nctarank(), item = blockIdx.x / size;
+    const unsigned tiles = (unsigned)(a.each + ROWS - 1) / ROWS, of_sequence = item / a.kv_heads;
+    c.head = (int)(item - of_sequence * a.kv_heads);
+    c.b = (int)(of_sequence / tiles);
+    c.tile = (int)(of_sequence - c.b * tiles);
+    c.s = sequence<SH>(a, c.b);
+    const unsigned units = (unsigned)(c.s.units - SH::OPENING), lo = units * rank / size;
+    c.unit = SH::OPENING + (int)lo;
+    u1 = units * (rank + 1) / size - lo;
+  } else {
+    Sequence mine = {};
+    const Deal d = deal<SH>(a, lane, gridDim.x, mine);
+    u0 = d.start(blockIdx.x);
+    u1 = d.start(blockIdx.x + 1);
+    const bool some = u0 < u1 && place<SH>(a, lane, mine, u0, c);
+    if (tid == 0) {                                  // for the second kernel: where this CTA begins
+      a.plan[blockIdx.x] = make_int4((int)d.total, some ? c.unit : 0, some ? c.s.units : 0, some ? c.head : 0);
+      a.plan[gridDim.x + blockIdx.x] = some ? make_int4(c.b, c.tile, c.s.q0, c.s.nq) : make_int4(0, 0, 0, 0);
+    }
+    if (!some) return;
+  }
 
   // ---- fetching
   const int psz = min(a.page_size, CT), pieces = CT / psz;
@@ -252,9 +278,8 @@ __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(c
     full_lo = a.window ? (int)max((long long)c.s.len - c.s.nq + min(j1, c.s.nq - 1) - a.window + 1, 0LL) : 0;
   };
 
-  // FULL: every row sees every key of the chunk
-  auto chunk = [&](auto full_tag, const uint8_t* st, int tok0, unsigned mask) {
-    constexpr bool FULL = decltype(full_tag)::value;
+  // full: every row sees every key of the chunk
+  auto chunk = [&](const uint8_t* st, int tok0, unsigned mask, bool full) {
     const uint8_t* const kp = st + 2 * SH::CODE_BYTES;
     const uint8_t* const vp = kp + SH::PARAM_BYTES;
     const int pg = g ^ (g >> 1 & 1);                 // the key of operand row g: neighbours alternate, which spreads the value rows over the banks
@@ -301,17 +326,28 @@ __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(c
           p[mt][nt][2 * e] = x.x;
           p[mt][nt][2 * e + 1] = x.y;
         }
-        if constexpr (!FULL) {
-          const int tok = tok0 + r0 + 8 * e;
-          const bool there = mask >> ((r0 + 8 * e) / psz) & 1u;
+      }
+    }
+    if (!full) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int at = mt * 16 + pg + 8 * e, tok = tok0 + at;
+          const bool there = mask >> (at / psz) & 1u;
+          if (!there || tok >= c.s.len) vb[mt][e] = 0;       // nothing was fetched, or nothing was ever written
+          // a value that is not finite spoils the rows that see it by their scores, and counts as 0 for the others
+          const float2 v = pair_of<T>(vb[mt][e]);
+          const bool bad = !(fabsf(v.x) <= 3.402823466e38f && fabsf(v.y) <= 3.402823466e38f);
+          if (bad) vb[mt][e] = 0;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 2; ++i) {
+              if (bad) p[mt][nt][2 * e + i] = CUDART_NAN_F;
               if (!there || tok > hi[nt][i] || tok < lo[nt][i]) p[mt][nt][2 * e + i] = -CUDART_INF_F;
-          if (!there || tok >= c.s.len) vb[mt][e] = 0;     // nothing was fetched, or nothing was ever written
+            }
         }
-      }
     }
     // running maxima; nothing is exchanged while no lane exceeds them
     float top[NT][2], big = 0.0f;
@@ -385,15 +421,8 @@ __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(c
           const Two pr(exp2_fast(x.x), exp2_fast(x.y));
           l[nt] = l[nt] + pr;
           const float2 sv = pair_of<T>(vb[mt][e]);
-          Two w2 = pr * Two(sv.x * inv_sigma), pm = pr * Two(sv.y);
-          if constexpr (FULL) {
-            lm[nt] = lm[nt] + pm;
-          } else {                                   // what a row does not see may be anything
-            const bool h0 = p[mt][nt][2 * e] == -CUDART_INF_F, h1 = p[mt][nt][2 * e + 1] == -CUDART_INF_F;
-            const float2 w = w2.both(), m = pm.both();
-            w2 = Two(h0 ? 0.0f : w.x, h1 ? 0.0f : w.y);
-            lm[nt] = lm[nt] + Two(h0 ? 0.0f : m.x, h1 ? 0.0f : m.y);
-          }
+          const Two w2 = pr * Two(sv.x * inv_sigma);
+          lm[nt] = fma2(pr, Two(sv.y), lm[nt]);
           const float2 w = w2.both();
           const uint32_t h = pack_half2(w.x, w.y);
           if constexpr (KEEP_ROUNDING) {
@@ -509,7 +538,12 @@ __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(c
         sum.z += v.x;
         sum.w += v.y;
       }
-      if (whole) {
+      if constexpr (CLUSTER) {                       // the CTA's part, at the places that only this thread reads
+        float* const to = merge + row * SH::MERGE_ROW + at;
+        *reinterpret_cast<float2*>(to) = make_float2(sum.x, sum.y);
+        *reinterpret_cast<float2*>(to + 16) = make_float2(sum.z, sum.w);
+        if (quad == 0) cta_ml[row] = make_float4(m, weight, 0.0f, 0.0f);
+      } else if (whole) {
         const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
         T* const dst = reinterpret_cast<T*>(a.out) + ((long long)(c.s.q0 + j) * a.q_heads + c.head * a.each + r - j * a.each) * D + 4 * quad;
         T v[4] = {from_float<T>(sum.x * inv), from_float<T>(sum.y * inv), from_float<T>(sum.z * inv), from_float<T>(sum.w * inv)};
@@ -519,15 +553,41 @@ __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(c
         if (quad == 0) a.part_ml[(long long)slot * ROWS + row] = make_float2(m, weight);
       }
     }
-    __syncthreads();
+    if constexpr (CLUSTER) {
+      cluster_arrive_release();
+      cluster_wait_acquire();
+      const unsigned rank = cluster_ctarank(), size = cluster_nctarank();
+      for (int i = tid + rank * (W * 32); i < ROWS * (D / 2); i += size * (W * 32)) {
+        const int row = i / (D / 2), pair = i % (D / 2);               // channels 2 pair, 2 pair + 1: pair j of lane g's channels at 16 j + 2 g
+        if (c.tile * ROWS + row >= a.each) continue;
+        const uint32_t value_at = smem_addr(merge + row * SH::MERGE_ROW + pair % (D / 16) * 16 + pair / (D / 16) * 2), ml_at = smem_addr(cta_ml + row);
+        float m = -CUDART_INF_F, weight = 0.0f;
+        for (unsigned x = 0; x < size; ++x) m = fmaxf(m, ld_cluster_f2(cluster_map(ml_at, x)).x);
+        float2 sum = make_float2(0.0f, 0.0f);
+        for (unsigned x = 0; x < size; ++x) {
+          const float2 st = ld_cluster_f2(cluster_map(ml_at, x)), v = ld_cluster_f2(cluster_map(value_at, x));
+          const float by = st.x == m ? 1.0f : exp2_fast(st.x - m);
+          weight = fmaf(st.y, by, weight);
+          sum.x = fmaf(v.x, by, sum.x);
+          sum.y = fmaf(v.y, by, sum.y);
+        }
+        const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
+        T v[2] = {from_float<T>(sum.x * inv), from_float<T>(sum.y * inv)};
+        *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + ((long long)c.s.q0 * a.q_heads + c.head * a.each + c.tile * ROWS + row) * D + 2 * pair) = *reinterpret_cast<const uint32_t*>(v);
+      }
+      cluster_arrive_relaxed();                      // nobody leaves while its shared memory is read
+      cluster_wait_acquire();
+    }
+    stats = stats == stats0 ? stats0 + W * ROWS : stats0;
   };
 
   int stage = 0;
   bool opens = true;
   int from_unit = 0;
+  if constexpr (CLUSTER) start_item();
 #pragma unroll 1
   for (unsigned u = u0; u < u1; ++u) {
-    if (opens) {
+    if (!CLUSTER && opens) {
       start_item();
       from_unit = c.unit;
       opens = false;
@@ -540,50 +600,55 @@ __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(c
       }
       phases ^= 1u << stage;
       const int tok0 = c.s.first + ((c.unit - SH::OPENING) * W + warp) * CT;
-      if (!dead) {
-        if (mask == all_pieces && tok0 + CT - 1 <= full_hi && tok0 >= full_lo)
-          chunk(std::true_type(), ring + stage * SH::STAGE, tok0, mask);
-        else
-          chunk(std::false_type(), ring + stage * SH::STAGE, tok0, mask);
-      }
+      if (!dead) chunk(ring + stage * SH::STAGE, tok0, mask, mask == all_pieces && tok0 + CT - 1 <= full_hi && tok0 >= full_lo);
       __syncwarp();
     }
     issue(stage);
     look_up();
     stage = stage + 1 == S ? 0 : stage + 1;
-    const bool ends = c.unit + 1 == c.s.units;
-    if (ends || u + 1 == u1) {
-      finish_item(ends && from_unit == 0, 2 * blockIdx.x + (from_unit == 0 ? 1 : 0));
-      opens = true;
+    if constexpr (CLUSTER) {
+      ++c.unit;
+    } else {
+      const bool ends = c.unit + 1 == c.s.units;
+      if (ends || u + 1 == u1) {
+        finish_item(ends && from_unit == 0, 2 * blockIdx.x + (from_unit == 0 ? 1 : 0));
+        opens = true;
+      }
+      advance<SH>(a, c);
     }
-    advance<SH>(a, c);
   }
+  if constexpr (CLUSTER) finish_item(false, 0);
 }
 
-// Joins the parts of an item that several CTAs of the kernel above worked on: one block per item and row.
+// Joins the items that a boundary between two CTAs of the kernel above runs through: block (x, y) for boundary x + 1 and two rows, if it is the first in
+// its item.
+constexpr int kJoinWarps = 4, kJoinRows = 2;      // warps of a row, rows of a block
 template <typename T, typename SH>
-__global__ void __launch_bounds__(128) kv4_attention_join_kernel(const AttnArgs a, unsigned ctas) {
+__global__ void __launch_bounds__(kJoinRows * kJoinWarps * 32) kv4_attention_join_kernel(const AttnArgs a, unsigned ctas) {
   constexpr int D = SH::D, ROWS = SH::ROWS, PER = D / 32;
-  __shared__ float sums[4][D];
-  __shared__ float2 ml[4];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y;
+  __shared__ float all_sums[kJoinRows][kJoinWarps][D];
+  __shared__ float2 all_ml[kJoinRows][kJoinWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32 % kJoinWarps, half = threadIdx.x / (32 * kJoinWarps), row = blockIdx.y * kJoinRows + half;
+  float(*const sums)[D] = all_sums[half];
+  float2* const ml = all_ml[half];
   grid_launch_dependents();
   grid_dependency_wait();
-  Sequence mine = {};
-  const Deal deal_ = deal<SH>(a, lane, ctas, mine);
-  Walk w;
-  unsigned u0 = 0;
-  if (!place<SH>(a, lane, mine, blockIdx.x, true, w, u0)) return;
-  const int r = w.tile * ROWS + row, j = r / a.each;
-  if (j >= w.s.nq) return;
-  const int i0 = (int)deal_.owner(u0), i1 = (int)deal_.owner(u0 + w.s.units - 1);
-  if (i0 == i1) return;                        // one CTA had it all and has written it
+  const int4 p = a.plan[blockIdx.x + 1], w = a.plan[ctas + blockIdx.x + 1];       // total, unit, units, head | sequence, tile, first query, queries
+  if (p.y == 0) return;
+  const int r = w.y * ROWS + row, j = r / a.each;
+  Deal d;
+  d.total = (unsigned)p.x;
+  d.each = d.total / ctas;
+  d.more = d.total - d.each * ctas;
+  const unsigned u0 = d.start(blockIdx.x + 1) - (unsigned)p.y;                    // the item's first unit
+  const int i0 = (int)d.owner(u0), i1 = (int)d.owner(u0 + (unsigned)p.z - 1);
+  if (i0 != (int)blockIdx.x) return;
   float m = -CUDART_INF_F, weight = 0.0f;
   float sum[PER];
 #pragma unroll
   for (int e = 0; e < PER; ++e) sum[e] = 0.0f;
-  for (int i = i0 + warp; i <= i1; i += 4) {
-    const int slot = 2 * i + (deal_.start(i) > u0 ? 0 : 1);
+  for (int i = j < w.w ? i0 + warp : i1 + 1; i <= i1; i += kJoinWarps) {
+    const int slot = 2 * i + (d.start(i) > u0 ? 0 : 1);
     const float2 s = a.part_ml[(long long)slot * ROWS + row];
     float v[PER];
     const float* src = a.part_o + ((long long)slot * ROWS + row) * D + lane * PER;
@@ -601,23 +666,25 @@ __global__ void __launch_bounds__(128) kv4_attention_join_kernel(const AttnArgs 
   for (int e = 0; e < PER; ++e) sums[warp][lane * PER + e] = sum[e];
   if (lane == 0) ml[warp] = make_float2(m, weight);
   __syncthreads();
-  for (int d = threadIdx.x; d < D; d += 128) {
+  if (j >= w.w) return;
+  for (int at = threadIdx.x % (kJoinWarps * 32); at < D; at += kJoinWarps * 32) {
     float top = -CUDART_INF_F, all = 0.0f, value = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = fmaxf(top, ml[i].x);
-    if (top != -CUDART_INF_F) {
+    for (int i = 0; i < kJoinWarps; ++i) top = fmaxf(top, ml[i].x);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float by = exp2_fast(ml[i].x - top);
-        all = fmaf(ml[i].y, by, all);
-        value = fmaf(sums[i][d], by, value);
-      }
+    for (int i = 0; i < kJoinWarps; ++i) {
+      const float by = ml[i].x == top ? 1.0f : exp2_fast(ml[i].x - top);
+      all = fmaf(ml[i].y, by, all);
+      value = fmaf(sums[i][at], by, value);
     }
-    reinterpret_cast<T*>(a.out)[((long long)(w.s.q0 + j) * a.q_heads + w.head * a.each + r - j * a.each) * D + d] =
-        from_float<T>(all == 0.0f ? 0.0f : value / all);
+    reinterpret_cast<T*>(a.out)[((long long)(w.z + j) * a.q_heads + p.w * a.each + r - j * a.each) * D + at] = from_float<T>(all == 0.0f ? 0.0f : value / all);
   }
 }
 
+#ifndef CLMAX
+#define CLMAX 1LL
+#define CLUNITS 4
+#endif
 constexpr int kFewRows = 32;      // rows for a key head up to which a sequence stays with this file's kernel
 constexpr int kMostPerSm = 2;      // CTAs of any shape on an SM
 
@@ -631,6 +698,17 @@ template <typename T, int D, int NT>
 int run(AttnArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
   using SH = Few<D, NT>;
   static_assert((SH::SMEM + 1024) * SH::PER_SM <= 228 * 1024 && SH::PER_SM <= kMostPerSm, "resident together");
+  if (!a.query_starts) {
+    // Few single tokens with few keys: a cluster for each item, which needs neither the list nor the second kernel.
+    const long long items = (long long)a.batch * ceil_div(a.each, SH::ROWS) * a.kv_heads, keys = (long long)a.table_width << a.page_shift;
+    const long long units = ((a.window ? min(keys, (long long)a.window + SH::CT) : keys) + SH::UNIT - 1) / SH::UNIT;
+    int size = 8;
+    while (size > 1 && (items * size > (long long)SH::PER_SM * sm_count() || size >= 2 * units)) size >>= 1;
+    if (items * size <= CLMAX * SH::PER_SM * sm_count() && units <= CLUNITS * size) {
+      XQT_SMEM_OPT_IN((kv4_attention_kernel<T, SH, true>), SH::SMEM);
+      return launch_pdl_cluster(kv4_attention_kernel<T, SH, true>, dim3((unsigned)(items * size)), dim3(SH::W * 32), size, SH::SMEM, stream, a);
+    }
+  }
   // as many items as there can be: full tiles, and one that is not full per sequence
   const long long most_rows = a.query_starts ? a.few_rows : a.each;
   const long long tiles = min((long long)a.tokens * a.each / SH::ROWS + a.batch, a.batch * ((most_rows + SH::ROWS - 1) / SH::ROWS));
@@ -638,13 +716,14 @@ int run(AttnArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream
   XQT_REQUIRE(items < (1LL << 31) - 1 && units < (1LL << 31));
   const int ctas = (int)min((long long)SH::PER_SM * sm_count(), units);
   const size_t o_bytes = (size_t)2 * ctas * SH::ROWS * D * 4;
-  XQT_REQUIRE(workspace && workspace_bytes >= o_bytes + (size_t)2 * ctas * SH::ROWS * 8 && ((uintptr_t)workspace & 15) == 0);
+  XQT_REQUIRE(workspace && workspace_bytes >= o_bytes + (size_t)2 * ctas * (SH::ROWS * 8 + 16) && ((uintptr_t)workspace & 15) == 0);
   a.part_o = reinterpret_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>((uint8_t*)workspace + o_bytes);
-  XQT_SMEM_OPT_IN((kv4_attention_kernel<T, SH>), SH::SMEM);
-  int rc = launch_pdl(kv4_attention_kernel<T, SH>, dim3((unsigned)ctas), dim3(SH::W * 32), SH::SMEM, stream, a);
-  if (rc) return rc;
-  return launch_pdl(kv4_attention_join_kernel<T, SH>, dim3((unsigned)items, SH::ROWS), dim3(128), 0, stream, a, (unsigned)ctas);
+  a.plan = reinterpret_cast<int4*>(a.part_ml + (size_t)2 * ctas * SH::ROWS);
+  XQT_SMEM_OPT_IN((kv4_attention_kernel<T, SH, false>), SH::SMEM);
+  int rc = launch_pdl(kv4_attention_kernel<T, SH, false>, dim3((unsigned)ctas), dim3(SH::W * 32), SH::SMEM, stream, a);
+  if (rc || ctas == 1) return rc;
+  return launch_pdl(kv4_attention_join_kernel<T, SH>, dim3((unsigned)ctas - 1, SH::ROWS / kJoinRows), dim3(kJoinRows * kJoinWarps * 32), 0, stream, a, (unsigned)ctas);
 }
 
 template <typename T>
@@ -662,7 +741,7 @@ int run_dim(const AttnArgs& a, int dim, void* workspace, size_t workspace_bytes,
 extern "C" size_t xqt_b200_kv4_attention_workspace_bytes(int tokens, int batch, int q_heads, int kv_heads, int dim, int has_query_starts) {
   using namespace xqt_b200;
   (void)batch;
-  const size_t few = (size_t)2 * kMostPerSm * sm_count() * 16 * (dim + 2) * 4;
+  const size_t few = (size_t)2 * kMostPerSm * sm_count() * (16 * (dim + 2) * 4 + 16);
   // the two kernels run one after the other and share it
   if (!has_query_starts || kv_heads < 1 || (long long)tokens * (q_heads / kv_heads) <= kFewRows) return few;
   const size_t prompt = kv4_prompt_workspace_bytes(dim);

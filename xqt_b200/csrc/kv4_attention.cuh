@@ -24,7 +24,7 @@ struct AttnArgs {
   void* out;
   float* part_o;             // [2 * CTAs][ROWS][D]
   float2* part_ml;           // [2 * CTAs][ROWS]
-  int4* plan;                // prompt kernel: where each CTA begins
+  int4* plan;                // [2 * CTAs] where each CTA begins
   unsigned* status;
   long long q_token, q_head, pages, table_stride;
   int tokens, batch, q_heads, kv_heads, each, page_size, page_shift, table_width, window, few_rows;     // few_rows: sequences with more rows for a key head go to the prompt kernel
@@ -112,39 +112,43 @@ __device__ __forceinline__ Deal deal(const AttnArgs& a, int lane, unsigned ctas,
   return d;
 }
 
-// The place of unit `u`, or with by_item of item (tile, head) number `u`; `before` gets the units in front of it.
+// the sequence that lane `lane` has
+__device__ __forceinline__ Sequence sequence_of(const Sequence& s, int lane) {
+  Sequence r;
+  r.q0 = __shfl_sync(0xffffffffu, s.q0, lane);
+  r.nq = __shfl_sync(0xffffffffu, s.nq, lane);
+  r.len = __shfl_sync(0xffffffffu, s.len, lane);
+  r.first = __shfl_sync(0xffffffffu, s.first, lane);
+  r.tiles = __shfl_sync(0xffffffffu, s.tiles, lane);
+  r.units = __shfl_sync(0xffffffffu, s.units, lane);
+  return r;
+}
+
+// The place of unit `u`.
 template <typename L>
-__device__ __forceinline__ bool place(const AttnArgs& a, int lane, const Sequence& mine, unsigned u, bool by_item, Walk& w, unsigned& before) {
-  unsigned base = 0, base_units = 0;
+__device__ __forceinline__ bool place(const AttnArgs& a, int lane, const Sequence& mine, unsigned u, Walk& w) {
+  unsigned base = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
     Sequence s = mine;
-    unsigned items = 0, units = 0;
+    unsigned units = 0;
     if (b0 + lane < a.batch) {
       if (b0 > 0) s = sequence<L>(a, b0 + lane);
-      items = (unsigned)s.tiles * a.kv_heads;
-      units = items * s.units;
+      units = (unsigned)s.tiles * a.kv_heads * s.units;
     }
-    const unsigned cum_units = scan32(units, lane), n = by_item ? items : units, cum = by_item ? scan32(items, lane) : cum_units;
+    const unsigned cum = scan32(units, lane);
     const unsigned over = __ballot_sync(0xffffffffu, base + cum > u);
     if (over) {
       const int at = __ffs(over) - 1;
-      const unsigned rest = u - base - __shfl_sync(0xffffffffu, cum - n, at);
+      const unsigned rest = u - base - __shfl_sync(0xffffffffu, cum - units, at);
       w.b = b0 + at;
-      w.s.q0 = __shfl_sync(0xffffffffu, s.q0, at);
-      w.s.nq = __shfl_sync(0xffffffffu, s.nq, at);
-      w.s.len = __shfl_sync(0xffffffffu, s.len, at);
-      w.s.first = __shfl_sync(0xffffffffu, s.first, at);
-      w.s.tiles = __shfl_sync(0xffffffffu, s.tiles, at);
-      w.s.units = __shfl_sync(0xffffffffu, s.units, at);
-      const unsigned item = by_item ? rest : rest / (unsigned)w.s.units;
-      w.unit = by_item ? 0 : (int)(rest - item * w.s.units);
+      w.s = sequence_of(s, at);
+      const unsigned item = rest / (unsigned)w.s.units;
+      w.unit = (int)(rest - item * w.s.units);
       w.tile = (int)(item / (unsigned)a.kv_heads);
       w.head = (int)(item - (unsigned)w.tile * a.kv_heads);
-      before = base_units + __shfl_sync(0xffffffffu, cum_units - units, at) + item * w.s.units;
       return true;
     }
     base += __shfl_sync(0xffffffffu, cum, 31);
-    base_units += __shfl_sync(0xffffffffu, cum_units, 31);
   }
   return false;
 }

@@ -222,17 +222,6 @@ __device__ __forceinline__ int prompt_chunks(const AttnArgs& a, const Sequence& 
   return end > begin ? (end - begin + SH::BN - 1) / SH::BN : 0;
 }
 
-__device__ __forceinline__ Sequence sequence_of(const Sequence& s, int lane) {
-  Sequence r;
-  r.q0 = __shfl_sync(0xffffffffu, s.q0, lane);
-  r.nq = __shfl_sync(0xffffffffu, s.nq, lane);
-  r.len = __shfl_sync(0xffffffffu, s.len, lane);
-  r.first = __shfl_sync(0xffffffffu, s.first, lane);
-  r.tiles = __shfl_sync(0xffffffffu, s.tiles, lane);
-  r.units = __shfl_sync(0xffffffffu, s.units, lane);
-  return r;
-}
-
 // Goes through the tiles of all sequences, 32 at a time, and calls visit(b, sequence, first tile, this lane's units) until it says to stop;
 // one warp.
 template <typename SH, typename V>

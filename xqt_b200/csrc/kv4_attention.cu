@@ -55,7 +55,7 @@ struct Shape {
   static constexpr bool PROMPT = false;
   static constexpr int CODE_BYTES = CT * KROW, PARAM_BYTES = CT * 4, STAGE = 2 * (CODE_BYTES + PARAM_BYTES);
   static constexpr int MERGE_ROW = D + 8;
-  static constexpr int MERGES = W / 2;                    // buffers: the warps write them in two rounds
+  static constexpr int MERGES = W / 2;                    // buffers: the warps add to them in rounds
   static constexpr int MERGE_BYTES = MERGES * ROWS * MERGE_ROW * 4, STAT_BYTES = (2 * W + 1) * ROWS * 16;      // the warps' statistics twice: an item's are written while the last one's are read
   static constexpr int SMEM = W * S * STAGE + MERGE_BYTES + STAT_BYTES + W * S * 8;
 };
@@ -80,7 +80,7 @@ __device__ __forceinline__ float2 ld_cluster_f2(uint32_t caddr) {
   return v;
 }
 
-// CLUSTER: single tokens; a cluster of CTAs takes one item, each an equal run of its units, and joins it through distributed shared memory.
+// CLUSTER: a cluster of CTAs takes one item, each an equal run of its units, and joins it through distributed shared memory.
 template <typename T, typename SH, bool CLUSTER>
 __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(const AttnArgs a) {
   constexpr int D = SH::D, NT = SH::NT, W = SH::W, CT = SH::CT, S = SH::S, ROWS = SH::ROWS, MT = SH::MT, KROW = SH::KROW;
@@ -104,12 +104,8 @@ __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(c
   Walk c;
   unsigned u0 = 0, u1;
   if constexpr (CLUSTER) {
-    const unsigned rank = cluster_ctarank(), size = cluster_nctarank(), item = blockIdx.x / size;
-    const unsigned tiles = (unsigned)(a.each + ROWS - 1) / ROWS, of_sequence = item / a.kv_heads;
-    c.head = (int)(item - of_sequence * a.kv_heads);
-    c.b = (int)(of_sequence / tiles);
-    c.tile = (int)(of_sequence - c.b * tiles);
-    c.s = sequence<SH>(a, c.b);
+    const unsigned rank = cluster_ctarank(), size = cluster_nctarank();
+    if (!place_item<SH>(a, lane, blockIdx.x / size, c)) return;        // (all of the cluster)
     const unsigned units = (unsigned)(c.s.units - SH::OPENING), lo = units * rank / size;
     c.unit = SH::OPENING + (int)lo;
     u1 = units * (rank + 1) / size - lo;
@@ -487,7 +483,7 @@ __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(c
     }
     __syncthreads();
 #pragma unroll 1
-    for (int round = 0; round < 2; ++round) {
+    for (int round = 0; round < W / SH::MERGES; ++round) {
       if (warp / SH::MERGES == round) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -559,7 +555,8 @@ __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(c
       const unsigned rank = cluster_ctarank(), size = cluster_nctarank();
       for (int i = tid + rank * (W * 32); i < ROWS * (D / 2); i += size * (W * 32)) {
         const int row = i / (D / 2), pair = i % (D / 2);               // channels 2 pair, 2 pair + 1: pair j of lane g's channels at 16 j + 2 g
-        if (c.tile * ROWS + row >= a.each) continue;
+        const int r = c.tile * ROWS + row, j = r / a.each;
+        if (j >= c.s.nq) continue;
         const uint32_t value_at = smem_addr(merge + row * SH::MERGE_ROW + pair % (D / 16) * 16 + pair / (D / 16) * 2), ml_at = smem_addr(cta_ml + row);
         float m = -CUDART_INF_F, weight = 0.0f;
         for (unsigned x = 0; x < size; ++x) m = fmaxf(m, ld_cluster_f2(cluster_map(ml_at, x)).x);
@@ -573,7 +570,7 @@ __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(c
         }
         const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
         T v[2] = {from_float<T>(sum.x * inv), from_float<T>(sum.y * inv)};
-        *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + ((long long)c.s.q0 * a.q_heads + c.head * a.each + c.tile * ROWS + row) * D + 2 * pair) = *reinterpret_cast<const uint32_t*>(v);
+        *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + ((long long)(c.s.q0 + j) * a.q_heads + c.head * a.each + r - j * a.each) * D + 2 * pair) = *reinterpret_cast<const uint32_t*>(v);
       }
       cluster_arrive_relaxed();                      // nobody leaves while its shared memory is read
       cluster_wait_acquire();
@@ -681,10 +678,6 @@ __global__ void __launch_bounds__(kJoinRows * kJoinWarps * 32) kv4_attention_joi
   }
 }
 
-#ifndef CLMAX
-#define CLMAX 1LL
-#define CLUNITS 4
-#endif
 constexpr int kFewRows = 32;      // rows for a key head up to which a sequence stays with this file's kernel
 constexpr int kMostPerSm = 2;      // CTAs of any shape on an SM
 
@@ -698,22 +691,22 @@ template <typename T, int D, int NT>
 int run(AttnArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
   using SH = Few<D, NT>;
   static_assert((SH::SMEM + 1024) * SH::PER_SM <= 228 * 1024 && SH::PER_SM <= kMostPerSm, "resident together");
-  if (!a.query_starts) {
-    // Few single tokens with few keys: a cluster for each item, which needs neither the list nor the second kernel.
-    const long long items = (long long)a.batch * ceil_div(a.each, SH::ROWS) * a.kv_heads, keys = (long long)a.table_width << a.page_shift;
-    const long long units = ((a.window ? min(keys, (long long)a.window + SH::CT) : keys) + SH::UNIT - 1) / SH::UNIT;
-    int size = 8;
-    while (size > 1 && (items * size > (long long)SH::PER_SM * sm_count() || size >= 2 * units)) size >>= 1;
-    if (items * size <= CLMAX * SH::PER_SM * sm_count() && units <= CLUNITS * size) {
-      XQT_SMEM_OPT_IN((kv4_attention_kernel<T, SH, true>), SH::SMEM);
-      return launch_pdl_cluster(kv4_attention_kernel<T, SH, true>, dim3((unsigned)(items * size)), dim3(SH::W * 32), size, SH::SMEM, stream, a);
-    }
-  }
   // as many items as there can be: full tiles, and one that is not full per sequence
   const long long most_rows = a.query_starts ? a.few_rows : a.each;
   const long long tiles = min((long long)a.tokens * a.each / SH::ROWS + a.batch, a.batch * ((most_rows + SH::ROWS - 1) / SH::ROWS));
   const long long items = tiles * a.kv_heads, units = items * (((long long)a.table_width << a.page_shift) / SH::UNIT + 1 + SH::OPENING);
   XQT_REQUIRE(items < (1LL << 31) - 1 && units < (1LL << 31));
+  // Few items with few keys: a cluster for each, which needs neither the list nor the second kernel (cluster | list: one sequence of 777 keys 6.6 |
+  // 9.0 us, 64 of 500 18 | 21).  Where items of many keys do not fill the SMs, or there are many items, the list's even shares win (two of 131,071
+  // keys, eight heads: 125 | 71; 64 up to 8192: 95 | 82).
+  const long long keys = (long long)a.table_width << a.page_shift, seen = a.window ? min(keys, (long long)a.window + min(most_rows / a.each, (long long)a.tokens) + SH::CT) : keys;
+  const long long of_item = (seen + SH::UNIT - 1) / SH::UNIT;
+  int size = 8;
+  while (size > 1 && (items * size > (long long)SH::PER_SM * sm_count() || size >= 2 * of_item)) size >>= 1;
+  if (items * size <= 4LL * SH::PER_SM * sm_count() && of_item <= 8 * size) {
+    XQT_SMEM_OPT_IN((kv4_attention_kernel<T, SH, true>), SH::SMEM);
+    return launch_pdl_cluster(kv4_attention_kernel<T, SH, true>, dim3((unsigned)(items * size)), dim3(SH::W * 32), size, SH::SMEM, stream, a);
+  }
   const int ctas = (int)min((long long)SH::PER_SM * sm_count(), units);
   const size_t o_bytes = (size_t)2 * ctas * SH::ROWS * D * 4;
   XQT_REQUIRE(workspace && workspace_bytes >= o_bytes + (size_t)2 * ctas * (SH::ROWS * 8 + 16) && ((uintptr_t)workspace & 15) == 0);

@@ -153,6 +153,37 @@ __device__ __forceinline__ bool place(const AttnArgs& a, int lane, const Sequenc
   return false;
 }
 
+// Item (tile, head) number `item` of the list.
+template <typename L>
+__device__ __forceinline__ bool place_item(const AttnArgs& a, int lane, unsigned item, Walk& w) {
+  if (!a.query_starts) {                             // the same number of items in each sequence
+    const unsigned tiles = (unsigned)(a.each + L::ROWS - 1) / L::ROWS, of_sequence = item / (unsigned)a.kv_heads;
+    w.head = (int)(item - of_sequence * a.kv_heads);
+    w.b = (int)(of_sequence / tiles);
+    w.tile = (int)(of_sequence - w.b * tiles);
+    w.s = sequence<L>(a, w.b);
+    return true;
+  }
+  unsigned base = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 32) {
+    Sequence s = {};
+    if (b0 + lane < a.batch) s = sequence<L>(a, b0 + lane);
+    const unsigned items = (unsigned)s.tiles * a.kv_heads, cum = scan32(items, lane);
+    const unsigned over = __ballot_sync(0xffffffffu, base + cum > item);
+    if (over) {
+      const int at = __ffs(over) - 1;
+      const unsigned rest = item - base - __shfl_sync(0xffffffffu, cum - items, at);
+      w.b = b0 + at;
+      w.s = sequence_of(s, at);
+      w.tile = (int)(rest / (unsigned)a.kv_heads);
+      w.head = (int)(rest - (unsigned)w.tile * a.kv_heads);
+      return true;
+    }
+    base += __shfl_sync(0xffffffffu, cum, 31);
+  }
+  return false;
+}
+
 }  // namespace kv4
 
 int kv4_prompt_launch(const kv4::AttnArgs& a, int dim, int dtype, void* workspace, size_t bytes, cudaStream_t stream);

@@ -124,6 +124,19 @@ def test_entries_check_their_arguments_before_any_cuda_call():
     assert append(dim=96) == 1 and append(tokens=-1) == 1 and append(heads=0) == 1 and append() == 1 and append(tokens=0) == 0
 
 
+def test_native_path_leaves_to_python_what_it_does_not_take():
+    host = native.attention_host()
+    codes, params = allocate_kv4_cache(2, 2, 64, page_size=16, dtype=torch.float16)
+    x, slots = torch.zeros(3, 2, 64, dtype=torch.float16), torch.arange(3)
+    table, lens = torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    assert host.kv4_append(x, x, codes, params, slots) is None and host.kv4_append(x, x) is None and host.kv4_append(None, x, codes, params, slots) is None
+    assert host.kv4_gather(codes, params, slots) is None and host.kv4_gather(codes, 1, slots) is None
+    assert host.kv4_attention(x, codes, params, table, lens, None, None, None, None) is None
+    assert host.qk_norm_rope(x, None, slots, rotary_frequencies(64)[0], None, None, None, 1e-6, False) is None
+    with pytest.raises(TypeError):
+        host.qk_norm_rope(x, None, slots, rotary_frequencies(64)[0], None, None, None, "eps", False)
+
+
 def test_definition_of_the_codes():
     x = torch.randn((7, 64), generator=seeded(1)).bfloat16()
     codes, scale, low = quantize(x)

@@ -453,6 +453,61 @@ def test_same_prompt_bits_every_time():
         assert torch.equal(kv4_attention(q, codes, params, wide(table, 64), seq_lens, query_starts=starts), first)
 
 
+def test_native_path_and_python_path_give_the_same():
+    from xqt_b200.ops import kv4, rotary
+
+    lens = [300, 77]
+    codes, params, table = make_cache(lens, 2, 128, 32, torch.bfloat16, 68)
+    x = _vectors(2, 12, 128, torch.bfloat16, 69).to(DEVICE)
+    seq_lens, slots, positions = torch.tensor(lens, dtype=torch.int32, device=DEVICE), torch.tensor([5, 40], device=DEVICE), torch.tensor([299, 76], device=DEVICE)
+    frequencies, weight = rotary.rotary_frequencies(128, device=DEVICE)[0], torch.rand(128, generator=seeded(70)).to(DEVICE)
+
+    def run():
+        q, k = rotary.qk_norm_rope(x[:, :8], x[:, 8:10], positions, frequencies, q_weight=weight, k_weight=weight, interleaved=True)
+        cache = [t.clone() for t in (codes, params)]
+        kv4_append(k, x[:, 10:], *cache, slots)
+        return (q, k, *cache, *kv4_gather(*cache, slots), kv4_attention(q, *cache, table, seq_lens, window=50, scale=0.1))
+
+    run()
+    assert kv4._native is not None and rotary._native is not None
+    fast = run()
+    kv4._native = rotary._native = None
+    for a, b in zip(fast, run()):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+_FIRST_CALL_IN_A_CAPTURE = """
+import os, sys
+sys.path.insert(0, os.environ["XQT_ROOT"]); sys.path.insert(0, os.path.join(os.environ["XQT_ROOT"], "tests"))
+import torch
+from test_kv4_gpu import DEVICE, _vectors, make_cache, wide
+from xqt_b200 import native
+from xqt_b200.ops.kv4 import kv4_attention
+codes, params, table = make_cache([200, 90], 2, 128, 32, torch.bfloat16, 1)
+q = _vectors(160, 8, 128, torch.bfloat16, 2).to(DEVICE)
+lens, starts = (torch.tensor(x, dtype=torch.int32, device=DEVICE) for x in ([200, 90], [0, 100, 160]))
+graph = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(graph):
+    held = kv4_attention(q, codes, params, wide(table, 32), lens, query_starts=starts), kv4_attention(q[:2], codes, params, table, lens)
+graph.replay()
+want = kv4_attention(q, codes, params, wide(table, 32), lens, query_starts=starts), kv4_attention(q[:2], codes, params, table, lens)
+assert torch.equal(held[0], want[0]) and torch.equal(held[1], want[1]) and native.workspace_status(DEVICE) == 0
+print("the same")
+"""
+
+
+def test_first_call_of_a_process_in_a_capture():
+    import os
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+
+    done = subprocess.run([sys.executable, "-c", _FIRST_CALL_IN_A_CAPTURE], env={**os.environ, "XQT_ROOT": str(ROOT)}, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "the same" in done.stdout, done.stderr[-2000:]
+
+
 def test_many_short_sequences():
     lens = [(7 * i) % 50 for i in range(700)]
     codes, params, table = make_cache(lens, 1, 64, 16, torch.float16, 41)

@@ -236,6 +236,16 @@ def status_word(device: torch.device) -> torch.Tensor:
     return word
 
 
+def status_pointer(device: torch.device) -> int:
+    """Address of :func:`status_word`; 0 (no status) in a graph capture that finds none yet: what a capture allocates is its own, and not zeroed
+    before a replay."""
+
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    if index not in _status_words and torch.cuda.is_current_stream_capturing():
+        return 0
+    return status_word(device).data_ptr()
+
+
 def workspace_status(device: torch.device) -> int:
     """Worst status word of the current stream's scratch buffers and of the device's status word
     (0 = every bounded wait completed)."""
@@ -258,5 +268,5 @@ def workspace_status(device: torch.device) -> int:
 
 __all__ = [
     "ACT", "AUTO_INTEGER", "BF16", "DTYPE_CODE", "FP16", "FP32", "LIBRARY_PATH", "SIGNATURES", "VARIANT", "VARIANT_NAMES",
-    "attention_host", "available", "check", "host", "library", "ptr", "status_word", "stream_handle", "version", "workspace", "workspace_status",
+    "attention_host", "available", "check", "host", "library", "ptr", "status_pointer", "status_word", "stream_handle", "version", "workspace", "workspace_status",
 ]

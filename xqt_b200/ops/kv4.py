@@ -166,7 +166,7 @@ def kv4_attention(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, bl
                 q.data_ptr(), codes.data_ptr(), params.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), native.ptr(query_starts), out.data_ptr(),
                 _Strides(*_steps(q), block_table.stride(0), 0), tokens, batch, q_heads, kv_heads, dim, pages, page_size, width,
                 0 if window is None else min(int(window), 2 ** 31 - 1), native.DTYPE_CODE[q.dtype], scale, workspace.data_ptr(), need,
-                native.status_word(device).data_ptr(), native.stream_handle(device))
+                native.status_pointer(device), native.stream_handle(device))
         native.check(code, "xqt_b200_kv4_attention")
         _native = native.attention_host()
     return out

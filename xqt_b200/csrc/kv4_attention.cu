@@ -644,21 +644,7 @@ __global__ void __launch_bounds__(kJoinRows * kJoinWarps * 32) kv4_attention_joi
   float sum[PER];
 #pragma unroll
   for (int e = 0; e < PER; ++e) sum[e] = 0.0f;
-  for (int i = j < w.w ? i0 + warp : i1 + 1; i <= i1; i += kJoinWarps) {
-    const int slot = 2 * i + (d.start(i) > u0 ? 0 : 1);
-    const float2 s = a.part_ml[(long long)slot * ROWS + row];
-    float v[PER];
-    const float* src = a.part_o + ((long long)slot * ROWS + row) * D + lane * PER;
-#pragma unroll
-    for (int e = 0; e < PER; e += 2) *reinterpret_cast<float2*>(v + e) = *reinterpret_cast<const float2*>(src + e);
-    if (s.y == 0.0f) continue;                 // it saw nothing (a NaN has no maximum, but a weight)
-    const float top = fmaxf(m, s.x);
-    const float keep = m == top ? 1.0f : exp2_fast(m - top), by = exp2_fast(s.x - top);
-    m = top;
-    weight = fmaf(s.y, by, weight * keep);
-#pragma unroll
-    for (int e = 0; e < PER; ++e) sum[e] = fmaf(v[e], by, sum[e] * keep);
-  }
+  join_parts<D>(a, ROWS, row, j < w.w ? i0 + warp : i1 + 1, i1, kJoinWarps, d, u0, m, weight, sum);
 #pragma unroll
   for (int e = 0; e < PER; ++e) sums[warp][lane * PER + e] = sum[e];
   if (lane == 0) ml[warp] = make_float2(m, weight);

@@ -184,6 +184,39 @@ __device__ __forceinline__ bool place_item(const AttnArgs& a, int lane, unsigned
   return false;
 }
 
+// Adds up row `row` of the parts of an item (first unit u0) that CTAs first, first + step, .. last hold, for the lane's D / 32 channels, four parts
+// in flight.  A part that saw nothing has weight 0, and its sums were never written.
+template <int D>
+__device__ __forceinline__ void join_parts(const AttnArgs& a, int rows, int row, int first, int last, int step, const Deal& d, unsigned u0, float& m, float& weight,
+                                           float (&sum)[D / 32]) {
+  constexpr int PER = D / 32;
+  const int lane = threadIdx.x & 31;
+  for (int i = first; i <= last; i += 4 * step) {
+    float2 s[4];
+    float v[4][PER];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int cta = i + b * step;
+      s[b] = make_float2(-CUDART_INF_F, 0.0f);
+      if (cta <= last) {
+        const long long at = (2LL * cta + (d.start(cta) > u0 ? 0 : 1)) * rows + row;
+        s[b] = a.part_ml[at];
+#pragma unroll
+        for (int e = 0; e < PER; e += 2) *reinterpret_cast<float2*>(&v[b][e]) = *reinterpret_cast<const float2*>(a.part_o + at * D + lane * PER + e);
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      if (s[b].y == 0.0f) continue;                  // (a NaN has no maximum, but a weight)
+      const float top = fmaxf(m, s[b].x), keep = m == top ? 1.0f : exp2_fast(m - top), by = exp2_fast(s[b].x - top);
+      m = top;
+      weight = fmaf(s[b].y, by, weight * keep);
+#pragma unroll
+      for (int e = 0; e < PER; ++e) sum[e] = fmaf(v[b][e], by, sum[e] * keep);
+    }
+  }
+}
+
 }  // namespace kv4
 
 int kv4_prompt_launch(const kv4::AttnArgs& a, int dim, int dtype, void* workspace, size_t bytes, cudaStream_t stream);

@@ -743,21 +743,7 @@ __global__ void __launch_bounds__(256) kv4_prompt_join_kernel(const AttnArgs a, 
     float m = -CUDART_INF_F, weight = 0.0f, sum[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) sum[e] = 0.0f;
-    for (unsigned i = i0; i <= i1; ++i) {
-      const long long at = (2LL * i + (d.start(i) > u0 ? 0 : 1)) * SH::ROWS + line;
-      const float2 s = a.part_ml[at];
-      if (s.y == 0.0f) continue;                     // it saw nothing, and may have written nothing else
-      const float top = fmaxf(m, s.x), keep = m == top ? 1.0f : exp2_fast(m - top), by = exp2_fast(s.x - top);
-      m = top;
-      weight = fmaf(s.y, by, weight * keep);
-      const float* const src = a.part_o + at * D + lane * PER;
-#pragma unroll
-      for (int e = 0; e < PER; e += 2) {
-        const float2 v = *reinterpret_cast<const float2*>(src + e);
-        sum[e] = fmaf(v.x, by, sum[e] * keep);
-        sum[e + 1] = fmaf(v.y, by, sum[e + 1] * keep);
-      }
-    }
+    join_parts<D>(a, SH::ROWS, line, (int)i0, (int)i1, 1, d, u0, m, weight, sum);
     const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
     T* const out = reinterpret_cast<T*>(a.out) + ((long long)(w.z + j) * a.q_heads + p.w * a.each + row - j * a.each) * D + lane * PER;
 #pragma unroll

@@ -65,6 +65,28 @@ def test_append_of_strided_vectors_and_padded_rows():
     assert all(bool((x[[1, 3, 6, 7]] == 0).all()) for x in got) and bool((got[0][0] != 0).any())
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads", [1, 3, 7])
+def test_append_at_every_magnitude_and_on_half_codes(dtype, heads):
+    """Ranges from the smallest number of the type to its largest, and vectors that stand exactly between two codes."""
+    info = torch.finfo(dtype)
+    low, high = (-24, 11) if dtype == torch.float16 else (-133, 122)
+    grid = torch.cat([torch.tensor([0.0, 30.0]), torch.randint(0, 31, (62,), generator=seeded(41)).float()])     # scale 2: odd ones are halves
+    rows = []
+    for e in range(low, high + 1):
+        rows += [grid.double() * 2.0 ** e, (grid.double() - 13) * 2.0 ** e, torch.randn(64, generator=seeded(900 + e), dtype=torch.float64) * 2.0 ** e]
+    x = torch.stack(rows).clamp(-info.max, info.max).to(dtype)
+    x = x[: len(x) // heads * heads].reshape(-1, heads, 64)
+    tokens = len(x)
+    codes, params = allocate_kv4_cache(tokens // 16 + 1, heads, 64, page_size=16, dtype=dtype, device=DEVICE)
+    slots = torch.arange(tokens)
+    kv4_append(x.to(DEVICE), x.flip(0).to(DEVICE), codes, params, slots.to(DEVICE))
+    for i, y in enumerate((x, x.flip(0))):
+        c, s, m = quantize(y)
+        assert torch.equal(params.cpu()[slots // 16, i, :, slots % 16], torch.stack((s, m), -1))
+        assert torch.equal(codes.cpu()[slots // 16, i, :, slots % 16], pack(c))
+
+
 def test_vectors_that_are_not_finite():
     x = _vectors(5, 1, 64, torch.bfloat16, 5)
     x[1, 0, 3], x[2, 0, 9], x[3, 0, 0] = NAN, INF, -INF

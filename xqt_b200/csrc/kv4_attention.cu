@@ -15,9 +15,13 @@
 // The keys are the 16-row operand and the queries the 8-column one (transposed products), so that eight rows -- the query heads of
 // one key head -- fill a tile.  Work is cut into units of W chunks of CT keys (a chunk per warp); the units of all (sequence, row tile,
 // head) items form one list, of which each CTA takes an equal contiguous share whatever the lengths are; items that
-// CTAs share are joined by a second kernel.  Each warp fetches its own chunks with bulk copies, S of them ahead.
+// CTAs share are joined by a second kernel, or (few items of few keys) by a cluster of CTAs per item in its distributed shared memory.
+// Each warp fetches its own chunks with bulk copies, S of them ahead.
 //
-// Bound by HBM: (dim + 8) bytes per key and head.
+// Its floor is HBM, (dim + 8) bytes per key and head, but it runs at half of that: the loads alone take 52 of 70 us (two documents of 131,071 keys,
+// 64 query heads on 8 of 128 channels: 4.1 TB/s), the arithmetic alone 57 (5 instructions per code word for the operands, ex2 and the sums of
+// a softmax in 8 columns), and two CTAs of four warps, all that the registers allow, do not hide one behind the other completely.
+// 64 sequences of up to 8192 keys, 8 heads: 82 us (3.6 TB/s); one of 777 keys: 7 us, launch and one chain of loads and products.
 #include "kv4_attention.cuh"
 
 namespace xqt_b200 {
@@ -668,8 +672,8 @@ constexpr int kFewRows = 32;      // rows for a key head up to which a sequence 
 constexpr int kMostPerSm = 2;      // CTAs of any shape on an SM
 
 // Two CTAs of four warps on an SM, with all the registers that leaves.  Keys per chunk: 64 for one 8-row tile of up to 128 channels (two
-// documents of 131,071 keys, 64 query heads on 8: 71 us; chunks of 32 keys with three CTAs of 168 registers: 81; with 64 keys, two CTAs of
-// two warps: 78), fewer where the sums of a chunk take more registers.
+// documents of 131,071 keys, 64 query heads on 8: 70 us; three CTAs of 168 registers with chunks of 64 keys: 72, of 32 keys: 83; with 64 keys, two CTAs
+// of two warps: 78), fewer where the sums of a chunk take more registers.
 template <int D, int NT>
 using Few = Shape<D, NT, 4, D == 256 ? 16 : NT == 1 ? 64 : 32, D * NT == 128 ? 3 : 4, 2>;
 
@@ -684,7 +688,7 @@ int run(AttnArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream
   XQT_REQUIRE(items < (1LL << 31) - 1 && units < (1LL << 31));
   // Few items with few keys: a cluster for each, which needs neither the list nor the second kernel (cluster | list: one sequence of 777 keys 6.6 |
   // 9.0 us, 64 of 500 18 | 21).  Where items of many keys do not fill the SMs, or there are many items, the list's even shares win (two of 131,071
-  // keys, eight heads: 125 | 71; 64 up to 8192: 95 | 82).
+  // keys, eight heads: 125 | 70; 64 up to 8192: 95 | 82).
   const long long keys = (long long)a.table_width << a.page_shift, seen = a.window ? min(keys, (long long)a.window + min(most_rows / a.each, (long long)a.tokens) + SH::CT) : keys;
   const long long of_item = (seen + SH::UNIT - 1) / SH::UNIT;
   int size = 8;
@@ -765,9 +769,7 @@ extern "C" int xqt_b200_kv4_attention(const void* q, const void* codes, const vo
   a.table_width = table_width;
   a.window = window;
   a.scale = scale * 1.4426950408889634f;
-  // Which sequences go to the prompt kernel.  Its tiles of 128 rows run near the tensor core's rate where they are full and fill the SMs, and one
-  // of its CTAs takes a sequence's keys alone; this file's kernel spreads any sequence over all SMs.
-  // Sequences with more rows go to the prompt kernel, unless the whole call is so little work that its two launches more are not worth it (keys: as
+  // Sequences with more than kFewRows rows go to the prompt kernel, whose tiles of 128 or 256 rows run at half of the tensor core's rate where they are full, unless the whole call is so little work that its two launches more are not worth it (keys: as
   // many as the table holds).  Both sides measured, this kernel for all | prompt kernel above 32 rows: one sequence, 40 queries of 32 heads on 2000
   // keys 25 | 33 us, 64 queries 31 | 36, 16 queries on 30,000 keys 62 | 66; 64 sequences of 16 queries on 2000 keys 332 | 275, of 9 queries 249 | 273.
   a.few_rows = INT_MAX;

@@ -2,15 +2,16 @@
 // for what a query sees: kv4_attention.cu), on the tensor cores.
 //
 // An item is TILES row tiles of 128 (row = query * heads of the key head + head) of one sequence and key head, and the keys they see, BN at
-// a time; the chunks of all items form one list, dealt out evenly to one CTA per SM, and items that CTAs share are joined by a second kernel.  Codes come in by bulk copies; four warps turn them into fp16 keys and values in shared memory (128-byte swizzle), once for all rows;
-// one thread issues S = Q K^T and O += P V (tcgen05, sums in tensor memory); four warps per row tile, a thread per row, do the softmax: P goes
-// back to tensor memory over the scores that it came from.  Scores are double-buffered: those of the next chunk are made while the softmax
-// works on this one's.
+// a time; the chunks of all items form one list, dealt out evenly to one CTA per SM, and items that CTAs share are joined by a second kernel.
+// Codes come in by bulk copies; four warps turn them into fp16 keys and values in shared memory (128-byte swizzle), once for all rows; one
+// thread per row tile issues S = Q K^T and O += P V (tcgen05, sums in tensor memory); four warps per row tile, a thread per row, do the
+// softmax: P goes back to tensor memory over the scores that it came from.  Scores are double-buffered: those of the next chunk are made
+// while the softmax works on this one's.
 //
 //   warp 0       table look-ups and bulk copies
 //   warp 2       allocates tensor memory, prefetches queries
 //   warps 1, 3   tcgen05.mma, one issuer per row tile: an answer of a barrier takes about 200 clocks, and one thread waiting for both tiles in
-//                turn set the pace (8192-token prompt: 605 us with all other work left out)
+//                turn set the pace (8192-token prompt: 476 us of 605 with all other work left out)
 //   warps 4-7    codes -> fp16
 //   warps 8-15   softmax, rescaling of O, result
 //
@@ -26,7 +27,10 @@
 // The order of a word's codes: pairs (0,4) (1,5) (2,6) (3,7) come out of one AND each, so channels stand in shared memory as 0 4 1 5 2 6 3 7 in
 // every group of eight; queries are stored in the same order, and the result is put back when it is written.
 //
-// Bound by the tensor core and by ex2 (16 a clock and SM), which take the same time for 128 channels.
+// Bound by the tensor core and by ex2 (16 a clock and SM), which take the same time for 128 channels; what is left between that and the measured
+// time is the chain scores -> softmax -> P -> product, of which two tiles overlap, and what an item costs before and after its chunks.
+// Measured: 628 us for the prompt of 8192 tokens (32 heads on 8 of 128 channels: 875 TFLOP/s, half of a library GEMM's rate), 468 us for chunks of
+// four prompts, 8188 queries of 40 heads on 8 in all (770 TFLOP/s).
 #include "kv4_attention.cuh"
 
 namespace xqt_b200 {
@@ -55,7 +59,7 @@ struct PromptShape {
 
 // Barriers, in 8-byte words behind the tiles.  Those of scores, P and O are per tile and chunk parity: a softmax warp may be a chunk ahead of its
 // neighbours, and a wait may come two products late.
-enum : int { kRawFull = 0, kRawEmpty = 4, kKReady = 8, kVReady = 12, kKEmpty = 16, kVEmpty = 20, kSFull = 24, kPReady = 28, kODone = 32, kGrown = 36, kQReady = 40, kBarriers = 42 };
+enum : int { kRawFull = 0, kRawEmpty = 4, kKReady = 8, kVReady = 12, kKEmpty = 16, kVEmpty = 20, kSFull = 24, kPReady = 28, kODone = 32, kGrown = 36, kQReady = 40 };
 constexpr int kRing = 16;          // chunks that loader, conversion and softmax may lie apart: more than 2 + 2 * STAGES
 
 template <int N>

@@ -9,11 +9,11 @@
 //   params T     [pages, 2, heads, page_size, 2]                      (scale, minimum)
 //
 // A head's tokens of one page are contiguous in both, so attention fetches them with one bulk copy each.  Both kernels move
-// 2 * dim bytes one way and dim / 2 + 4 the other; 8 channels a lane: one 16-byte access to the vector, one 4-byte access to the codes, two
-// vectors a lane in flight.  What bounds them is the issue of instructions, not HBM: an append needs about 9 of them per channel (minimum,
-// maximum, rounding, the test for ties, packing), which is why minimum and maximum run on packed pairs, the division is a product and codes are packed
-// in fp32.  Measured, 16,001 tokens of 8 heads of 128 channels: append 36 us (83 MB: 2.3 TB/s), gather 22 us (3.8 TB/s), both at 3.2 to 3.3 of 4
-// instructions a clock.
+// 2 * dim bytes one way and dim / 2 + 4 the other.  A lane takes the same channels of a token's key and value: what it computes
+// once (the place in the cache, by multiplication) serves both, and both loads are in flight together.  An append is bound by the issue of
+// instructions before HBM (minimum, maximum, rounding, the test for halves, packing), so minimum and maximum run on packed pairs as they
+// come, everything else on packed fp32, and nothing divides.  Measured, 16,001 tokens of 8 heads of 128 channels: append fp16 19.5 us, bf16 20.5
+// (83 MB: 4.2 TB/s; with divisions 8 channels a lane and keys apart from values 36), gather 15 us (5.6 TB/s, HBM); up to 256 tokens 2.3 to 2.7 us.
 #include <type_traits>
 
 #include "pairs.cuh"
@@ -79,31 +79,42 @@ __device__ __forceinline__ float reciprocal(float x) {         // to 2^-23 of it
   return y;
 }
 
-// The key and the value of one token and head per group of DIM / 8 lanes.  Minimum and maximum on packed pairs as they come, the minimum
+// The key and the value of one token and head per group of DIM / 16 lanes (16 channels a lane: what is computed once per lane, the place and the scale, is a third of
+// the work at 8).  Minimum and maximum on packed pairs as they come, the minimum
 // negated so that both are maxima, NaN kept.  The division is a product with the reciprocal, which is off by less than 2^-18 of a code: the
-// quotients that close to half a code are divided.
+// quotients that close to half a code are looked at again.
 template <typename T, int DIM>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const CacheArgs a) {
-  constexpr int LANES = DIM / 8, kGroups = 256 / LANES;
+  constexpr int LANES = DIM / 16, kGroups = 256 / LANES;
   constexpr float kHalf = 0.5f - 1.0f / 65536.0f, kMagic = 12582912.0f, kMost = 3.402823466e38f;     // kMagic: 1.5 * 2^23, rounds to whole numbers
   constexpr float kNormal = std::is_same<T, __half>::value ? 6.103515625e-05f : 1e-30f;
   using P = typename Pair<T>::type;
   const int lane = threadIdx.x % LANES;
   const unsigned item = blockIdx.x * kGroups + threadIdx.x / LANES;
   long long at = -1;
-  uint4 raw[2] = {};
+  uint4 raw[2][2] = {};
   if (item < (unsigned)a.tokens * a.heads) {
     int token, head;
     at = place_of(a, item, token, head);
     if (at >= 0) {
 #pragma unroll
-      for (int b = 0; b < 2; ++b) raw[b] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.x[b]) + token * a.x_token[b] + head * a.x_head[b] + 8 * lane);
+      for (int b = 0; b < 2; ++b) {
+        const uint4* const src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.x[b]) + token * a.x_token[b] + head * a.x_head[b] + 16 * lane);
+        raw[b][0] = src[0];
+        raw[b][1] = src[1];
+      }
     }
   }
 #pragma unroll
   for (int b = 0; b < 2; ++b) {
-    const P* const e = reinterpret_cast<const P*>(&raw[b]);
-    const P high2 = __hmax2_nan(__hmax2_nan(e[0], e[1]), __hmax2_nan(e[2], e[3])), low2 = __hneg2(__hmin2_nan(__hmin2_nan(e[0], e[1]), __hmin2_nan(e[2], e[3])));
+    const P* const e = reinterpret_cast<const P*>(raw[b]);
+    P high2 = e[0], low2 = e[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+      high2 = __hmax2_nan(high2, e[i]);
+      low2 = __hmin2_nan(low2, e[i]);
+    }
+    low2 = __hneg2(low2);
     P both = __hmax2_nan(lows(high2, low2), highs(high2, low2));      // (maximum, -minimum)
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) {
@@ -117,42 +128,47 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const CacheArgs a) {
     const bool good = range <= kMost && fabsf(low) <= kMost && fabsf(high) <= kMost;     // no NaN, no infinity
     float scale = to_float<T>(from_float<T>(fifteenth(range)));
     if (scale == 0.0f) scale = 1.0f;
-    Two x[4];
+    const Two inverse(reciprocal(scale)), minus(-low);
+    uint32_t word[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = floats(e[i]);
-      x[i] = Two(f.x, f.y) + Two(-low);
-    }
-    const Two inverse(reciprocal(scale));
-    float code[8], near = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const Two r = fma2(x[i], inverse, Two(kMagic)) + Two(-kMagic);
-      const float2 c = r.both(), off = fma2(x[i], inverse, r * Two(-1.0f)).both();
-      code[2 * i] = c.x;
-      code[2 * i + 1] = c.y;
-      near = fmaxf(near, fmaxf(fabsf(off.x), fabsf(off.y)));
-    }
-    // a scale that is a normal number is too low by 2^-8 of itself at most, so no quotient reaches 15.5; the others are divided and clamped
-    if (near > kHalf || !(scale >= kNormal)) {
+    for (int h = 0; h < 2; ++h) {
+      Two x[4], code[4];
+      float near = 0.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 f = x[i].both();
-        code[2 * i] = fminf(rintf(__fdiv_rn(f.x, scale)), 15.0f);
-        code[2 * i + 1] = fminf(rintf(__fdiv_rn(f.y, scale)), 15.0f);
+        const float2 f = floats(e[4 * h + i]);
+        x[i] = Two(f.x, f.y) + minus;
+        code[i] = fma2(x[i], inverse, Two(kMagic)) + Two(-kMagic);
+        const float2 off = fma2(x[i], inverse, code[i] * Two(-1.0f)).both();
+        near = fmaxf(near, fmaxf(fabsf(off.x), fabsf(off.y)));
       }
+      // A scale that is a normal number is too low by 2^-8 of itself at most, so no quotient reaches 15.5.  Near a half the quotient is corrected
+      // once, which rounds it as the division does: the remainder is exact, the correction good to 2^-20 of a step, and a quotient by the
+      // 8 or 11 bits of a scale is at least 2^-12 of a step away from where rounding turns.  Bf16 vectors stand on halves often.
+      if (near > kHalf) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const Two q = x[i] * inverse;
+          code[i] = fma2(fma2(q, Two(-scale), x[i]), inverse, q) + Two(kMagic) + Two(-kMagic);
+        }
+      }
+      if (!(scale >= kNormal)) {                       // divided and clamped
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = x[i].both();
+          code[i] = Two(fminf(rintf(__fdiv_rn(f.x, scale)), 15.0f), fminf(rintf(__fdiv_rn(f.y, scale)), 15.0f));
+        }
+      }
+      // 16 bits at a time are exact in fp32; 2^23 puts them in the low bits
+      const float2 lo = fma2(code[1], Two(256.0f), code[0]).both(), hi = fma2(code[3], Two(256.0f), code[2]).both();
+      word[h] = __byte_perm(__float_as_uint(fmaf(lo.y, 16.0f, lo.x) + 8388608.0f), __float_as_uint(fmaf(hi.y, 16.0f, hi.x) + 8388608.0f), 0x5410);
     }
-    uint32_t word;
-    if (good) {                                      // 16 bits at a time are exact in fp32
-      const float even = fmaf(code[3], 4096.0f, fmaf(code[2], 256.0f, fmaf(code[1], 16.0f, code[0])));
-      const float odd = fmaf(code[7], 4096.0f, fmaf(code[6], 256.0f, fmaf(code[5], 16.0f, code[4])));
-      word = __byte_perm(__float_as_uint(even + 8388608.0f), __float_as_uint(odd + 8388608.0f), 0x5410);
-    } else {
-      word = 0;
+    if (!good) {
+      word[0] = word[1] = 0;
       scale = low = __int_as_float(0x7fffffff);
     }
     const long long to = at + (b ? (long long)a.heads * a.page_size : 0);
-    reinterpret_cast<uint32_t*>(a.codes + to * (DIM / 2))[lane] = word;
+    reinterpret_cast<uint2*>(a.codes + to * (DIM / 2))[lane] = make_uint2(word[0], word[1]);
     if (lane == 0) {
       const P pair = rounded(scale, low, T());
       reinterpret_cast<uint32_t*>(a.params)[to] = *reinterpret_cast<const uint32_t*>(&pair);
@@ -195,7 +211,7 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(const CacheArgs a) {
 
 template <typename T, int DIM>
 int launch(const CacheArgs& a, bool append, cudaStream_t stream) {
-  const int of_block = 256 / (DIM / 8);
+  const int of_block = 256 / (DIM / (append ? 16 : 8));
   const long long grid = ((long long)a.tokens * a.heads + of_block - 1) / of_block;
   if (append)
     kv4_append_kernel<T, DIM><<<(unsigned)grid, 256, 0, stream>>>(a);
@@ -234,7 +250,7 @@ extern "C" int xqt_b200_kv4_append(const void* k, const void* v, void* codes, vo
   XQT_REQUIRE(served(tokens, heads, dim, pages, page_size, dtype));
   if (tokens == 0 || pages == 0) return 0;
   XQT_REQUIRE(k && v && codes && params && slots && strides);
-  XQT_REQUIRE((((uintptr_t)k | (uintptr_t)v) & 15) == 0 && (((uintptr_t)codes | (uintptr_t)params) & 3) == 0);
+  XQT_REQUIRE((((uintptr_t)k | (uintptr_t)v) & 15) == 0 && ((uintptr_t)codes & 7) == 0 && ((uintptr_t)params & 3) == 0);
   XQT_REQUIRE(((strides[0] | strides[1] | strides[2] | strides[3]) & 7) == 0);
   CacheArgs a = {};
   a.x[0] = k;

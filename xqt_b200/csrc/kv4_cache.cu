@@ -79,9 +79,9 @@ __device__ __forceinline__ float reciprocal(float x) {         // to 2^-23 of it
   return y;
 }
 
-// The key and the value of one token and head per group of DIM / 16 lanes (16 channels a lane: what is computed once per lane, the place and the scale, is a third of
-// the work at 8).  Minimum and maximum on packed pairs as they come, the minimum
-// negated so that both are maxima, NaN kept.  The division is a product with the reciprocal, which is off by less than 2^-18 of a code: the
+// The key and the value of one token and head per group of DIM / 16 lanes (16 channels a lane: what is computed once per lane, the place
+// and the scale, is a third of the work at 8).  Minimum and maximum on packed pairs as they come, the minimum negated so that both
+// are maxima, NaN kept.  The division is a product with the reciprocal, which is off by less than 2^-18 of a code: the
 // quotients that close to half a code are looked at again.
 template <typename T, int DIM>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const CacheArgs a) {

@@ -21,6 +21,11 @@
 // in the fp32 factor of the scores and at the end.  P is formed against a running maximum that moves only when a row exceeds
 // it by 2^8, so O is rescaled rarely; P <= 2^8 fits fp16.
 //
+// Rounding keys, values and P to fp16 adds about as much error each as rounding the result does: nothing beside a bf16 result's own rounding, but twice
+// an fp16 result's.  So for fp16 the converting warps keep what their rounding leaves of keys and values as a second operand, and both products are made
+// twice (PARTS = 2): the error is 1.3 to 1.4 roundings of the result instead of 2.  It costs shared memory (two stages instead of four; 32 keys at
+// a time for 256 channels) and time: the 8192-token prompt 690 | 552 us (64 channels, fp16 | bf16), 1082 | 628 (128), 3850 | 1750 (256).
+//
 // A vector that is not finite counts as NaN: its key becomes NaN, its value 0, so the rows that see it are NaN and the others never
 // meet it.  Keys that are not there (no page, past the end) become 0 and are masked.
 //
@@ -31,6 +36,8 @@
 // time is the chain scores -> softmax -> P -> product, of which two tiles overlap, and what an item costs before and after its chunks.
 // Measured: 628 us for the prompt of 8192 tokens (32 heads on 8 of 128 channels: 875 TFLOP/s, half of a library GEMM's rate), 468 us for chunks of
 // four prompts, 8188 queries of 40 heads on 8 in all (770 TFLOP/s).
+#include <type_traits>
+
 #include "kv4_attention.cuh"
 
 namespace xqt_b200 {
@@ -39,22 +46,23 @@ namespace {
 
 using namespace kv4;
 
-template <int D_, int TILES_, int STAGES_>
+template <int D_, int TILES_, int STAGES_, int PARTS_, int BN_>
 struct PromptShape {
-  static constexpr int D = D_, TILES = TILES_, STAGES = STAGES_, BN = 64;     // STAGES: of codes, keys and values
+  static constexpr int D = D_, TILES = TILES_, STAGES = STAGES_, BN = BN_;    // STAGES: of codes, keys and values
+  static constexpr int PARTS = PARTS_;                         // 2: what rounding a key or value to fp16 leaves is a second operand
   static constexpr int GROUP_WARPS = 4 / STAGES;               // that convert one chunk
   static constexpr int ROWS = 128 * TILES, UNIT = BN, CT = BN;
-  static constexpr int OPENING = 7;                            // what an item costs besides its chunks, in chunks
+  static constexpr int OPENING = 7 * 64 / BN;                  // what an item costs besides its chunks, in chunks
   static constexpr bool PROMPT = true;
   static constexpr int THREADS = 256 + 128 * TILES;
   static constexpr int BLOCKS = D / 64;                        // 128-byte wide column blocks of an operand
-  static constexpr int Q_BYTES = ROWS * D * 2, KV_BYTES = BN * D * 2;
+  static constexpr int Q_BYTES = ROWS * D * 2, PART_BYTES = BN * D * 2, KV_BYTES = PARTS * PART_BYTES;
   static constexpr int CODE_BYTES = BN * D / 2, PARAM_BYTES = BN * 4, RAW_BYTES = 2 * (CODE_BYTES + PARAM_BYTES);
   static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + STAGES * KV_BYTES, OFF_RAW = OFF_V + STAGES * KV_BYTES, OFF_MISC = OFF_RAW + STAGES * RAW_BYTES;
   static constexpr int SMEM = OFF_MISC + 768;
   // tensor memory: two buffers of scores per tile from column 0, P over the first half of its scores; O from 256
   static constexpr uint32_t O_COL = 256;
-  static_assert(2 * TILES * BN <= 256 && TILES * D <= 256 && SMEM <= 227 * 1024 && (STAGES == 2 || STAGES == 4), "tensor and shared memory");
+  static_assert(2 * TILES * BN <= 256 && TILES * D <= 256 && SMEM <= 227 * 1024 && (STAGES == 2 || STAGES == 4) && (BN == 64 || (BN == 32 && STAGES == 2)), "tensor and shared memory");
 };
 
 // Barriers, in 8-byte words behind the tiles.  Those of scores, P and O are per tile and chunk parity: a softmax warp may be a chunk ahead of its
@@ -108,6 +116,23 @@ __device__ __forceinline__ uint4 eight(uint32_t x, __half2 s, __half2 m) {
   r.y = half2_bits(__hfma2(__hsub2(bits_half2((x & 0x00f000f0u) | 0x54005400u), k64), s, m));
   r.z = half2_bits(__hfma2(__hsub2(bits_half2((y & 0x000f000fu) | 0x64006400u), k1024), s, m));
   r.w = half2_bits(__hfma2(__hsub2(bits_half2((y & 0x00f000f0u) | 0x54005400u), k64), s, m));
+  return r;
+}
+
+// the same, and what the rounding left (sums of two halves and products of two are exact with their errors)
+__device__ __forceinline__ void both_parts(__half2 c, __half2 s, __half2 m, uint32_t& high, uint32_t& low) {
+  const __half2 p = __hmul2_rn(c, s), of_p = __hfma2(c, s, __hneg2(p)), h = __hadd2_rn(p, m), b = __hsub2_rn(h, p);
+  high = half2_bits(h);
+  low = half2_bits(__hadd2_rn(__hadd2_rn(__hsub2_rn(p, __hsub2_rn(h, b)), __hsub2_rn(m, b)), of_p));
+}
+__device__ __forceinline__ uint4 eight(uint32_t x, __half2 s, __half2 m, uint4& low) {
+  const __half2 k1024 = bits_half2(0x64006400u), k64 = bits_half2(0x54005400u);
+  const uint32_t y = x >> 8;
+  uint4 r;
+  both_parts(__hsub2_rn(bits_half2((x & 0x000f000fu) | 0x64006400u), k1024), s, m, r.x, low.x);
+  both_parts(__hsub2_rn(bits_half2((x & 0x00f000f0u) | 0x54005400u), k64), s, m, r.y, low.y);
+  both_parts(__hsub2_rn(bits_half2((y & 0x000f000fu) | 0x64006400u), k1024), s, m, r.z, low.z);
+  both_parts(__hsub2_rn(bits_half2((y & 0x00f000f0u) | 0x54005400u), k64), s, m, r.w, low.w);
   return r;
 }
 
@@ -456,8 +481,11 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
             tc_fence_after();
             const uint64_t kd = k_desc + kr.slot * (SH::KV_BYTES >> 4);
 #pragma unroll
-            for (int s = 0; s < D / 16; ++s)
-              umma_ss(s_tile + (n & 1) * BN, q_desc + (s >> 2) * (128 * 128 >> 4) + 2 * (s & 3), kd + (s >> 2) * (BN * 128 >> 4) + 2 * (s & 3), kScores, s ? 1u : 0u);
+            for (int part = 0; part < SH::PARTS; ++part)
+#pragma unroll
+              for (int s = 0; s < D / 16; ++s)
+                umma_ss(s_tile + (n & 1) * BN, q_desc + (s >> 2) * (128 * 128 >> 4) + 2 * (s & 3), kd + part * (SH::PART_BYTES >> 4) + (s >> 2) * (BN * 128 >> 4) + 2 * (s & 3), kScores,
+                        part || s ? 1u : 0u);
             umma_commit(bar(kSFull + 2 * tile + (n & 1)));
             umma_commit(bar(kKEmpty + kr.slot));
             kr.next();
@@ -469,7 +497,10 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
             tc_fence_after();
             const uint64_t vd = v_desc + vr.slot * (SH::KV_BYTES >> 4);
 #pragma unroll
-            for (int s = 0; s < BN / 16; ++s) umma_ts_f16(o_tile, s_tile + (last & 1) * BN + 8 * s, vd + s * (2048 >> 4), kOut, last > before || s ? 1u : 0u);
+            for (int part = 0; part < SH::PARTS; ++part)
+#pragma unroll
+              for (int s = 0; s < BN / 16; ++s)
+                umma_ts_f16(o_tile, s_tile + (last & 1) * BN + 8 * s, vd + part * (SH::PART_BYTES >> 4) + s * (2048 >> 4), kOut, last > before || part || s ? 1u : 0u);
             umma_commit(bar(kVEmpty + vr.slot));
             umma_commit(bar(kODone + 2 * tile + (last & 1)));      // the last of what is in flight: the softmax waits for it
             vr.next();
@@ -507,11 +538,12 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
         const uint32_t mask = s_mask[n % kRing];
         const int t0 = w.begin + i * BN;
         // the chunk's largest key and value element; what is not there or not finite does not count
-        float2 k[2], v[2];
-        bool there[2], k_good[2], v_good[2];
+        constexpr int HALVES = BN / 32;
+        float2 k[HALVES], v[HALVES];
+        bool there[HALVES], k_good[HALVES], v_good[HALVES];
         float top_k = 0.0f, top_v = 0.0f;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < HALVES; ++h) {
           const int row = lane + 32 * h;
           there[h] = (mask >> (row >> 4) & 1u) && t0 + row < w.s.len;
           k[h] = pair_of<T>(kp[row]);
@@ -544,27 +576,41 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
           guarded(bar((which ? kVEmpty : kKEmpty) + slot), phase ^ 1);
           const uint8_t* const codes = raw + which * SH::CODE_BYTES;
           uint8_t* const dst = smem + (which ? SH::OFF_V : SH::OFF_K) + slot * SH::KV_BYTES;
+          // two warps share a chunk: 32 of its 64 rows each, or half of the channels of its 32
+          constexpr bool BY_ROWS = GROUP == 2 && HALVES == 2, BY_PIECES = GROUP == 2 && HALVES == 1;
 #pragma unroll 1
-          for (int h = GROUP == 2 ? warp & 1 : 0; h < (GROUP == 2 ? (warp & 1) + 1 : 2); ++h) {
-            const int row = lane + 32 * h;
-            const bool here = h ? there[1] : there[0], good = (h ? v_good[1] : v_good[0]) && (which || (h ? k_good[1] : k_good[0]));
-            const float2 par = which ? (h ? v[1] : v[0]) : (h ? k[1] : k[0]);
+          for (int h = BY_ROWS ? warp & 1 : 0; h < (BY_ROWS ? (warp & 1) + 1 : HALVES); ++h) {
+            const int row = lane + 32 * h, L = HALVES - 1;
+            const bool here = h ? there[L] : there[0], good = (h ? v_good[L] : v_good[0]) && (which || (h ? k_good[L] : k_good[0]));
+            const float2 par = which ? (h ? v[L] : v[0]) : (h ? k[L] : k[0]);
             const float by = which ? fv : fk, bad = which ? 0.0f : nan;
             const __half2 s = __float2half2_rn(!here ? 0.0f : good ? par.x * by : bad), m = __float2half2_rn(!here ? 0.0f : good ? par.y * by : bad);
             const int turn = D == 64 ? row >> 2 : D == 128 ? row >> 1 : row;       // which piece first: spreads the rows over the banks
             const uint8_t* const src = codes + row * (D / 2);
             uint8_t* const lines = dst + row * 128;
-            uint4 x = *reinterpret_cast<const uint4*>(src + turn % PIECES * 16);
+            constexpr int MINE = BY_PIECES ? PIECES / 2 : PIECES;
+            const int from = BY_PIECES ? (warp & 1) * MINE : 0;
+            uint4 x = *reinterpret_cast<const uint4*>(src + (from + turn % MINE) * 16);
 #pragma unroll 1
-            for (int e = 0; e < PIECES; ++e) {
-              const int piece = (turn + e) % PIECES;
-              const uint4 following = *reinterpret_cast<const uint4*>(src + (turn + e + 1) % PIECES * 16);
+            for (int e = 0; e < MINE; ++e) {
+              const int piece = from + (turn + e) % MINE;
+              const uint4 following = *reinterpret_cast<const uint4*>(src + (from + (turn + e + 1) % MINE) * 16);
               uint8_t* const line = lines + (piece >> 1) * (BN * 128);
               const int first = (piece & 1) * 4, swizzle = row & 7;
-              *reinterpret_cast<uint4*>(line + (((first + 0) ^ swizzle) << 4)) = eight(x.x, s, m);
-              *reinterpret_cast<uint4*>(line + (((first + 1) ^ swizzle) << 4)) = eight(x.y, s, m);
-              *reinterpret_cast<uint4*>(line + (((first + 2) ^ swizzle) << 4)) = eight(x.z, s, m);
-              *reinterpret_cast<uint4*>(line + (((first + 3) ^ swizzle) << 4)) = eight(x.w, s, m);
+              auto put = [&](int at, uint32_t codes8) {
+                uint8_t* const to = line + ((at ^ swizzle) << 4);
+                if constexpr (SH::PARTS == 2) {
+                  uint4 low;
+                  *reinterpret_cast<uint4*>(to) = eight(codes8, s, m, low);
+                  *reinterpret_cast<uint4*>(to + SH::PART_BYTES) = low;
+                } else {
+                  *reinterpret_cast<uint4*>(to) = eight(codes8, s, m);
+                }
+              };
+              put(first + 0, x.x);
+              put(first + 1, x.y);
+              put(first + 2, x.z);
+              put(first + 3, x.w);
               x = following;
             }
           }
@@ -618,7 +664,7 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
         const int t0 = w.begin + (lo + n - before) * BN;
         const float f = fminf(fmaxf(factor * s_key[n % kRing], 7.5e-37f), 1.3e30f), ratio = s_value[n % kRing];
         const uint32_t there = s_mask[n % kRing];
-        const bool all = there == 0xfu && t0 + BN - 1 <= hi_key && t0 >= from;
+        const bool all = there == (1u << BN / 16) - 1 && t0 + BN - 1 <= hi_key && t0 >= from;
         const bool masked = __any_sync(0xffffffffu, !all);
         // which of the 32 keys from t on this row sees
         auto visible = [&](int h) {
@@ -645,14 +691,15 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
         };
         uint32_t ra[32], rb[32];
         tmem_ld_32x32(s_at, ra);
-        tmem_ld_32x32(s_at + 32, rb);
+        if constexpr (BN == 64) tmem_ld_32x32(s_at + 32, rb);
         wait_ld_dep32(ra);
-        wait_ld_dep32(rb);
+        if constexpr (BN == 64) wait_ld_dep32(rb);
         if (masked) {
           hide(ra, 0);
-          hide(rb, 1);
+          if constexpr (BN == 64) hide(rb, 1);
         }
-        float top = fmaxf(largest(ra), largest(rb));
+        float top = largest(ra);
+        if constexpr (BN == 64) top = fmaxf(top, largest(rb));
         top *= f;
         const bool moves = top > m + 8.0f || (m == kLowest && top > kLowest);
         if (__any_sync(0xffffffffu, moves) || ratio != 1.0f) {
@@ -693,7 +740,7 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
         };
         weigh(ra, 0);
         s_ready = n + 1 < n_end && mbar_test_wait(bar(kSFull + 2 * tile + (n + 1 & 1)), n + 1 >> 1 & 1);
-        weigh(rb, 1);
+        if constexpr (BN == 64) weigh(rb, 1);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -763,9 +810,9 @@ long long prompt_units(const AttnArgs& a) {
 }
 size_t prompt_bytes(int ctas, int rows, int dim) { return (size_t)2 * ctas * rows * (dim * 4 + 8) + (size_t)2 * ctas * 16; }
 
-template <typename T, int D, int TILES, int STAGES>
+template <typename T, int D, int TILES, int STAGES, int PARTS, int BN = 64>
 int run(AttnArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
-  using SH = PromptShape<D, TILES, STAGES>;
+  using SH = PromptShape<D, TILES, STAGES, PARTS, BN>;
   const long long units = prompt_units<SH>(a);
   XQT_REQUIRE(units < (1LL << 31));
   const int ctas = (int)min((long long)sm_count(), units);
@@ -781,9 +828,11 @@ int run(AttnArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream
 
 template <typename T>
 int run_dim(const AttnArgs& a, int dim, void* workspace, size_t bytes, cudaStream_t stream) {
-  if (dim == 64) return run<T, 64, 2, 4>(a, workspace, bytes, stream);
-  if (dim == 128) return run<T, 128, 2, 4>(a, workspace, bytes, stream);
-  return run<T, 256, 1, 2>(a, workspace, bytes, stream);
+  // (see above: fp16 results are held to more than one fp16 rounding each of keys, values and P would leave)
+  constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 1;
+  if (dim == 64) return run<T, 64, 2, 4, PARTS>(a, workspace, bytes, stream);
+  if (dim == 128) return run<T, 128, 2, PARTS == 2 ? 2 : 4, PARTS>(a, workspace, bytes, stream);
+  return run<T, 256, 1, 2, PARTS, PARTS == 2 ? 32 : 64>(a, workspace, bytes, stream);
 }
 
 }  // namespace

@@ -691,8 +691,10 @@ int run(AttnArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream
   // keys, eight heads: 125 | 70; 64 up to 8192: 95 | 82).
   const long long keys = (long long)a.table_width << a.page_shift, seen = a.window ? min(keys, (long long)a.window + min(most_rows / a.each, (long long)a.tokens) + SH::CT) : keys;
   const long long of_item = (seen + SH::UNIT - 1) / SH::UNIT;
+  // (the cluster's size goes by the items of queries dealt out evenly; what the grid has over them finds nothing and ends)
+  const long long even = min(tiles, a.batch * (((long long)a.tokens * a.each + (long long)a.batch * SH::ROWS - 1) / ((long long)a.batch * SH::ROWS))) * a.kv_heads;
   int size = 8;
-  while (size > 1 && (items * size > (long long)SH::PER_SM * sm_count() || size >= 2 * of_item)) size >>= 1;
+  while (size > 1 && (even * size > (long long)SH::PER_SM * sm_count() || size >= 2 * of_item)) size >>= 1;
   if (items * size <= 4LL * SH::PER_SM * sm_count() && of_item <= 8 * size) {
     XQT_SMEM_OPT_IN((kv4_attention_kernel<T, SH, true>), SH::SMEM);
     return launch_pdl_cluster(kv4_attention_kernel<T, SH, true>, dim3((unsigned)(items * size)), dim3(SH::W * 32), size, SH::SMEM, stream, a);

@@ -677,6 +677,31 @@ constexpr int kMostPerSm = 2;      // CTAs of any shape on an SM
 template <int D, int NT>
 using Few = Shape<D, NT, 4, D == 256 ? 16 : NT == 1 ? 64 : 32, D * NT == 128 ? 3 : 4, 2>;
 
+// Clusters of `size` CTAs (2, 4 or 8) that are resident together, asked for once per kernel and device.
+template <auto Kern>
+int resident_clusters(int size, int threads, size_t smem) {
+  static int cached[64][3] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sm_count() / size;
+  int& known = cached[dev][size == 8 ? 2 : size == 4 ? 1 : 0];
+  if (known == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(sm_count() / size * size));
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)size;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int v = 0;
+    if (cudaOccupancyMaxActiveClusters(&v, Kern, &cfg) != cudaSuccess || v <= 0) v = sm_count() / size;
+    known = v;
+  }
+  return known;
+}
+
 template <typename T, int D, int NT>
 int run(AttnArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
   using SH = Few<D, NT>;
@@ -691,14 +716,20 @@ int run(AttnArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream
   // keys, eight heads: 125 | 70; 64 up to 8192: 95 | 82).
   const long long keys = (long long)a.table_width << a.page_shift, seen = a.window ? min(keys, (long long)a.window + min(most_rows / a.each, (long long)a.tokens) + SH::CT) : keys;
   const long long of_item = (seen + SH::UNIT - 1) / SH::UNIT;
-  // (the cluster's size goes by the items of queries dealt out evenly; what the grid has over them finds nothing and ends)
+  // A cluster's size goes by the items of queries dealt out evenly and by what is resident together.  What the grid has over those items finds
+  // nothing and ends, for which an eighth of the places is left (16 x 5 queries in a window of 1024: 14.9 us, by all that there can
+  // be 19.4; 9 x 7 queries in a window of 694: with all places taken 15.2 us, like this
+  // 9.5; nine sequences of 900 keys: sizes that fill the SMs but are not resident together 13.5, like this 9.6).
+  XQT_SMEM_OPT_IN((kv4_attention_kernel<T, SH, true>), SH::SMEM);
   const long long even = min(tiles, a.batch * (((long long)a.tokens * a.each + (long long)a.batch * SH::ROWS - 1) / ((long long)a.batch * SH::ROWS))) * a.kv_heads;
   int size = 8;
-  while (size > 1 && (even * size > (long long)SH::PER_SM * sm_count() || size >= 2 * of_item)) size >>= 1;
-  if (items * size <= 4LL * SH::PER_SM * sm_count() && of_item <= 8 * size) {
-    XQT_SMEM_OPT_IN((kv4_attention_kernel<T, SH, true>), SH::SMEM);
-    return launch_pdl_cluster(kv4_attention_kernel<T, SH, true>, dim3((unsigned)(items * size)), dim3(SH::W * 32), size, SH::SMEM, stream, a);
+  while (size > 1) {
+    const long long places = resident_clusters<kv4_attention_kernel<T, SH, true>>(size, SH::W * 32, SH::SMEM);
+    if (even + min(items - even, places / 8) <= places && size < 2 * of_item) break;
+    size >>= 1;
   }
+  if (items * size <= 4LL * SH::PER_SM * sm_count() && of_item <= 8 * size)
+    return launch_pdl_cluster(kv4_attention_kernel<T, SH, true>, dim3((unsigned)(items * size)), dim3(SH::W * 32), size, SH::SMEM, stream, a);
   const int ctas = (int)min((long long)SH::PER_SM * sm_count(), units);
   const size_t o_bytes = (size_t)2 * ctas * SH::ROWS * D * 4;
   XQT_REQUIRE(workspace && workspace_bytes >= o_bytes + (size_t)2 * ctas * (SH::ROWS * 8 + 16) && ((uintptr_t)workspace & 15) == 0);

@@ -10,7 +10,7 @@
 // Bound by HBM: every channel is read and written once.  A block makes the cosines of up to 16 tokens in shared memory, then its lane groups go
 // through the heads of those tokens: dim / 16 lanes (padded to a power of two) hold one head, 16 channels a lane, chosen so that both
 // channels of a pair are in one lane.  Sums of squares, products and turns are packed fp32 instructions: with single ones the kernel waited on issue.
-// Measured, heads of 128 channels: 8191 tokens of 32 + 8 heads 33 us (5.1 TB/s), 32,760 tokens of 20 + 20 heads on three axes 120 us (5.6 TB/s;
+// Measured, heads of 128 channels: 8191 tokens of 32 + 8 heads 31 us (5.4 TB/s), 32,760 tokens of 20 + 20 heads on three axes 120 us (5.6 TB/s;
 // a copy reaches 6.6); a call of one token 3.1 us, which is its launch and one chain load -> sum -> store.
 #include "pairs.cuh"
 
@@ -64,7 +64,7 @@ __device__ __forceinline__ uint4 pack8(const Two (&f)[4]) {
   return make_uint4(pack2(f[0], T()), pack2(f[1], T()), pack2(f[2], T()), pack2(f[3], T()));
 }
 
-constexpr int kThreads = 256, kMostTokens = 16;
+constexpr int kThreads = 256, kPerSm = 4, kMostTokens = 16;      // kPerSm: blocks on an SM
 
 // The two runs of 8 channels of lane l.
 template <bool INTERLEAVED>
@@ -83,7 +83,7 @@ __device__ __forceinline__ void runs(const RopeArgs& a, int l, int& c0, int& c1)
 
 // LANES: lanes of a head, a power of two; lanes past dim / 16 only take part in the sums.
 template <typename T, int LANES, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads, 4) rope_kernel(const RopeArgs a) {
+__global__ void __launch_bounds__(kThreads, kPerSm) rope_kernel(const RopeArgs a) {
   // four floats of every lane side by side, so that a quarter warp reads 128 contiguous bytes: pair 8 l + 4 h + i at 4 (l + 16 h) + i, and the
   // lane's channel e of run r at 4 (l + 16 (2 r + e / 4)) + e % 4
   __shared__ __align__(16) float s_cos[kMostTokens][128], s_sin[kMostTokens][128], s_weight[2][256];
@@ -262,9 +262,9 @@ extern "C" int xqt_b200_qk_norm_rope(const void* q, const void* k, void* q_out, 
   a.dim = dim;
   a.rotary = rotary;
   a.eps = eps;
-  // Tokens of a block: their cosines are made together, so more of them fill its threads; fewer fill the SMs.  Halved until there are two
-  // blocks for each SM.
-  a.block_tokens = kMostTokens;
-  while (a.block_tokens > 1 && ceil_div(tokens, a.block_tokens) < 2 * sm_count()) a.block_tokens >>= 1;
+  // Tokens of a block: their cosines are made together, so more of them fill its threads; as many as make whole waves of blocks (tokens
+  // of 32 + 8 heads, this | powers of two for two blocks an SM: 4096 16.8 | 17.9 us, 6000 24.7 | 28.4, 8191 31.2 | 33.4, 12,000 46.7 | 55).
+  const long long wave = (long long)kPerSm * sm_count(), waves = (tokens + wave * kMostTokens - 1) / (wave * kMostTokens);
+  a.block_tokens = (int)((tokens + wave * waves - 1) / (wave * waves));
   return dtype == XQT_B200_BF16 ? launch_lanes<__nv_bfloat16>(a, interleaved != 0, stream) : launch_lanes<__half>(a, interleaved != 0, stream);
 }

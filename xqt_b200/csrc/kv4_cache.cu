@@ -93,6 +93,8 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const CacheArgs a) {
   const unsigned item = blockIdx.x * kGroups + threadIdx.x / LANES;
   long long at = -1;
   uint4 raw[2][2] = {};
+  sm100::grid_launch_dependents();
+  sm100::grid_dependency_wait();
   if (item < (unsigned)a.tokens * a.heads) {
     int token, head;
     at = place_of(a, item, token, head);
@@ -182,6 +184,8 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(const CacheArgs a) {
   using P = typename Pair<T>::type;
   const int lane = threadIdx.x % LANES;
   const unsigned item = blockIdx.x * kGroups + threadIdx.x / LANES;
+  sm100::grid_launch_dependents();
+  sm100::grid_dependency_wait();
   if (item >= (unsigned)a.tokens * a.heads) return;
   int token, head;
   const long long at = place_of(a, item, token, head);
@@ -213,11 +217,8 @@ template <typename T, int DIM>
 int launch(const CacheArgs& a, bool append, cudaStream_t stream) {
   const int of_block = 256 / (DIM / (append ? 16 : 8));
   const long long grid = ((long long)a.tokens * a.heads + of_block - 1) / of_block;
-  if (append)
-    kv4_append_kernel<T, DIM><<<(unsigned)grid, 256, 0, stream>>>(a);
-  else
-    kv4_gather_kernel<T, DIM><<<(unsigned)grid, 256, 0, stream>>>(a);
-  return launch_status();
+  return append ? launch_pdl(kv4_append_kernel<T, DIM>, dim3((unsigned)grid), dim3(256), 0, stream, a)
+                : launch_pdl(kv4_gather_kernel<T, DIM>, dim3((unsigned)grid), dim3(256), 0, stream, a);
 }
 
 int dispatch(CacheArgs a, int dim, int dtype, bool append, cudaStream_t stream) {

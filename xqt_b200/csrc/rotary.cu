@@ -87,6 +87,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) rope_kernel(const RopeArgs a
   // four floats of every lane side by side, so that a quarter warp reads 128 contiguous bytes: pair 8 l + 4 h + i at 4 (l + 16 h) + i, and the
   // lane's channel e of run r at 4 (l + 16 (2 r + e / 4)) + e % 4
   __shared__ __align__(16) float s_cos[kMostTokens][128], s_sin[kMostTokens][128], s_weight[2][256];
+  sm100::grid_launch_dependents();          // (the next kernel's launch under this one's end: 8191 tokens, calls back to back, 31.5 us, without 33.1)
+  sm100::grid_dependency_wait();
   const int pairs = a.rotary / 2, token0 = blockIdx.x * a.block_tokens, block_tokens = min(a.block_tokens, a.tokens - token0);
   for (int i = threadIdx.x; i < block_tokens * pairs; i += kThreads) {
     const int token = i / pairs, pair = i - token * pairs, spot = 4 * ((pair >> 3) + 16 * (pair >> 2 & 1)) + (pair & 3);
@@ -204,11 +206,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) rope_kernel(const RopeArgs a
 template <typename T, int LANES>
 int launch(const RopeArgs& a, bool interleaved, cudaStream_t stream) {
   const unsigned grid = (unsigned)ceil_div(a.tokens, a.block_tokens);
-  if (interleaved)
-    rope_kernel<T, LANES, true><<<grid, kThreads, 0, stream>>>(a);
-  else
-    rope_kernel<T, LANES, false><<<grid, kThreads, 0, stream>>>(a);
-  return launch_status();
+  return interleaved ? launch_pdl(rope_kernel<T, LANES, true>, dim3(grid), dim3(kThreads), 0, stream, a)
+                     : launch_pdl(rope_kernel<T, LANES, false>, dim3(grid), dim3(kThreads), 0, stream, a);
 }
 
 template <typename T>

@@ -461,8 +461,9 @@ int xqt_b200_qk_norm_rope(const void* q, const void* k, void* q_out, void* k_out
  * for c * s + m.  A vector with an infinity or NaN gets s = m = NaN.
  *   codes  uint8 [pages, 2 (key, value), heads, page_size, dim / 2], low nibble = even channel
  *   params T     [pages, 2, heads, page_size, 2] = (s, m)
- * dim 64, 128 or 256; page_size a power of two, 16 to 4096; tokens * heads < 2^30.  slots [tokens] (int64 with wide_slots, else int32): page * page_size + row of each token; a slot outside
- * the cache is skipped (append) or read as zeros (gather).  The slots of one append are distinct.
+ * dim 64, 128 or 256; page_size a power of two, 16 to 4096; tokens * heads < 2^30; codes, params, vectors start on 16 bytes.
+ * slots [tokens] (int64 with wide_slots, else int32): page * page_size + row of each token; a slot outside the cache is skipped
+ * (append) or read as zeros (gather).  The slots of one append are distinct.
  * append: k, v [tokens, heads, dim]; strides (host): token and head stride of k, then of v, in elements, multiples of 8.
  * gather: k_out, v_out [tokens, heads, dim] contiguous. */
 int xqt_b200_kv4_append(const void* k, const void* v, void* codes, void* params, const void* slots,

@@ -381,6 +381,17 @@ def test_fp16_results_are_little_more_than_rounded(dim, heads, each, count):
 
 
 @pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("offset", [-20.0, 3.0, 1000.0])
+def test_fp16_prompts_of_vectors_far_from_zero(dim, offset):
+    """Minima large beside the range (and of either sign), where code * scale + minimum cancels or loses its low bits in fp16."""
+    lens, counts = [333, 70], [200, 70]
+    codes, params, table = make_cache(lens, 2, dim, 32, torch.float16, 73)
+    table = wide(table, 32)
+    params[..., 1] += offset
+    check(_vectors(270, 8, dim, torch.float16, 74, 0.25), codes, params, table, lens, counts)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
 def test_prompts_of_many_sequences_beside_single_tokens(dim):
     lens, counts = [40, 700, 33, 1, 512, 90, 0, 2000] * 3, [40, 1, 9, 1, 512, 33, 3, 700] * 3
     codes, params, table = make_cache(lens, 2, dim, 32, torch.bfloat16, 52)

@@ -19,7 +19,8 @@
 // three operands go in with a power of two: a query row with its own (largest element in [1, 2)), the keys of a chunk with one
 // for the chunk (largest in [2^13, 2^14)), values with one that only grows along the sequence (O is rescaled then).  The powers come back
 // in the fp32 factor of the scores and at the end.  P is formed against a running maximum that moves only when a row exceeds
-// it by 2^8, so O is rescaled rarely; P <= 2^8 fits fp16.
+// it by 2^8, so O is rescaled rarely, and times 2^7 (in its sum and in O alike): P <= 2^15 fits fp16, and an element below 2^-14, whose
+// rounding is not relative to it any more, stands for at most 2^-21 of the row's largest; what rounds to 0 for 2^-32.
 //
 // Rounding keys, values and P to fp16 adds about as much error each as rounding the result does: nothing beside a bf16 result's own rounding, but twice
 // an fp16 result's.  So for fp16 the converting warps keep what their rounding leaves of keys and values as a second operand, and both products are made
@@ -68,6 +69,7 @@ struct PromptShape {
 // Barriers, in 8-byte words behind the tiles.  Those of scores, P and O are per tile and chunk parity: a softmax warp may be a chunk ahead of its
 // neighbours, and a wait may come two products late.
 enum : int { kRawFull = 0, kRawEmpty = 4, kKReady = 8, kVReady = 12, kKEmpty = 16, kVEmpty = 20, kSFull = 24, kPReady = 28, kODone = 32, kGrown = 36, kQReady = 40 };
+constexpr float kLift = 7.0f;      // log2 of P where a score equals the running maximum
 constexpr int kRing = 16;          // chunks that loader, conversion and softmax may lie apart: more than 2 + 2 * STAGES
 
 template <int N>
@@ -726,7 +728,7 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
             }
           }
         }
-        const Two f2(f), minus(m == kLowest ? 0.0f : -m);
+        const Two f2(f), minus(m == kLowest ? 0.0f : kLift - m);
         auto weigh = [&](const uint32_t (&r)[32], int at) {
           uint32_t h[16];
 #pragma unroll

@@ -17,11 +17,11 @@ DEVICE = torch.device("cuda", 0)
 PAGE = 64
 
 
-def long_prompt(keys, dim, dtype, queries, exponent=None, seed=81):
-    """A key head per SM, so that every one has whole items; the tables go round 64 pages.  Values lie in [0.53, 1.47] with a mean of 1.  With ``exponent`` the first key is
+def long_prompt(keys, dim, dtype, queries, exponent=None, seed=81, heads=None):
+    """A key head per SM, so that every one has whole items (unless ``heads`` says otherwise); the tables go round 64 pages.  Values lie in [0.53, 1.47] with a mean of 1.  With ``exponent`` the first key is
     2 ** exponent times as probable as the others are on average, and its values are 0.  -> arguments, and those of the first two heads for the reference."""
 
-    heads = torch.cuda.get_device_properties(0).multi_processor_count
+    heads = heads or torch.cuda.get_device_properties(0).multi_processor_count
     gen = torch.Generator(device=DEVICE).manual_seed(seed)
     codes = torch.randint(0, 256, (65, 2, heads, PAGE, dim // 2), dtype=torch.uint8, device=DEVICE, generator=gen)
     params = torch.empty((65, 2, heads, PAGE, 2), dtype=dtype, device=DEVICE)
@@ -57,4 +57,51 @@ def test_many_weak_keys_beside_a_strong_one(dim, exponent):
     assert float((bound / want.abs()).max()) < 1 / 8             # some rows' strong key is 2^29 times as probable: their bound still says something
     worst = float(((got - want).abs() / bound).max())
     assert worst <= 1, f"{worst} bounds; {float(((got - want).abs() / want.abs()).max())} of the result"
+    assert native.workspace_status(DEVICE) == 0
+
+
+def summed(dtype, want):
+    """What the tensor core's sums may lose: of each product the bits below 2^-24 of the running sum, which is of one sign here, in runs of 4096 keys with
+    two products each (fp16) or of 16,384 with one (bf16)."""
+    return (2 * 4096 if dtype == torch.float16 else 16384) * 2.0 ** -24 * want.abs()
+
+
+@pytest.mark.parametrize("dtype,dim,keys", [(torch.float16, 64, 131072), (torch.float16, 128, 131072), (torch.float16, 256, 131072), (torch.bfloat16, 64, 1 << 20)])
+def test_long_sums_of_values_of_one_sign(dtype, dim, keys):
+    call, small = long_prompt(keys, dim, dtype, 40)
+    got = kv4_attention(*call[:5], query_starts=call[5], scale=0.25)[:, :2].double()
+    want, bound = attention(*small, scale=0.25, rounded=torch.float16)
+    worst = float(((got - want).abs() / (bound + summed(dtype, want))).max())
+    assert worst <= 1, f"{worst} bounds"
+    assert native.workspace_status(DEVICE) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("keys", [4096, 16384, 20032])
+@pytest.mark.parametrize("heads,window", [(None, None), (100, None), (100, 9000)])
+def test_runs_of_keys_in_whole_and_in_shared_items(dtype, dim, keys, heads, window):
+    """Around the lengths at which a sum is put aside, with items of one CTA and of two; hidden pages so that whole runs see nothing, and queries that are not finite."""
+    call, small = long_prompt(keys, dim, dtype, 70, heads=heads)
+    call[0][5, 1, 3] = float("inf")
+    for hidden in (None, slice(0, 70), slice(max(keys // PAGE - 70, 0), keys // PAGE)):
+        table, short = call[3].clone(), small[3].clone()
+        if hidden is not None:
+            table[:, hidden] = -1
+            short[:, hidden] = -1
+        got = kv4_attention(*call[:3], table, call[4], query_starts=call[5], window=window)[:, :2].double()
+        want, bound = attention(*small[:3], short, *small[4:], rounded=torch.float16, window=window)
+        sees = torch.arange(keys).reshape(-1, PAGE)[(short[0] >= 0)]
+        last = torch.arange(keys - 70, keys)
+        nothing = torch.tensor([not bool(((sees <= i) & (sees > i - (window or keys))).any()) for i in last.tolist()])
+        assert bool((got[nothing.to(DEVICE)] == 0).all())
+        spoilt = torch.zeros((70, 2), dtype=torch.bool, device=DEVICE)
+        spoilt[5, 1] = not bool(nothing[5])
+        assert bool(torch.isnan(got[spoilt]).all()) and bool(torch.isfinite(got[~spoilt]).all())
+        over = (got - want).abs()[~spoilt] - (bound + summed(dtype, want))[~spoilt]
+        assert bool((over <= 0).all()), f"{float(over.max())} over"
+    first = kv4_attention(*call[:5], query_starts=call[5], window=window)
+    for _ in range(3):
+        again = kv4_attention(*call[:5], query_starts=call[5], window=window)
+        assert torch.equal(again.view(torch.uint8), first.view(torch.uint8))
     assert native.workspace_status(DEVICE) == 0

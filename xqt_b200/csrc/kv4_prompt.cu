@@ -25,7 +25,12 @@
 // Rounding keys, values and P to fp16 adds about as much error each as rounding the result does: nothing beside a bf16 result's own rounding, but twice
 // an fp16 result's.  So for fp16 the converting warps keep what their rounding leaves of keys and values as a second operand, and both products are made
 // twice (PARTS = 2): the error is 1.3 to 1.4 roundings of the result instead of 2.  It costs shared memory (two stages instead of four; 32 keys at
-// a time for 256 channels) and time: the 8192-token prompt 690 | 552 us (64 channels, fp16 | bf16), 1082 | 628 (128), 3850 | 1750 (256).
+// a time for 256 channels) and time: the 8192-token prompt 697 | 558 us (64 channels, fp16 | bf16), 1115 | 629 (128), 4005 | 1766 (256).
+//
+// The tensor core cuts off the bits of a product that stand below its running sum's, so a sum that grew over a whole long context would be too small, by
+// 1.6 half steps of an fp16 result after 131,072 keys of equal weight, by up to 4 where one key is far more probable than the others.  O therefore
+// starts afresh after a RUN of keys (4096 for fp16, 16,384 for bf16, whose result holds 8 times less): what it held is added, rounded to
+// nearest, to the row's part in the workspace (2048 queries on 65,536 keys, without | with: fp16 3914 | 3992 us, bf16 2120 | 2159).
 //
 // A vector that is not finite counts as NaN: its key becomes NaN, its value 0, so the rows that see it are NaN and the others never
 // meet it.  Keys that are not there (no page, past the end) become 0 and are masked.
@@ -35,7 +40,7 @@
 //
 // Bound by the tensor core and by ex2 (16 a clock and SM), which take the same time for 128 channels; what is left between that and the measured
 // time is the chain scores -> softmax -> P -> product, of which two tiles overlap, and what an item costs before and after its chunks.
-// Measured: 628 us for the prompt of 8192 tokens (32 heads on 8 of 128 channels: 875 TFLOP/s, half of a library GEMM's rate), 468 us for chunks of
+// Measured: 629 us for the prompt of 8192 tokens (32 heads on 8 of 128 channels: 874 TFLOP/s, half of a library GEMM's rate), 468 us for chunks of
 // four prompts, 8188 queries of 40 heads on 8 in all (770 TFLOP/s).
 #include <type_traits>
 
@@ -54,6 +59,7 @@ struct PromptShape {
   static constexpr int GROUP_WARPS = 4 / STAGES;               // that convert one chunk
   static constexpr int ROWS = 128 * TILES, UNIT = BN, CT = BN;
   static constexpr int OPENING = 7 * 64 / BN;                  // what an item costs besides its chunks, in chunks
+  static constexpr int RUN = (PARTS == 2 ? 4096 : 16384) / BN;   // chunks that O is summed over in tensor memory
   static constexpr bool PROMPT = true;
   static constexpr int THREADS = 256 + 128 * TILES;
   static constexpr int BLOCKS = D / 64;                        // 128-byte wide column blocks of an operand
@@ -182,16 +188,23 @@ __device__ __noinline__ float load_queries(const T* src, uint8_t* dst, float sca
   return factor;
 }
 
-// The 32 rows of a warp from tensor memory, times `by`, to their addresses (or null): as T, or as fp32 parts.
+// The 32 rows of a warp from tensor memory, times `by`: kResult, to the rows of the result; kPart, to the rows' parts (fp32); kAdded, added to those; kScaled,
+// added to what they hold times `keep`; kSum, the same, but to the rows of the result.  Each lane gives its own row's addresses (0: no row) and factors.
+enum : int { kResult, kPart, kAdded, kScaled, kSum };
 template <typename T, int D>
-__device__ __noinline__ void store_rows(uint32_t o_at, unsigned long long mine, float by, bool whole) {
+__device__ __noinline__ void store_rows(uint32_t o_at, unsigned long long part, unsigned long long out, float by, float keep, int how) {
   const int lane = threadIdx.x & 31;
   // Four lanes write 64 bytes of a row together (a lane alone would touch a line of its own with every store): they exchange 16-byte pieces,
-  // piece i of row k for piece k of row i.
-  unsigned long long rows_at[4];
+  // piece i of row k for piece k of row i.  A part's piece is the same lane's every time, so nothing depends on an order among lanes.
+  unsigned long long parts_at[4], outs_at[4];
+  float keeps[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) rows_at[k] = __shfl_sync(0xffffffffu, mine, (lane & 28) + k);
-  auto exchange_and_store = [&](uint4 (&x)[4], int offset) {
+  for (int k = 0; k < 4; ++k) {
+    parts_at[k] = __shfl_sync(0xffffffffu, part, (lane & 28) + k);
+    outs_at[k] = __shfl_sync(0xffffffffu, out, (lane & 28) + k);
+    keeps[k] = __shfl_sync(0xffffffffu, keep, (lane & 28) + k);
+  }
+  auto exchange = [&](uint4 (&x)[4]) {
     auto swap = [](uint4& keep_low, uint4& keep_high, bool upper, int o) {
       uint4 give = upper ? keep_low : keep_high;
       give.x = __shfl_xor_sync(0xffffffffu, give.x, o);
@@ -205,9 +218,6 @@ __device__ __noinline__ void store_rows(uint32_t o_at, unsigned long long mine, 
     swap(x[2], x[3], lane & 1, 1);
     swap(x[0], x[2], lane & 2, 2);
     swap(x[1], x[3], lane & 2, 2);
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (rows_at[k] != 0) *reinterpret_cast<uint4*>(rows_at[k] + offset + 16 * (lane & 3)) = x[k];
   };
 #pragma unroll 1
   for (int c = 0; c < D / 32; ++c) {
@@ -216,14 +226,17 @@ __device__ __noinline__ void store_rows(uint32_t o_at, unsigned long long mine, 
     wait_ld_dep32(r);
     auto value = [&](int e) { return __uint_as_float(r[(e & ~7) + ((e & 7) < 4 ? 2 * (e & 7) : 2 * (e & 7) - 7)]) * by; };      // channel e of these 32
     uint4 x[4];
-    if (whole) {
+    if (how == kResult) {
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         T* const t = reinterpret_cast<T*>(&x[b]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) t[e] = from_float<T>(value(8 * b + e));
       }
-      exchange_and_store(x, 64 * c);
+      exchange(x);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (outs_at[k] != 0) *reinterpret_cast<uint4*>(outs_at[k] + 64 * c + 16 * (lane & 3)) = x[k];
     } else {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -231,7 +244,28 @@ __device__ __noinline__ void store_rows(uint32_t o_at, unsigned long long mine, 
         for (int b = 0; b < 4; ++b)
           x[b] = make_uint4(__float_as_uint(value(16 * h + 4 * b)), __float_as_uint(value(16 * h + 4 * b + 1)), __float_as_uint(value(16 * h + 4 * b + 2)),
                             __float_as_uint(value(16 * h + 4 * b + 3)));
-        exchange_and_store(x, 128 * c + 64 * h);
+        exchange(x);
+        const int offset = 128 * c + 64 * h + 16 * (lane & 3);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (parts_at[k] == 0) continue;
+          float4 v = make_float4(__uint_as_float(x[k].x), __uint_as_float(x[k].y), __uint_as_float(x[k].z), __uint_as_float(x[k].w));
+          float4* const at = reinterpret_cast<float4*>(parts_at[k] + offset);
+          if (how == kAdded) {                       // no answer to wait for (with kScaled always the fp16 figure above is 4239)
+            atomicAdd(at, v);
+            continue;
+          }
+          if (how >= kScaled) {
+            const float4 old = __ldcg(at);
+            v = make_float4(fmaf(old.x, keeps[k], v.x), fmaf(old.y, keeps[k], v.y), fmaf(old.z, keeps[k], v.z), fmaf(old.w, keeps[k], v.w));
+          }
+          if (how == kSum) {
+            T t[4] = {from_float<T>(v.x), from_float<T>(v.y), from_float<T>(v.z), from_float<T>(v.w)};
+            *reinterpret_cast<uint2*>(outs_at[k] + offset / 2) = *reinterpret_cast<uint2*>(t);
+          } else {
+            *at = v;
+          }
+        }
       }
     }
   }
@@ -241,6 +275,13 @@ __device__ __noinline__ void store_rows(uint32_t o_at, unsigned long long mine, 
 struct PromptItem {
   int b, tile, head, unit, begin, chunks;
   Sequence s;
+};
+
+// Chunks [lo, hi) of an item, SH::RUN at most: whether they are the first and the last of those that are this CTA's, whether those are the whole item
+// and whether they are its beginning; and how many chunks the CTA has had before.
+struct Run {
+  int lo, hi, before;
+  bool first, last, whole, opens;
 };
 
 // the keys that some row of a tile sees start in chunk begin / BN; how many chunks
@@ -382,17 +423,22 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
-  // The CTA's part of the list: `body` gets an item, its chunks [lo, hi) that are this CTA's, whether that is all of it and whether it is its
-  // beginning, and how many chunks the CTA has had before.  Every role goes through it for itself.
-  auto segments = [&](auto body) {
+  // The CTA's part of the list: `body` gets an item and a run of its chunks.  Every role goes through it for itself.
+  auto runs = [&](auto body) {
     PromptItem w = *s_start;
     unsigned left = s_range[1] - s_range[0];
     int before = 0;
     while (left > 0) {
       const unsigned units = (unsigned)(w.chunks + SH::OPENING), take = min(units - w.unit, left);
       const int lo = max(w.unit - SH::OPENING, 0), hi = max((int)(w.unit + take) - SH::OPENING, 0);
-      body(w, lo, hi, w.unit == 0 && take == units, w.unit == 0, before);
-      before += hi - lo;
+      const bool opens = w.unit == 0, whole = opens && take == units;
+      int at = lo;
+      do {
+        const int to = min(at + SH::RUN, hi);
+        body(w, Run{at, to, before, at == lo, to == hi, whole, opens});
+        before += to - at;
+        at = to;
+      } while (at < hi);
       left -= take;
       if (left > 0) prompt_next<SH>(a, w);
     }
@@ -432,7 +478,8 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
     const uint32_t target = smem_addr(smem + SH::OFF_RAW) +
                             (kind == 0 ? 0 : kind == 1 ? SH::CODE_BYTES : kind == 2 ? 2 * SH::CODE_BYTES : 2 * SH::CODE_BYTES + SH::PARAM_BYTES) + piece * psz * row_bytes;
     Ring<SH::STAGES> ring;
-    segments([&](const PromptItem& w, int lo, int hi, bool, bool, int before) {
+    runs([&](const PromptItem& w, const Run& run) {
+      const int lo = run.lo, hi = run.hi, before = run.before;
       const uint8_t* const source = (kind < 2 ? a.codes : a.params) + ((long long)(kind & 1) * a.kv_heads + w.head) * a.page_size * row_bytes;
       const int* const table = a.table + w.b * a.table_stride;
       auto look_up = [&](int i) {
@@ -471,10 +518,13 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
       // scores run one chunk ahead; a buffer of theirs is free again behind the product that read P from it (the tensor core works in order)
       Ring<SH::STAGES> kr, vr;
       uint32_t q_phase = 0;
-      segments([&](const PromptItem&, int lo, int hi, bool, bool, int before) {
+      runs([&](const PromptItem&, const Run& run) {
+        const int lo = run.lo, hi = run.hi, before = run.before;
         if (hi == lo) return;
-        polled(bar(kQReady + tile), q_phase);
-        q_phase ^= 1;
+        if (run.first) {
+          polled(bar(kQReady + tile), q_phase);
+          q_phase ^= 1;
+        }
         bool k_ready = false;
         const int n_end = before + hi - lo;
         for (int n = before; n <= n_end; ++n) {
@@ -512,8 +562,8 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------ the queries of all the CTA's items into L2, ahead of their use
-    segments([&](const PromptItem& w, int lo, int hi, bool, bool, int) {
-      if (hi == lo) return;
+    runs([&](const PromptItem& w, const Run& run) {
+      if (run.hi == run.lo || !run.first) return;
       for (int r = lane; r < SH::ROWS; r += 32) {
         const int row = w.tile * SH::ROWS + r, j = row / a.each;
         if (j >= w.s.nq) return;
@@ -530,7 +580,8 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
     constexpr int GROUP = SH::GROUP_WARPS;
     const int slot = (warp & 3) / GROUP;
     const uint8_t* const raw = smem + SH::OFF_RAW + slot * SH::RAW_BYTES;
-    segments([&](const PromptItem& w, int lo, int hi, bool, bool, int before) {
+    runs([&](const PromptItem& w, const Run& run) {
+      const int lo = run.lo, hi = run.hi, before = run.before;
       for (int n = before + (slot - before % SH::STAGES + SH::STAGES) % SH::STAGES; n < before + hi - lo; n += SH::STAGES) {
         const int i = lo + n - before;
         const uint32_t phase = n / SH::STAGES & 1;
@@ -628,29 +679,28 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
     const int tile = (warp - 8) >> 2, quarter = warp & 3, line = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_tile = tmem + lanes + 2 * tile * BN, o_at = tmem + lanes + SH::O_COL + tile * D;
-    // a finished segment whose O is still in tensor memory: it is written when the queries of the next one are on their way
+    // a finished run whose O is still in tensor memory: it is written when the queries of the next one are on their way
     T* out = nullptr;
     float* part = nullptr;
-    float out_by = 0.0f;
-    int out_n = -1;
-    bool out_whole = false;
+    float out_by = 0.0f, out_keep = 0.0f;
+    int out_n = -1, out_how = kResult;
     auto flush = [&]() {
       if (out_n < 0) return;
       guarded(bar(kODone + 2 * tile + (out_n & 1)), out_n >> 1 & 1);
       tc_fence_after();
-      out_n = -1;
-      const unsigned long long mine = part != nullptr ? reinterpret_cast<unsigned long long>(part) : reinterpret_cast<unsigned long long>(out);
-      store_rows<T, D>(o_at, mine, out_by, out_whole);
+      store_rows<T, D>(o_at, reinterpret_cast<unsigned long long>(part), reinterpret_cast<unsigned long long>(out), out_by, out_keep, out_how);
     };
-    segments([&](const PromptItem& w, int lo, int hi, bool whole, bool opens, int before) {
+    float factor = 0.0f;                             // what the row's scores are multiplied by
+    runs([&](const PromptItem& w, const Run& run) {
+      const int lo = run.lo, hi = run.hi, before = run.before;
       const int row = w.tile * SH::ROWS + tile * 128 + line;
       const bool real = row < w.s.nq * a.each;
       const int j = real ? row / a.each : 0, head = w.head * a.each + (real ? row - j * a.each : 0);
       const int hi_key = real ? w.s.len - w.s.nq + j : -1, from = a.window ? (int)max((long long)w.s.len - w.s.nq + j - a.window + 1, 0LL) : 0;
       const int n_end = before + hi - lo;
-      float factor = 0.0f, m = kLowest;
+      float m = kLowest;
       Two l(0.0f);
-      if (hi > lo) {
+      if (hi > lo && run.first) {
         const T* const src = real ? reinterpret_cast<const T*>(a.q) + (long long)(w.s.q0 + j) * a.q_token + (long long)head * a.q_head : nullptr;
         factor = load_queries<T, D>(src, smem + tile * (BLOCKS * 128 * 128) + quarter * 32 * 128, a.scale);
         fence_proxy_async();
@@ -658,6 +708,11 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
         if (lane == 0) mbar_arrive(bar(kQReady + tile));
       }
       flush();
+      out = nullptr;                                 // none of it is held while the chunks need the registers
+      part = nullptr;
+      out_by = out_keep = 0.0f;
+      out_n = -1;
+      out_how = kResult;
       bool s_ready = false;
       for (int n = before; n < n_end; ++n) {
         if (!s_ready) guarded(bar(kSFull + 2 * tile + (n & 1)), n >> 1 & 1);
@@ -749,18 +804,25 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
         if (lane == 0) mbar_arrive(bar(kPReady + 2 * tile + (n & 1)));
       }
       const float2 sums = l.both();
-      const float weight = sums.x + sums.y;
-      const long long slot_row = (long long)(2 * blockIdx.x + (opens ? 1 : 0)) * SH::ROWS + tile * 128 + line;
+      // Parts stand relative to the first run's maximum, or to a later one's that is above it by 2^8; less 2^15, so that they are no larger than sums of
+      // values.  A whole item of several runs is summed where the part of an item that ends in another CTA will stand.
+      const long long slot_row = (long long)(2 * blockIdx.x + (run.opens ? 1 : 0)) * SH::ROWS + tile * 128 + line;
+      const float2 past = run.first || !real ? make_float2(kLowest, 0.0f) : a.part_ml[slot_row];
+      const bool moves = past.x == kLowest || m > past.x + 8.0f;
+      const float top = moves ? fmaxf(past.x, m) : past.x, keep = past.x == top ? 1.0f : exp2_fast(past.x - top);
+      const float by = (m == top ? 1.0f : exp2_fast(m - top)) * 0x1p-15f, weight = fmaf(past.y, keep, (sums.x + sums.y) * by);
       T* const row_out = real ? reinterpret_cast<T*>(a.out) + ((long long)(w.s.q0 + j) * a.q_heads + head) * D : nullptr;
-      if (!whole && real) a.part_ml[slot_row] = make_float2(m, weight);
+      if (!(run.whole && run.last) && real) a.part_ml[slot_row] = make_float2(top, weight);
       if (hi > lo) {
-        const float scale = s_scale[(n_end - 1) % kRing];
+        const float scale = s_scale[(n_end - 1) % kRing] * by;
         out_n = n_end - 1;
-        out_whole = whole;
-        out = whole ? row_out : nullptr;
-        part = whole || !real ? nullptr : a.part_o + slot_row * D;
-        out_by = !whole ? scale : weight == 0.0f ? 0.0f : scale / weight;
-      } else if (whole && real) {                    // no keys at all
+        out = row_out;
+        part = real ? a.part_o + slot_row * D : nullptr;
+        const bool result = run.whole && run.last, scaled = __any_sync(0xffffffffu, keep != 1.0f);
+        out_how = run.first ? (result ? kResult : kPart) : result ? kSum : scaled ? kScaled : kAdded;
+        out_by = !result ? scale : weight == 0.0f ? 0.0f : scale / weight;
+        out_keep = !result ? keep : weight == 0.0f ? 0.0f : keep / weight;
+      } else if (run.whole && real) {                // no keys at all
         for (int c = 0; c < D / 8; ++c) reinterpret_cast<uint4*>(row_out)[c] = make_uint4(0, 0, 0, 0);
       }
     });

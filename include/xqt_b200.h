@@ -481,7 +481,8 @@ int xqt_b200_kv4_gather(const void* codes, const void* params, const void* slots
  * sees nothing is 0; lengths and starts are clamped to the table and to `tokens`; rows of no sequence are not written.
  * The work list -- row tiles times key heads times chunks of the keys that the table holds -- has fewer than 2^31 entries, more are refused.
  * strides (host): token and head stride of q in elements (multiples of 8), row stride of
- * table.  Workspace of the given size, 16-byte aligned, any contents, not shared with a call that may overlap. */
+ * table.  Workspace of the given size, 16-byte aligned, any contents, not shared with a call that may overlap.  status: null, or a word that the
+ * device can write (pinned host memory, say): 1 when a bounded wait ran out, after which the result is not valid. */
 size_t xqt_b200_kv4_attention_workspace_bytes(int tokens, int batch, int q_heads, int kv_heads, int dim,
                                               int has_query_starts);
 int xqt_b200_kv4_attention(const void* q, const void* codes, const void* params, const int* table, const int* seq_lens,

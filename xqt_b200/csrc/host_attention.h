@@ -14,7 +14,7 @@ decltype(&xqt_b200_kv4_gather) gather_entry = nullptr;
 decltype(&xqt_b200_kv4_attention) attention_entry = nullptr;
 decltype(&xqt_b200_kv4_attention_workspace_bytes) workspace_entry = nullptr;
 PyObject* on_error = nullptr;          // called with (code, symbol): raises
-unsigned int* status_words[64] = {};   // per device, null until the Python side has made it
+const unsigned int volatile* status_words[64] = {};   // per device, in pinned host memory; null until the Python side has made it
 
 struct NotServed {};
 
@@ -222,7 +222,7 @@ PyObject* kv4_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor &q = tensor(args[0]), &codes = tensor(args[1]), &params = tensor(args[2]), &table = tensor(args[3]), &lens = tensor(args[4]);
     const at::Tensor *starts = maybe(args[5]), *given = maybe(args[8]);
     const Cache c = cache(codes, params);
-    need(c.device < 64 && status_words[c.device] != nullptr);
+    need(c.device < 64 && status_words[c.device] != nullptr && *status_words[c.device] == 0);      // (an earlier call's wait ran out: the Python function raises)
     on(q, c.device);
     need(q.dim() == 3 && q.scalar_type() == c.type && q.size(2) == c.dim);
     const int tokens = small(q.size(0)), q_heads = small(q.size(1));
@@ -271,7 +271,7 @@ PyObject* kv4_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       const WithoutGil released;
       code = attention_entry(q.data_ptr(), codes.data_ptr(), params.data_ptr(), static_cast<const int*>(table.data_ptr()), static_cast<const int*>(lens.data_ptr()),
                              starts ? static_cast<const int*>(starts->data_ptr()) : nullptr, out.data_ptr(), strides, tokens, batch, q_heads, c.heads, c.dim, c.pages,
-                             c.page_size, width, (int)window, code_of(c.type), (float)scale, workspace.data_ptr(), bytes, status_words[c.device], stream);
+                             c.page_size, width, (int)window, code_of(c.type), (float)scale, workspace.data_ptr(), bytes, const_cast<unsigned int*>(status_words[c.device]), stream);
     }
     if (failed(code, "xqt_b200_kv4_attention")) return nullptr;
     if (given != nullptr) {
@@ -297,12 +297,12 @@ PyObject* set_entries(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
-// set_status_word(device, address): of a tensor that lives as long as the process
+// set_status_word(device, address): of a pinned tensor that lives as long as the process
 PyObject* set_status_word(PyObject*, PyObject* args) {
   int device;
   unsigned long long at;
   if (!PyArg_ParseTuple(args, "iK", &device, &at)) return nullptr;
-  if (device >= 0 && device < 64) status_words[device] = reinterpret_cast<unsigned int*>(at);
+  if (device >= 0 && device < 64) status_words[device] = reinterpret_cast<const unsigned int volatile*>(at);
   Py_RETURN_NONE;
 }
 

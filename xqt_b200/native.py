@@ -17,7 +17,7 @@ import threading
 
 import torch
 
-from .errors import CudaCallError, NativeLibraryError
+from .errors import CudaCallError, NativeLibraryError, XQTBackendError
 
 LIBRARY_PATH = pathlib.Path(__file__).resolve().parent / "libxqt_b200.so"
 
@@ -232,22 +232,38 @@ def status_word(device: torch.device) -> torch.Tensor:
     if word is None:
         word = torch.zeros(64, dtype=torch.int32, device=torch.device("cuda", index))
         _status_words[index] = word
-        host().set_status_word(index, word.data_ptr())
     return word
 
 
-def status_pointer(device: torch.device) -> int:
-    """Address of :func:`status_word`; 0 (no status) in a graph capture that finds none yet: what a capture allocates is its own, and not zeroed
-    before a replay."""
+# Per device, in pinned memory that kernels write and the host reads without a synchronisation: the attention kernels' status.
+_pinned_status: dict[int, torch.Tensor] = {}
+
+
+def pinned_status(device: torch.device) -> torch.Tensor:
+    """Word in pinned host memory (zero until a kernel's bounded wait runs out) that lives as long as the process, so that captured graphs may hold its
+    address; see :func:`check_waits`."""
 
     index = device.index if device.index is not None else torch.cuda.current_device()
-    if index not in _status_words and torch.cuda.is_current_stream_capturing():
-        return 0
-    return status_word(device).data_ptr()
+    word = _pinned_status.get(index)
+    if word is None:
+        word = torch.zeros(16, dtype=torch.int32, pin_memory=True)
+        host().set_status_word(index, word.data_ptr())
+        _pinned_status[index] = word
+    return word
+
+
+def check_waits(device: torch.device) -> None:
+    """Raise, once, if a kernel that has finished on ``device`` gave up a wait and reported it to :func:`pinned_status`."""
+
+    word = _pinned_status.get(device.index if device.index is not None else torch.cuda.current_device())
+    if word is not None and int(word[0]) != 0:
+        code = int(word[0])
+        word.zero_()
+        raise XQTBackendError(f"a wait inside an earlier attention kernel on {device} ran out (status {code}): the results since then are not valid")
 
 
 def workspace_status(device: torch.device) -> int:
-    """Worst status word of the current stream's scratch buffers and of the device's status word
+    """Worst status word of the current stream's scratch buffers and of the device's status words
     (0 = every bounded wait completed)."""
 
     index = device.index if device.index is not None else torch.cuda.current_device()
@@ -255,6 +271,10 @@ def workspace_status(device: torch.device) -> int:
     word = _status_words.get(index)
     if word is not None:
         worst = int(word[0].item()) & 0xFFFFFFFF
+    pinned = _pinned_status.get(index)
+    if pinned is not None:
+        torch.cuda.current_stream(device).synchronize()
+        worst = max(worst, int(pinned[0]) & 0xFFFFFFFF)
     for key, current in list(_workspaces.items()):
         if key[:2] != (index, stream_handle(device)):
             continue
@@ -268,5 +288,6 @@ def workspace_status(device: torch.device) -> int:
 
 __all__ = [
     "ACT", "AUTO_INTEGER", "BF16", "DTYPE_CODE", "FP16", "FP32", "LIBRARY_PATH", "SIGNATURES", "VARIANT", "VARIANT_NAMES",
-    "attention_host", "available", "check", "host", "library", "ptr", "status_pointer", "status_word", "stream_handle", "version", "workspace", "workspace_status",
+    "attention_host", "available", "check", "check_waits", "host", "library", "pinned_status", "ptr", "status_word", "stream_handle", "version", "workspace",
+    "workspace_status",
 ]

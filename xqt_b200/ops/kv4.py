@@ -122,7 +122,10 @@ def kv4_attention(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, bl
 
     Lengths stay on the device (the call can be captured in a CUDA graph and replayed with others); they are clamped to the table and to the rows
     of ``q``.  Rows of ``q`` that belong to no sequence are not written: in a new result they hold anything, in ``out`` (contiguous)
-    what they held."""
+    what they held.
+
+    Waits inside the kernels are bounded.  Should one run out, that call's result is wrong: the next call on the device raises (:func:`xqt_b200.native.check_waits`
+    does so without one, after a synchronisation or a graph's replay)."""
 
     global _native
     if _native is not None:
@@ -159,6 +162,7 @@ def kv4_attention(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, bl
         if not _rows16(q):
             q = q.clone(memory_format=torch.contiguous_format)
         library = native.library()
+        native.check_waits(device)
         with torch.cuda.device(device):
             need = library.xqt_b200_kv4_attention_workspace_bytes(tokens, batch, q_heads, kv_heads, dim, query_starts is not None)
             workspace = torch.empty(need, dtype=torch.uint8, device=device)      # the allocator's: each captured graph has its own
@@ -166,7 +170,7 @@ def kv4_attention(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, bl
                 q.data_ptr(), codes.data_ptr(), params.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), native.ptr(query_starts), out.data_ptr(),
                 _Strides(*_steps(q), block_table.stride(0), 0), tokens, batch, q_heads, kv_heads, dim, pages, page_size, width,
                 0 if window is None else min(int(window), 2 ** 31 - 1), native.DTYPE_CODE[q.dtype], scale, workspace.data_ptr(), need,
-                native.status_pointer(device), native.stream_handle(device))
+                native.pinned_status(device).data_ptr(), native.stream_handle(device))
         native.check(code, "xqt_b200_kv4_attention")
         _native = native.attention_host()
     return out

@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
-  // The CTA's part of the list: `body` gets an item and a run of its chunks.  Every role goes through it for itself.
+  // The CTA's part of the list: `body` gets an item and a run of its chunks.  Every role goes through it for itself.  Returns how many chunks there were.
   auto runs = [&](auto body) {
     PromptItem w = *s_start;
     unsigned left = s_range[1] - s_range[0];
@@ -442,8 +442,10 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
       left -= take;
       if (left > 0) prompt_next<SH>(a, w);
     }
+    return before;
   };
-  // every wait is bounded: when one runs out nothing waits any more, and the host is told
+  // Every wait is bounded: when one runs out, no role waits for another any more, and the host is told.  Who has copies or products in flight then waits for
+  // those, with a limit again, before the CTA gives its memory back.
   auto guarded = [&](uint32_t b, uint32_t parity) {
     if (*s_abort == 0u && !mbar_wait(b, parity)) {
       *s_abort = 1u;
@@ -469,6 +471,7 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
     if (a.status) *a.status = 1u;
   };
 
+  int mine = 0;                                      // warp 0: where its ring stands; issuers: their products
   if (warp == 0) {
     // ------------------------------------------------------------ codes and parameters into the raw ring
     const int psz = min(a.page_size, BN), pieces = BN / psz, groups = psz / 16;
@@ -495,17 +498,19 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
 #pragma unroll
         for (int p = 0; p < BN / 16; ++p) mask |= (votes >> (4 * (p / groups)) & 1u) << p;
         guarded(bar(kRawEmpty + stage), ring.phase ^ 1);
+        if (!__all_sync(0xffffffffu, *s_abort == 0u)) break;      // one answer for the warp: what is announced is copied, and the ring stands still
         if (lane == 0) {
           s_mask[(before + i - lo) % kRing] = mask;
           mbar_expect_tx(bar(kRawFull + stage), (uint32_t)(__popc(mask) * 16 * 2 * (D / 2 + 4)));
         }
         __syncwarp();
         const int at = w.begin + i * BN + piece * psz;
-        if (valid && *s_abort == 0u)
+        if (valid)
           bulk_g2s(target + stage * SH::RAW_BYTES, source + page * page_bytes + (long long)(at & (a.page_size - 1)) * row_bytes, (uint32_t)(psz * row_bytes), bar(kRawFull + stage));
         page = following;
       }
     });
+    mine = 2 * ring.slot + ring.phase;
   } else if (warp == 1 || (TILES == 2 && warp == 3)) {
     // ------------------------------------------------------------ the tensor core, for one row tile
     if (elect_one()) {
@@ -518,7 +523,7 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
       // scores run one chunk ahead; a buffer of theirs is free again behind the product that read P from it (the tensor core works in order)
       Ring<SH::STAGES> kr, vr;
       uint32_t q_phase = 0;
-      runs([&](const PromptItem&, const Run& run) {
+      mine = runs([&](const PromptItem&, const Run& run) {
         const int lo = run.lo, hi = run.hi, before = run.before;
         if (hi == lo) return;
         if (run.first) {
@@ -830,6 +835,15 @@ __global__ void __launch_bounds__(SH::THREADS, 1) kv4_prompt_kernel(const AttnAr
   }
   tc_fence_before();
   __syncthreads();
+  if (*s_abort != 0u) {                              // (here, behind all roles: inside them it moves their code, and the 8192-token prompt takes 676 us)
+    if (warp == 0) {                                 // (a stage that was never filled counts as done)
+      for (int s = 0; s < SH::STAGES; ++s) mbar_wait(bar(kRawFull + s), s < mine >> 1 ? mine & 1 : ~mine & 1);
+    } else if (mine > 0) {                           // the last product, and so those before it
+      mbar_spin(bar(kODone + 2 * (warp >> 1) + (mine - 1 & 1)), mine - 1 >> 1 & 1);
+    }
+    tc_fence_before();
+    __syncthreads();
+  }
   if (warp == 2) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);

@@ -478,7 +478,7 @@ int xqt_b200_kv4_gather(const void* codes, const void* params, const void* slots
  * query_starts[b] .. query_starts[b+1] (null: row b, tokens == batch), which are its last tokens, and seq_lens[b] keys, key i in
  * row i % page_size of page table[b][i / page_size] (table [batch, table_width], int32, row stride strides[2]).  A query sees the keys up
  * to its own position, with window > 0 only the last `window` of them; keys of a page number outside [0, pages) are not seen; a row that
- * sees nothing is 0; lengths and starts are clamped to the table and to `tokens`; rows of no sequence are not written.
+ * sees nothing is 0; |scale| < 2^127; lengths and starts are clamped to the table and to `tokens`; rows of no sequence are not written.
  * The work list -- row tiles times key heads times chunks of the keys that the table holds -- has fewer than 2^31 entries, more are refused.
  * strides (host): token and head stride of q in elements (multiples of 8), row stride of
  * table.  Workspace of the given size, 16-byte aligned, any contents, not shared with a call that may overlap.  status: null, or a word that the

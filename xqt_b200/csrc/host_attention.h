@@ -245,7 +245,7 @@ PyObject* kv4_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (args[6] != Py_None) {
       scale = PyFloat_AsDouble(args[6]);
       if (scale == -1.0 && PyErr_Occurred()) return nullptr;
-      need(std::isfinite(scale));
+      need(std::fabs(scale) < 0x1p127);              // (false for NaN)
     }
     long long window = 0;
     if (args[7] != Py_None) {

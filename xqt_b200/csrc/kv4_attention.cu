@@ -774,7 +774,7 @@ extern "C" int xqt_b200_kv4_attention(const void* q, const void* codes, const vo
   XQT_REQUIRE(dtype == XQT_B200_FP16 || dtype == XQT_B200_BF16);
   XQT_REQUIRE(page_size >= 16 && page_size <= 4096 && (page_size & (page_size - 1)) == 0);
   XQT_REQUIRE(pages >= 0 && pages < (1LL << 31) && table_width >= 0 && (long long)table_width * page_size <= (1LL << 30));
-  XQT_REQUIRE(window >= 0 && (long long)tokens * (q_heads / kv_heads) < (1LL << 31) - 4096);
+  XQT_REQUIRE(window >= 0 && fabsf(scale) < 0x1p127f && (long long)tokens * (q_heads / kv_heads) < (1LL << 31) - 4096);
   if (tokens == 0 || batch == 0) return 0;
   XQT_REQUIRE(q && out && seq_lens && strides && (table_width == 0 || table) && (pages == 0 || (codes && params)));
   XQT_REQUIRE((query_starts != nullptr) || tokens == batch);

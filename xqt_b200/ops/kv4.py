@@ -7,7 +7,6 @@ head), so a key of 128 channels takes 68 bytes where bf16 takes 256.  Layout: ``
 from __future__ import annotations
 
 import ctypes
-import math
 
 import torch
 
@@ -151,8 +150,8 @@ def kv4_attention(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, bl
     if window is not None and window < 1:
         raise XQTBackendError("kv4_attention: a window holds a key at least")
     scale = dim ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise XQTBackendError("kv4_attention: the scale is finite")
+    if not abs(scale) < 2.0 ** 127:          # the kernels hold scale * log2(e) in fp32
+        raise XQTBackendError("kv4_attention: the scale is finite and below 2^127")
     _on_gpu("kv4_attention", codes)
     if out is None:
         out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=device)

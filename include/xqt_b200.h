@@ -473,7 +473,8 @@ int xqt_b200_kv4_gather(const void* codes, const void* params, const void* slots
                         int heads, int dim, long long pages, int page_size, int wide_slots, int dtype,
                         xqt_b200_stream_t stream);
 
-/* Attention over that cache: out = softmax(scale * q K^T + mask) V, q and out [tokens, q_heads, dim] (out contiguous), q_heads a
+/* Attention over that cache: out = softmax(scale * q K^T + mask) V, q and out [tokens, q_heads, dim] (out contiguous; it may be q, but not
+ * overlap it otherwise), q_heads a
  * multiple of kv_heads (consecutive query heads share a key head).  Sequence b has the query rows
  * query_starts[b] .. query_starts[b+1] (null: row b, tokens == batch), which are its last tokens, and seq_lens[b] keys, key i in
  * row i % page_size of page table[b][i / page_size] (table [batch, table_width], int32, row stride strides[2]).  A query sees the keys up

@@ -21,3 +21,12 @@ def test_scales_beyond_fp32(scale):
     entry = lambda value, tokens: native.library().xqt_b200_kv4_attention(  # noqa: E731
         16, 16, 16, 16, 16, 0, 16, (ctypes.c_longlong * 4)(), tokens, 1, 1, 1, 64, 1, 16, 1, 0, 0, value, 0, 0, 0, 0)
     assert entry(scale, 0) == 1 and entry(-1.7e38, 0) == 0        # no tokens: nothing to launch
+
+
+def test_address_ranges():
+    from xqt_b200.ops.kv4 import _overlap
+
+    x = torch.empty(4 * 6 * 64)
+    y = x.view(4, 6, 64)
+    assert _overlap(y, y) and _overlap(y[:, :3], y[:, 3:]) and not _overlap(y[:2], y[2:]) and not _overlap(y[:1, :3], y[:1, 3:])
+    assert _overlap(y[:2], y[1:]) and not _overlap(y[:0], y) and not _overlap(y, torch.empty(1))

@@ -38,6 +38,15 @@ int small(int64_t v) {
   need(v >= 0 && v <= INT32_MAX);
   return (int)v;
 }
+// whether the address ranges that two tensors span meet (neither is empty)
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  auto end = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return reinterpret_cast<uintptr_t>(t.data_ptr()) + (uintptr_t)(last + 1) * t.element_size();
+  };
+  return reinterpret_cast<uintptr_t>(a.data_ptr()) < end(b) && reinterpret_cast<uintptr_t>(b.data_ptr()) < end(a);
+}
 // token and head stride of a [tokens, heads, dim] tensor whose channels are contiguous and start on 16 bytes
 void rows(const at::Tensor& t, long long* strides) {
   const int64_t token = t.size(0) > 1 ? t.stride(0) : 0, head = t.size(1) > 1 ? t.stride(1) : 0;
@@ -259,6 +268,7 @@ PyObject* kv4_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (given != nullptr) {
       on(*given, c.device);
       need(given->scalar_type() == c.type && given->sizes() == q.sizes() && given->is_contiguous() && aligned(*given));
+      need((given->data_ptr() == q.data_ptr() && q.is_contiguous()) || !overlap(q, *given));
       out = *given;
     } else {
       out = fresh({tokens, q_heads, c.dim}, c.type, c.device);

@@ -46,6 +46,16 @@ def _cache(what: str, codes: torch.Tensor, params: torch.Tensor) -> tuple[int, i
     return pages, heads, page_size, 2 * half
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges that two tensors span meet."""
+
+    def span(x: torch.Tensor) -> tuple[int, int]:
+        return x.data_ptr(), x.data_ptr() + (sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1) * x.element_size()
+
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a.numel() > 0 and b.numel() > 0 and a0 < b1 and b0 < a1
+
+
 def _on_gpu(what: str, codes: torch.Tensor) -> None:
     if not codes.is_cuda:
         raise XQTBackendError(f"{what} expects CUDA tensors")
@@ -121,7 +131,7 @@ def kv4_attention(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, bl
 
     Lengths stay on the device (the call can be captured in a CUDA graph and replayed with others); they are clamped to the table and to the rows
     of ``q``.  Rows of ``q`` that belong to no sequence are not written: in a new result they hold anything, in ``out`` (contiguous)
-    what they held.
+    what they held.  ``out`` may be ``q`` itself where that is contiguous, but may not overlap it otherwise.
 
     Waits inside the kernels are bounded.  Should one run out, that call's result is wrong: the next call on the device raises (:func:`xqt_b200.native.check_waits`
     does so without one, after a synchronisation or a graph's replay)."""
@@ -157,6 +167,8 @@ def kv4_attention(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, bl
         out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=device)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != device or not out.is_contiguous() or out.data_ptr() % 16:
         raise XQTBackendError("kv4_attention: out has the shape, type and device of the queries, contiguous and on 16 bytes")
+    elif _overlap(q, out) and not (q.data_ptr() == out.data_ptr() and q.is_contiguous()):
+        raise XQTBackendError("kv4_attention: out is the queries themselves (contiguous) or does not overlap them")
     if tokens and batch:
         if not _rows16(q):
             q = q.clone(memory_format=torch.contiguous_format)

@@ -105,3 +105,32 @@ def test_runs_of_keys_in_whole_and_in_shared_items(dtype, dim, keys, heads, wind
         again = kv4_attention(*call[:5], query_starts=call[5], window=window)
         assert torch.equal(again.view(torch.uint8), first.view(torch.uint8))
     assert native.workspace_status(DEVICE) == 0
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("counts,dtype,ratio", [([600, 300], torch.bfloat16, 24), ([600, 300], torch.float16, 12), ([7, 5], torch.bfloat16, 12), ([7, 5], torch.float16, 12)])
+def test_large_finite_vectors_that_a_row_does_not_see(dim, counts, dtype, ratio):
+    """Later keys and values 2^ratio times as large as their neighbours, in the same chunks: rows before them are as exact as without."""
+    from test_kv4_gpu import _vectors, make_cache, wide
+
+    lens = [600, 900]
+    codes, params, table = make_cache(lens, 2, dim, 64, dtype, 83)
+    large = {0: [595, 598, 599], 1: [897, 899]}
+    for b, keys in large.items():
+        for key in keys:
+            params[int(table[b, key // 64]), :, :, key % 64] *= 2.0 ** ratio
+    assert bool(torch.isfinite(params[int(table[0, 9]), :, :, :24]).all())
+    q = _vectors(sum(counts), 8, dim, dtype, 84).to(DEVICE)
+    seq_lens, starts = torch.tensor(lens, dtype=torch.int32), torch.tensor([0, counts[0], sum(counts)], dtype=torch.int32)
+    got = kv4_attention(q, codes, params, wide(table, 64), seq_lens.to(DEVICE), query_starts=starts.to(DEVICE)).double()
+    want, bound = attention(q, codes, params, table, seq_lens, starts, rounded=torch.float16 if max(counts) > 32 else None)
+    clear = torch.tensor([lens[b] - counts[b] + i < large[b][0] for b in (0, 1) for i in range(counts[b])], device=DEVICE)
+    # the bound takes a sequence's largest key for all of its rows: the rows before it get theirs from a cache without the large ones
+    plain = params.clone()
+    for b, keys in large.items():
+        for key in keys:
+            plain[int(table[b, key // 64]), :, :, key % 64] *= 2.0 ** -ratio
+    same, bound = attention(q, codes, plain, table, seq_lens, starts, rounded=torch.float16 if max(counts) > 32 else None)
+    assert bool(clear.any()) and not bool(clear.all()) and torch.equal(want[clear], same[clear])
+    over = (got - same).abs()[clear] - bound[clear]
+    assert bool((over <= 0).all()), f"{float(over.max())} over a bound of {float(bound[clear].max())}"

@@ -133,6 +133,11 @@ def kv4_attention(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, bl
     of ``q``.  Rows of ``q`` that belong to no sequence are not written: in a new result they hold anything, in ``out`` (contiguous)
     what they held.  ``out`` may be ``q`` itself where that is contiguous, but may not overlap it otherwise.
 
+    The products take fp16 operands under powers of two that neighbours share, also those that a row does not see: in prompts an element of a key keeps its
+    precision down to 2^-28 of the largest in its 64 keys, an element of a value down to 2^-28 of the largest in the (up to 16,384) keys up to
+    its chunk's end, and counts as 0 below 2^-39; for few queries a probability times the scale of its value does so down to 2^-29 and below 2^-40 of the
+    largest such scale so far.  Scores and what they are summed from stay below 2^100.
+
     Waits inside the kernels are bounded.  Should one run out, that call's result is wrong: the next call on the device raises (:func:`xqt_b200.native.check_waits`
     does so without one, after a synchronisation or a graph's replay)."""
 

@@ -445,7 +445,7 @@ int xqt_b200_swiglu(const void* gate_up, void* output, int m, int inter, int dty
 /* RMS norm of query and key heads and the position rotation in one pass (no counterpart in the reference):
  *   y = x * rsqrt(mean(x^2) + eps) * weight   where the weight is given (fp16 / bf16 / fp32 [dim]; null: y = x), then pair j of the
  *   first `rotary` channels -- (j, j + rotary/2), interleaved: (2j, 2j+1) -- turned by positions[axes[j]][token] * frequencies[j]
- *   radians; fp32 arithmetic, one rounding, the angle exact modulo a turn at any position.
+ * radians; fp32 arithmetic, one rounding; the angle is off by at most 2^-53 * |position| turns besides (frequencies up to 2 pi).
  * q [tokens, q_heads, dim], k [tokens, k_heads, dim] (k_heads 0: none) and their outputs with strides; an output may be its input.
  * strides (host): token and head stride in elements of q, q_out, k, k_out (8 values, multiples of 8), then axis and token
  * stride of positions.  positions: [axis_count, tokens] of int64 (wide_positions) or int32; frequencies: [rotary/2], device memory,

@@ -8,8 +8,9 @@
 // Neither K nor V is ever formed.  The matrix instructions (mma.sync m16n8k16, fp16 operands, fp32 sums) run on the codes themselves: a
 // nibble in the low bits of a half is the subnormal c * 2^-24, so one AND per two codes makes an operand, and
 //   q . K_t = s_t * sum(c q) + m_t * sum(q)          P V = sum((p_t s_t) c) + sum(p_t m_t)
-// puts scales and minima on the scores and on the probabilities.  Queries are scaled by a power of two per row so that fp16 holds them
-// to 2^-12 of each element down to 2^-26 of the row's largest; p_t s_t is rounded to fp16 against a running power of two above the scales, with
+// puts scales and minima on the scores and on the probabilities.  Queries are scaled by a power of two per row so that fp16 holds
+// them exactly down to 2^-26 of the row's largest (2^-22 in the odd channels, whose operand is 16 times smaller; the sum that goes with m is taken
+// before that); p_t s_t is rounded to fp16 against a running power of two above the scales, with
 // 2^15 of headroom, so nothing underflows; softmax statistics and all sums are fp32.
 //
 // The keys are the 16-row operand and the queries the 8-column one (transposed products), so that eight rows -- the query heads of

@@ -4,8 +4,9 @@
 //   pair j of the first `rotary` channels -- (j, j + rotary/2), or (2j, 2j+1) where they are interleaved -- turns by
 //   position[axis_j, token] * frequency_j; the other channels pass.  fp32 arithmetic, one rounding.
 //
-// The angle is kept as a 64-bit fixed-point fraction of a turn: position * fraction wraps exactly modulo one turn, so a far
-// position loses nothing (fp32 angles are off by 2^-24 of the angle itself: 0.006 rad at position 100,000).
+// The angle is kept as a 64-bit fixed-point fraction of a turn: position * fraction wraps exactly modulo one turn.  What is left is the rounding of
+// frequency / (2 pi) to 64-bit floating point, at most 2^-53 * |position| turns (for frequencies up to a turn per position): below the fp32 of sine and cosine for every 32-bit position (fp32
+// angles are off by 2^-24 of the angle itself: 0.006 rad at position 100,000).
 //
 // Bound by HBM: every channel is read and written once.  A block makes the cosines of up to 16 tokens in shared memory, then its lane groups go
 // through the heads of those tokens: dim / 16 lanes (padded to a power of two) hold one head, 16 channels a lane, chosen so that both

@@ -85,8 +85,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     ``x * rsqrt(mean(x^2) + eps) * weight``; without one that side is not normed.  ``positions`` int32 / int64 ``[tokens]`` or ``[axes, tokens]``;
     ``frequencies`` float64 ``[pairs]``, radians per position of each pair of channels (a multiple of 8 pairs, none: no rotation); ``axes`` int32
     ``[pairs]``, the axis that each pair follows (None: axis 0; numbers outside are clamped).  Pair ``j`` is channels ``(j, j + pairs)``, or
-    ``(2j, 2j + 1)`` with ``interleaved``; channels from ``2 * pairs`` on are not turned.  fp32 arithmetic, rounded once; angles are exact modulo a
-    turn at any position.
+    ``(2j, 2j + 1)`` with ``interleaved``; channels from ``2 * pairs`` on are not turned.  fp32 arithmetic, rounded once; angles are
+    off by at most 2^-53 of a turn per position besides (1.5e-6 radians at position 2^31).
 
     ``out = (q_out, k_out)``: written instead of new tensors; either may be the input itself (in place), but may not overlap an input otherwise."""
 

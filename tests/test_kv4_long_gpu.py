@@ -134,3 +134,28 @@ def test_large_finite_vectors_that_a_row_does_not_see(dim, counts, dtype, ratio)
     assert bool(clear.any()) and not bool(clear.all()) and torch.equal(want[clear], same[clear])
     over = (got - same).abs()[clear] - bound[clear]
     assert bool((over <= 0).all()), f"{float(over.max())} over a bound of {float(bound[clear].max())}"
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_million_keys_beside_a_strong_one_for_single_tokens(dtype):
+    """Single tokens: 2^20 keys at 2^-24 of one whose values are half of theirs, in items of one CTA: sums to which each weak key adds half of their last bit."""
+    keys, dim, each = 1 << 20, 64, 4
+    heads = 2 * torch.cuda.get_device_properties(0).multi_processor_count
+    gen = torch.Generator(device=DEVICE).manual_seed(85)
+    codes = torch.randint(0, 256, (65, 2, heads, PAGE, dim // 2), dtype=torch.uint8, device=DEVICE, generator=gen)
+    params = torch.empty((65, 2, heads, PAGE, 2), dtype=dtype, device=DEVICE)
+    params[:, 0, ..., 0], params[:, 0, ..., 1] = 2.0 ** -6, -7.5 * 2.0 ** -6
+    params[:, 1, ..., 0], params[:, 1, ..., 1] = 1 / 16, 2 - 7.5 / 16
+    codes[64, 0, :, 0], params[64, 0, :, 0, 0], params[64, 0, :, 0, 1] = 0x0F, 1 / 15, 0.0       # 1 in the even channels
+    codes[64, 1, :, 0], params[64, 1, :, 0, 0], params[64, 1, :, 0, 1] = 0, 1.0, 1.0
+    q = torch.zeros((1, heads * each, dim))
+    q[..., 0::2] = 24 * math.log(2) / (dim // 2)
+    q = q.to(dtype).to(DEVICE)
+    table = (torch.arange(keys // PAGE, dtype=torch.int32) % 64).reshape(1, -1)
+    table[0, 0] = 64
+    lens = torch.tensor([keys], dtype=torch.int32)
+    got = kv4_attention(q, codes, params, table.to(DEVICE), lens.to(DEVICE), scale=1.0)[:, :2 * each].double()
+    want, bound = attention(q[:, :2 * each], codes[:, :, :2], params[:, :, :2], table, lens, scale=1.0)
+    assert bool((bound < 2 * torch.finfo(dtype).eps / 2 * want.abs()).all())
+    worst = float(((got - want).abs() / bound).max())
+    assert worst <= 1, f"{worst} bounds"

@@ -413,6 +413,7 @@ __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(c
     uint32_t pf[MT][NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      Two of_chunk(0.0f), of_minima(0.0f);           // (keys one by one would be lost beside a strong one in a sum of a million; same time)
       const Two minus(mx[nt][0] == -CUDART_INF_F ? 0.0f : -mx[nt][0], mx[nt][1] == -CUDART_INF_F ? 0.0f : -mx[nt][1]);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
@@ -420,10 +421,10 @@ __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(c
         for (int e = 0; e < 2; ++e) {
           const float2 x = (Two(p[mt][nt][2 * e], p[mt][nt][2 * e + 1]) + minus).both();
           const Two pr(exp2_fast(x.x), exp2_fast(x.y));
-          l[nt] = l[nt] + pr;
+          of_chunk = of_chunk + pr;
           const float2 sv = pair_of<T>(vb[mt][e]);
           const Two w2 = pr * Two(sv.x * inv_sigma);
-          lm[nt] = fma2(pr, Two(sv.y), lm[nt]);
+          of_minima = fma2(pr, Two(sv.y), of_minima);
           const float2 w = w2.both();
           const uint32_t h = pack_half2(w.x, w.y);
           if constexpr (KEEP_ROUNDING) {
@@ -432,6 +433,8 @@ __global__ void __launch_bounds__(SH::W * 32, SH::PER_SM) kv4_attention_kernel(c
           }
           pf[mt][nt][e] = transpose8x8(h);
         }
+      l[nt] = l[nt] + of_chunk;
+      lm[nt] = lm[nt] + of_minima;
     }
     const uint8_t* const vs = st + SH::CODE_BYTES + g * (4 * VWORDS);
     const int x0 = 2 * t ^ (t & 1), y0 = x0 ^ 1;

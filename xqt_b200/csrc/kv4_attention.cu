@@ -717,7 +717,8 @@ int run(AttnArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream
   XQT_REQUIRE(items < (1LL << 31) - 1 && units < (1LL << 31));
   // Few items with few keys: a cluster for each, which needs neither the list nor the second kernel (cluster | list: one sequence of 777 keys 6.6 |
   // 9.0 us, 64 of 500 18 | 21).  Where items of many keys do not fill the SMs, or there are many items, the list's even shares win (two of 131,071
-  // keys, eight heads: 125 | 70; 64 up to 8192: 95 | 82).
+  // keys, eight heads: 125 | 70; 64 up to 8192: 95 | 82).  Keys are what the table has room for: one sequence of 777 keys behind a table of 131,072 takes
+  // the list and 9.2 us.
   const long long keys = (long long)a.table_width << a.page_shift, seen = a.window ? min(keys, (long long)a.window + min(most_rows / a.each, (long long)a.tokens) + SH::CT) : keys;
   const long long of_item = (seen + SH::UNIT - 1) / SH::UNIT;
   // A cluster's size goes by the items of queries dealt out evenly and by what is resident together.  What the grid has over those items finds
@@ -809,6 +810,7 @@ extern "C" int xqt_b200_kv4_attention(const void* q, const void* codes, const vo
   // Sequences with more than kFewRows rows go to the prompt kernel, whose tiles of 128 or 256 rows run at half of the tensor core's rate where they are full, unless the whole call is so little work that its two launches more are not worth it (keys: as
   // many as the table holds).  Both sides measured, this kernel for all | prompt kernel above 32 rows: one sequence, 40 queries of 32 heads on 2000
   // keys 25 | 33 us, 64 queries 31 | 36, 16 queries on 30,000 keys 62 | 66; 64 sequences of 16 queries on 2000 keys 332 | 275, of 9 queries 249 | 273.
+  // All with tables that fit; behind one of 131,072 keys the rule takes the second side (40 queries on 2000 keys: 31 us instead of 24).
   a.few_rows = INT_MAX;
   if (query_starts != nullptr && (long long)tokens * a.each > kFewRows &&
       (double)tokens * q_heads * table_width * page_size * dim > 768e6) {

@@ -38,10 +38,10 @@
 // The order of a word's codes: pairs (0,4) (1,5) (2,6) (3,7) come out of one AND each, so channels stand in shared memory as 0 4 1 5 2 6 3 7 in
 // every group of eight; queries are stored in the same order, and the result is put back when it is written.
 //
-// Bound by the tensor core and by ex2 (16 a clock and SM), which take the same time for 128 channels; what is left between that and the measured
-// time is the chain scores -> softmax -> P -> product, of which two tiles overlap, and what an item costs before and after its chunks.
-// Measured: 629 us for the prompt of 8192 tokens (32 heads on 8 of 128 channels: 874 TFLOP/s, half of a library GEMM's rate), 468 us for chunks of
-// four prompts, 8188 queries of 40 heads on 8 in all (770 TFLOP/s).
+// Bound by shared memory (operands 42 % of the clocks for 128 channels in bf16, the warps' own accesses 23 %), the tensor core and ex2 (16 a clock and SM),
+// 41 % each; what is left between that and the measured time is the chain scores -> softmax -> P -> product, of which two tiles overlap, and what an item costs before and after its chunks.
+// Measured: 629 us for the prompt of 8192 tokens (32 heads on 8 of 128 channels: 874 TFLOP/s, half of a library GEMM's rate), 474 us for chunks of
+// four prompts, 8188 queries of 40 heads on 8 in all (760 TFLOP/s).
 #include <type_traits>
 
 #include "kv4_attention.cuh"

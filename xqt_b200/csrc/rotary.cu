@@ -11,8 +11,8 @@
 // Bound by HBM: every channel is read and written once.  A block makes the cosines of up to 16 tokens in shared memory, then its lane groups go
 // through the heads of those tokens: dim / 16 lanes (padded to a power of two) hold one head, 16 channels a lane, chosen so that both
 // channels of a pair are in one lane.  Sums of squares, products and turns are packed fp32 instructions: with single ones the kernel waited on issue.
-// Measured, heads of 128 channels: 8191 tokens of 32 + 8 heads 31 us (5.4 TB/s), 32,760 tokens of 20 + 20 heads on three axes 120 us (5.6 TB/s;
-// a copy reaches 6.6); a call of one token 3.1 us, which is its launch and one chain load -> sum -> store.
+// Measured, heads of 128 channels: 8191 tokens of 32 + 8 heads 31 us (5.4 TB/s), 32,760 tokens of 20 + 20 heads on three axes 120 us (5.6 TB/s,
+// a copy reaches 6.6; 131 us where the inputs change from call to call); a call of one token 3.1 us, which is its launch and one chain load -> sum -> store.
 #include "pairs.cuh"
 
 namespace xqt_b200 {

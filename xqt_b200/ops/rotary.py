@@ -88,7 +88,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     ``(2j, 2j + 1)`` with ``interleaved``; channels from ``2 * pairs`` on are not turned.  fp32 arithmetic, rounded once; angles are
     off by at most 2^-53 of a turn per position besides (1.5e-6 radians at position 2^31).
 
-    ``out = (q_out, k_out)``: written instead of new tensors; either may be the input itself (in place), but may not overlap an input otherwise."""
+    ``out = (q_out, k_out)``: written instead of new tensors; either may be the input itself (in place), but may not overlap an input otherwise, nor may
+    they overlap each other."""
 
     global _native
     if _native is not None and out is None:
@@ -140,6 +141,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
             if given is not None and (given.dtype != dtype or given.device != device or given.shape != x.shape or not _rows16(given)
                                       or not _dense(given.shape, given.stride())):
                 _bad("an output has its input's shape, type and device, contiguous channels on 16 bytes, and no shared addresses")
+        if tokens and k is not None:
+            for a, b in ((q_out, k_out), (q_out, k), (k_out, q)):
+                if a.data_ptr() == b.data_ptr():
+                    _bad("the outputs do not overlap each other or the other one's input")
     if tokens:
         if not _rows16(q):
             q = q.clone(memory_format=torch.contiguous_format)
